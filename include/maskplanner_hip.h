@@ -590,6 +590,25 @@ int mp_lambda_segments_f32(const float* poses, const float* stroke_ids, const in
                            int64_t lambda, int64_t overlapping, int64_t R, float* out_traj, float* out_ids, int32_t* status,
                            mp_stream_t stream);
 
+/* ---- layer normalisation over the last axis ---------------------------------------------------------------------------------
+ *   mean_r = sum_j x_rj / cols;  rstd_r = 1 / sqrt(sum_j (x_rj - mean_r)^2 / cols + eps);  y = weight * (x - mean) * rstd + bias
+ *   x [rows, cols], rows x_row_stride elements apart (>= 0; a row itself is contiguous), y [rows, cols] contiguous, both of `dtype`; weight /
+ *   bias [cols] of `param_dtype` (MP_DTYPE_F32, or dtype itself) or NULL (1 / 0).  mean / rstd [rows] f32: both (for the backward pass) or
+ *   both NULL.  Arithmetic in fp32, one rounding at the end.  rows, cols < 2^31. */
+#define MP_DTYPE_F32 0
+#define MP_DTYPE_F16 1
+#define MP_DTYPE_BF16 2
+int mp_layer_norm_fwd(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_row_stride, const void* weight, const void* bias,
+                      int param_dtype, double eps, void* y, float* mean, float* rstd, mp_stream_t stream);
+/* With g = weight * dy and z = (x - mean) * rstd:  dx = rstd * (g - mean_j(g) - z * mean_j(g * z)),  dweight = sum_r dy * z,  dbias = sum_r dy.
+ *   dx [rows, cols] contiguous of `dtype`, dweight / dbias [cols] of `param_dtype`; each may be NULL (not wanted).  workspace:
+ *   mp_layer_norm_bwd_workspace_bytes bytes when dweight or dbias is wanted.  Sums in a fixed order: bitwise reproducible.  rows = 0 writes
+ *   zeros to dweight / dbias. */
+size_t mp_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols, int dtype);
+int mp_layer_norm_bwd(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, int dtype, int64_t rows, int64_t cols,
+                      const void* weight, int param_dtype, const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                      void* workspace, size_t workspace_bytes, mp_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -955,3 +955,91 @@ def bn_relu_rows(x, bn, dropout=None):
         RELU_TAP.append(y.detach() > 0)
     return y
 
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# layer normalisation
+# ----------------------------------------------------------------------------------------------------------------
+_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # include/maskplanner_hip.h MP_DTYPE_*
+
+
+def _rows_of(x):
+    """x [..., D] as rows of contiguous elements at one stride: (tensor, row stride).  A view where the layout allows it, else a copy."""
+    D = x.shape[-1]
+    if x.ndim != 2:
+        x = x.reshape(-1, D)
+    if D > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x, x.stride(0)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        D = x.shape[-1]
+        x2, xs = _rows_of(x)
+        rows = x2.shape[0]
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        wanted = any(ctx.needs_input_grad)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if wanted else None
+        like = weight if weight is not None else bias
+        wt = _DTYPE[like.dtype if like is not None else x.dtype]
+        mean = stats.data_ptr() if wanted and rows else None
+        _run("layer_norm", x, _lib.load().mp_layer_norm_fwd, x2.data_ptr(), _DTYPE[x.dtype], rows, D, xs, _p(weight), _p(bias), wt, eps,
+             y.data_ptr(), mean, mean + 4 * rows if mean else None)
+        if wanted:
+            ctx.save_for_backward(x, weight, stats)
+            ctx.wt = wt
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        # once_differentiable's wrapper costs 4-5 us of the ~60 us host time of a small call: only where a second derivative can be asked for
+        return (_LayerNorm._backward_once if torch.is_grad_enabled() else _LayerNorm._backward)(ctx, grad_y)
+
+    @staticmethod
+    def _backward(ctx, grad_y):
+        x, weight, stats = ctx.saved_tensors
+        D = x.shape[-1]
+        x2, xs = _rows_of(x)
+        dy, dys = _rows_of(grad_y if grad_y.dtype == x.dtype else grad_y.to(x.dtype))
+        rows = x2.shape[0]
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        wdtype = (torch.float32, torch.float16, torch.bfloat16)[ctx.wt]
+        gw = torch.empty((D,), dtype=wdtype, device=x.device) if need_w else None
+        gb = torch.empty((D,), dtype=wdtype, device=x.device) if need_b else None
+        lib, dt = _lib.load(), _DTYPE[x.dtype]
+        nbytes = lib.mp_layer_norm_bwd_workspace_bytes(rows, D, dt) if (need_w or need_b) else 0
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
+        mean = stats.data_ptr()
+        _run("layer_norm_bwd", x, lib.mp_layer_norm_bwd, dy.data_ptr(), dys, x2.data_ptr(), xs, dt, rows, D, _p(weight), ctx.wt, mean,
+             mean + 4 * rows, _p(gx), _p(gw), _p(gb), _p(ws), nbytes)
+        return gx, gw, gb, None
+
+    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer normalisation of x [..., D] over its last axis: weight * (x - mean) / sqrt(var + eps) + bias, one launch forward; backward the
+    gradients of x, weight and bias (two launches, fixed summation order).  x float32, float16 or bfloat16; weight / bias [D] in float32 or
+    x's type, both of one type, or None.  Any leading shape, also none or an empty one; rows may be strided (a view with another element
+    stride is copied).  Arithmetic in fp32, rounded once to x's type.  Not differentiable twice."""
+    _need_hip(x, weight, bias)
+    if x.ndim == 0 or x.shape[-1] < 1:
+        raise ValueError("layer_norm expects [..., D] input with D >= 1")
+    if x.dtype not in _DTYPE:
+        raise ValueError(f"layer_norm takes float32, float16 or bfloat16 input, not {x.dtype}")
+    like = weight if weight is not None else bias
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != x.shape[-1:]:
+            raise ValueError(f"layer_norm: {name} must have shape ({x.shape[-1]},), not {tuple(t.shape)}")
+        if t.dtype != like.dtype or t.dtype not in (torch.float32, x.dtype):
+            raise ValueError("layer_norm: weight and bias are float32 or of the input's type, both of one type")
+        if t.device != x.device:
+            raise ValueError(f"layer_norm: {name} is on {t.device}, the input on {x.device}")
+    if not eps >= 0:
+        raise ValueError("layer_norm: eps must not be negative")
+    return _LayerNorm.apply(x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), float(eps))
