@@ -156,6 +156,9 @@ SIGNATURES = {
                                  _sz, _vp]),
     "mp_sa_mlp_bwd_bf16": (_int, [_vp, _i64, _i64, _int, ctypes.POINTER(MlpLayer), _int, _vp, _vp, _vp, _vp,
                                  ctypes.POINTER(MlpGrads), _vp, _i64, _vp, _sz, _vp]),
+    "mp_orthogonalize_workspace_bytes": (_sz, [_i64, _vp, _vp, _int, _int]),
+    "mp_orthogonalize": (_int, [_i64, _vp, _vp, _vp, _vp, _int, _int, _vp, _dbl, _vp, _sz, _vp]),
+    "mp_muon_step": (_int, [_i64, _vp, _vp, _vp, _vp, _vp, _int, _dbl, _dbl, _int, _dbl, _int, _int, _vp, _dbl, _vp, _sz, _vp]),
     "mp_layer_norm_fwd": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _int, _dbl, _vp, _vp, _vp, _vp]),
     "mp_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64, _int]),
     "mp_layer_norm_bwd": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

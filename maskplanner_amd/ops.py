@@ -1043,3 +1043,112 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if not eps >= 0:
         raise ValueError("layer_norm: eps must not be negative")
     return _LayerNorm.apply(x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), float(eps))
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Newton-Schulz orthogonalisation, Muon update
+# ----------------------------------------------------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+MUON_SCALES = {None: 0, "original": 1, "match_rms": 2}
+
+
+def _ptrs(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _ns_setup(op, mats, steps, coefficients, eps):
+    """Common checks of the list calls -> (dtype code, rows, cols, coefficients, workspace, its size)."""
+    first = mats[0]
+    if first.dtype not in _DTYPE:
+        raise ValueError(f"{op} takes float32, float16 or bfloat16 matrices, not {first.dtype}")
+    for t in mats:
+        if t.dtype != first.dtype or t.device != first.device:
+            raise ValueError(f"{op}: all matrices of a call have one type and one device")
+    coefficients = tuple(float(c) for c in coefficients)
+    if len(coefficients) != 3:
+        raise ValueError(f"{op}: three coefficients (a, b, c)")
+    if not 1 <= int(steps) <= 16:
+        raise ValueError(f"{op}: 1 to 16 steps")
+    if not eps >= 0:
+        raise ValueError(f"{op}: eps must not be negative")
+    n = len(mats)
+    rows = (ctypes.c_int64 * n)(*[t.shape[0] for t in mats])
+    cols = (ctypes.c_int64 * n)(*[t.numel() // t.shape[0] if t.shape[0] else 0 for t in mats])
+    dt = _DTYPE[first.dtype]
+    nbytes = _lib.load().mp_orthogonalize_workspace_bytes(n, rows, cols, dt, int(steps))
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=first.device) if nbytes else None
+    return dt, rows, cols, (ctypes.c_double * 3)(*coefficients), ws, nbytes
+
+
+@torch.no_grad()
+def orthogonalize(matrices, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """Newton-Schulz orthogonalisation of every matrix G: X = G / max(|G|_F, eps), `steps` times X <- (a I + b A + c A^2) X with A = X X^T
+    (of the transpose where G has more rows than columns): singular values go to about 1, singular vectors stay.  `matrices`: a list of 2-D
+    tensors of one type (float32, float16, bfloat16; any sizes; strided ones are copied) -> a list of new tensors, or one tensor [..., m, n] ->
+    one tensor.  All matrices go through each stage in one launch.  Products in fp32 accuracy, rounded once.  Not differentiable.  The
+    coefficients must keep s <- |s (a + b s^2 + c s^4)| <= 16 for starts in [0, 1]."""
+    if torch.is_tensor(matrices):
+        _need_hip(matrices)
+        if matrices.ndim < 2:
+            raise ValueError("orthogonalize expects [..., m, n] input")
+        flat = matrices.contiguous()
+        out = torch.empty_like(flat)
+        m, n = flat.shape[-2:]
+        if flat.numel():
+            _orthogonalize_into(list(flat.view(-1, m, n).unbind(0)), list(out.view(-1, m, n).unbind(0)), steps, coefficients, eps)
+        return out
+    mats = list(matrices)
+    _need_hip(*mats)
+    for t in mats:
+        if t.ndim != 2:
+            raise ValueError("orthogonalize expects a list of 2-D matrices")
+    if not mats:
+        return []
+    mats = [t.contiguous() for t in mats]
+    out = [torch.empty_like(t) for t in mats]
+    _orthogonalize_into(mats, out, steps, coefficients, eps)
+    return out
+
+
+def _orthogonalize_into(mats, out, steps, coefficients, eps):
+    dt, rows, cols, coef, ws, nbytes = _ns_setup("orthogonalize", mats, steps, coefficients, eps)
+    _run("orthogonalize", mats[0], _lib.load().mp_orthogonalize, len(mats), _ptrs(mats), _ptrs(out), rows, cols, dt, int(steps), coef, float(eps),
+         _p(ws), nbytes)
+
+
+@torch.no_grad()
+def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale="original", steps=5,
+              coefficients=NEWTON_SCHULZ, eps=1e-7):
+    """One Muon update of a list of weights, in place: m <- m + (1 - momentum)(g - m), u = g + momentum (m - g) (nesterov) or m,
+    p <- (1 - lr weight_decay) p - lr s orthogonalize(u).  s: "original" sqrt(max(1, rows / columns)), "match_rms"
+    0.2 sqrt(max(rows, columns)), None 1.  params: contiguous, float32, float16 or bfloat16, at least two axes (the first one is the matrix's
+    rows, the rest its columns); grads: of the same shapes and type; momentum_buffers: contiguous float32 of the same shapes.  lr and the other
+    numbers are fixed in a recorded graph."""
+    params, grads, bufs = list(params), list(grads), list(momentum_buffers)
+    if not len(params) == len(grads) == len(bufs):
+        raise ValueError("muon_step: one gradient and one momentum buffer per parameter")
+    if scale not in MUON_SCALES:
+        raise ValueError(f"muon_step: scale is one of {list(MUON_SCALES)}")
+    if not params:
+        return
+    _need_hip(*params, *grads, *bufs)
+    seen = set()
+    for p, g, m in zip(params, grads, bufs):
+        if p.ndim < 2:
+            raise ValueError("muon_step updates matrices: a parameter has fewer than two axes")
+        if g.shape != p.shape or m.shape != p.shape or g.dtype != p.dtype or g.device != p.device or m.device != p.device:
+            raise ValueError("muon_step: gradient and momentum have the parameter's shape and device, the gradient its type")
+        if m.dtype != torch.float32:
+            raise ValueError("muon_step: momentum buffers are float32")
+        if not (p.is_contiguous() and m.is_contiguous()):
+            raise ValueError("muon_step updates contiguous parameters and momentum buffers")
+        for t in (p, m):
+            if t.numel() and t.data_ptr() in seen:
+                raise ValueError("muon_step: a parameter or momentum buffer is given twice")
+            seen.add(t.data_ptr())
+    grads = [g.contiguous() for g in grads]
+    dt, rows, cols, coef, ws, nbytes = _ns_setup("muon_step", params, steps, coefficients, eps)
+    _run("muon_step", params[0], _lib.load().mp_muon_step, len(params), _ptrs(params), _ptrs(grads), _ptrs(bufs), rows, cols, dt, float(lr),
+         float(momentum), int(bool(nesterov)), float(weight_decay), MUON_SCALES[scale], int(steps), coef, float(eps), _p(ws), nbytes)
+    torch.autograd.graph.increment_version(params)
+    torch.autograd.graph.increment_version(bufs)
