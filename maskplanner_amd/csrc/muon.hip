@@ -43,11 +43,13 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     const float* rdev;       // alpha is multiplied by rdev^rpow
     int M, N, kc, oc, otc, rpow, sym, tiles_n;
     float alpha, cb, ca, so, fmul, fdecay;
-    int tile0;               // first workgroup
+    int tile0, unit0;        // first tile, first unit (a unit: one chunk of one tile) of the launch
 };
 struct Probs {
     Prob p[MAX_PROB];
-    int count, splits, kper;      // splits > 1: chunks of kper, partial accumulators to memory
+    int count, tiles, units;      // totals
+    int whole;                    // tiles of the first `whole` workgroups, one each; the rest is cut into equal ranges of units
+    int cut0, cut, cuts;          // the ranges: first unit, units a range, how many
     int fin_dtype, fin_update;    // fin_update: fin = fdecay * fin - fmul * value
     float* part;
 };
@@ -55,13 +57,17 @@ static_assert(sizeof(Probs) <= 3584, "travels in the kernel arguments");
 
 __host__ __device__ inline int chunks(int64_t k) { return (int)((k + 31) / 32); }
 
-// 16 bytes a lane straight into LDS (lane i at dst + 16 i); waited for by wait_vm0 in front of a barrier
+// 16 bytes a lane straight into LDS (lane i at dst + 16 i); waited for by wait_vm in front of a barrier
 __device__ __forceinline__ void to_lds16(const void* src, void* dst)
 {
     const unsigned l = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)dst);
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(l) : "memory");
 }
-__device__ __forceinline__ void wait_vm0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_vm()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt is a six-bit counter");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ void store_fin(void* p, int dtype, size_t i, float v)
@@ -77,34 +83,56 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, size_t i)
     return (float)static_cast<const __bf16*>(p)[i];
 }
 
-struct TileAt { int prob, m0, n0, split, index; };
-
-__device__ __forceinline__ TileAt find_tile(const Probs& a, int block, int TM, int TN)
+// four consecutive elements at any element address, zeros from `left` on
+__device__ __forceinline__ void load4(const void* p, int dtype, size_t i, int64_t left, float (&v)[4])
 {
-    TileAt t;
-    int i = 0;
-    while (i + 1 < a.count && block >= a.p[i + 1].tile0) ++i;       // uniform: scalar loop over <= 24 entries
-    t.prob = i;
-    const int local = block - a.p[i].tile0;
-    t.split = local % a.splits;
-    const int tile = local / a.splits;
-    int ti, tj;
-    if (a.p[i].sym) {        // lower triangle: tile = ti (ti + 1) / 2 + tj
-        ti = (int)((sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
-        while (ti * (ti + 1) / 2 > tile) --ti;
-        tj = tile - ti * (ti + 1) / 2;
-    } else {
-        ti = tile / a.p[i].tiles_n;
-        tj = tile % a.p[i].tiles_n;
-    }
-    t.m0 = ti * TM;
-    t.n0 = tj * TN;
-    t.index = block / a.splits;       // (tile0 is a multiple of splits)
-    return t;
+    if (left >= 4) {
+        if (dtype == MP_DTYPE_F32) __builtin_memcpy(v, static_cast<const float*>(p) + i, 16);
+        else if (dtype == MP_DTYPE_F16) {
+            _Float16 t[4];
+            __builtin_memcpy(t, static_cast<const _Float16*>(p) + i, 8);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+        } else {
+            __bf16 t[4];
+            __builtin_memcpy(t, static_cast<const __bf16*>(p) + i, 8);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+        }
+    } else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < left ? load_any(p, dtype, i + e) : 0.0f;
 }
 
-__device__ __forceinline__ void put_planes(_Float16* img, int row, int nchunk, int col, const float (&v)[4], int n)
+// Tiles of a symmetric product: row ti of tiles holds the tj with any element on or below the diagonal, tj < (ti + 1) TM / TN (the last row:
+// as many as there are columns).  Row-major order.
+__host__ __device__ inline int tiles_of(int M, int N, int sym, int TM, int TN)
+{
+    const int tm = (M + TM - 1) / TM, tn = (N + TN - 1) / TN, q = TM / TN;
+    if (!sym) return tm * tn;
+    const int last = q * tm < tn ? q * tm : tn;
+    return q * (tm * (tm - 1) / 2) + last;
+}
+
+__device__ __forceinline__ void tile_at(const Prob& p, int tile, int TM, int TN, int& m0, int& n0)
+{
+    int ti, tj;
+    if (p.sym) {
+        const int q = TM / TN;
+        const int f = tile / q;                        // q (ti + 1) ti / 2 + tj = tile
+        ti = (int)((sqrtf(8.0f * (float)f + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= f) ++ti;
+        while (ti * (ti + 1) / 2 > f) --ti;
+        tj = tile - q * (ti * (ti + 1) / 2);
+    } else {
+        ti = tile / p.tiles_n;
+        tj = tile % p.tiles_n;
+    }
+    m0 = ti * TM;
+    n0 = tj * TN;
+}
+
+__device__ __forceinline__ void put_planes(_Float16* img, int row, int nchunk, int col, const float (&v)[4])
 {
     half4 h, l;
 #pragma unroll
@@ -113,217 +141,297 @@ __device__ __forceinline__ void put_planes(_Float16* img, int row, int nchunk, i
         l[e] = (_Float16)(v[e] - (float)h[e]);
     }
     _Float16* q = img + ((size_t)row * nchunk + (col >> 5)) * 64 + (col & 31);
-    if (n == 4) {
-        *reinterpret_cast<half4*>(q) = h;
-        *reinterpret_cast<half4*>(q + 32) = l;
-    } else
-        for (int e = 0; e < n; ++e) {
-            q[e] = h[e];
-            q[32 + e] = l[e];
-        }
+    *reinterpret_cast<half4*>(q) = h;
+    *reinterpret_cast<half4*>(q + 32) = l;
 }
 
-// Wave (wm, wn) of 2 x 2 holds WM x WN blocks of 32 x 32; block register r of lane q: row (r & 3) + 8 (r >> 2) + 4 (q >> 5), column q & 31.
-template <int WM, int WN>
-__device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, const TileAt& t, float16v (&acc)[WM][WN])
+__device__ __forceinline__ float alpha_of(const Prob& p)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave >> 1) * WM * 32, wn = (wave & 1) * WN * 32;
-    float alpha = p.alpha;
-    if (p.rpow) {
-        const float r = *p.rdev;
-        alpha *= p.rpow == 2 ? r * r : r;
-    }
+    if (!p.rpow) return p.alpha;
+    const float r = *p.rdev;
+    return p.alpha * (p.rpow == 2 ? r * r : r);
+}
+
+// `rows` (a multiple of 32) x TN accumulators at (r0, c0) of the product, in LDS with row stride TN + 1, to wherever the problem wants
+// them.  Through LDS because a result goes out in two orientations: eight consecutive elements a lane (16 bytes of each plane, 64-byte
+// runs) either way.
+template <int TN>
+__device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t, int rows, int r0, int c0)
+{
+    const float alpha = alpha_of(p);
     const int padN = p.oc * 32, padM = p.otc * 32;
+    for (int q = threadIdx.x; q < rows * (TN / 8); q += 256) {
+        const int rl = q / (TN / 8), cl = q % (TN / 8) * 8, row = r0 + rl, col = c0 + cl;
+        if (row >= p.M) continue;
+        float* tt = t + rl * (TN + 1) + cl;
+        float v[8];
 #pragma unroll
-    for (int i = 0; i < WM; ++i)
+        for (int e = 0; e < 8; ++e) v[e] = alpha * tt[e];
+        if (p.C && col < padN) {
+            const half8* c = reinterpret_cast<const half8*>(p.C + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31));
+            const half8 h = c[0], l = c[4];
 #pragma unroll
-        for (int j = 0; j < WN; ++j) {
-            const int col = t.n0 + wn + j * 32 + (lane & 31);
-#pragma unroll
-            for (int rg = 0; rg < 4; ++rg) {
-                const int row0 = t.m0 + wm + i * 32 + rg * 8 + (lane >> 5) * 4;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = row0 + e;
-                    float x = alpha * acc[i][j][rg * 4 + e];
-                    if (p.C && row < p.M && col < p.N) {
-                        const _Float16* c = p.C + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31);
-                        x += p.cb * ((float)c[0] + (float)c[32]);
-                    }
-                    if (row == col) x += p.ca;
-                    v[e] = x;
-                }
-                if (p.fin) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = row0 + e;
-                        if (row < p.M && col < p.N) {
-                            const size_t at = (size_t)row * p.N + col;
-                            float x = v[e];
-                            if (a.fin_update) x = p.fdecay * load_any(p.fin, a.fin_dtype, at) - p.fmul * x;
-                            store_fin(p.fin, a.fin_dtype, at, x);
-                        }
-                    }
-                }
-                if (p.out) {
-                    // columns N .. padN - 1 are written as zeros.  A symmetric result takes its lower half: row >= column here, mirrored below.
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = row0 + e;
-                        if (row < p.M && col < padN && (!p.sym || row >= col)) {
-                            const float x = col < p.N ? v[e] * p.so : 0.0f;
-                            const _Float16 h = (_Float16)x;
-                            _Float16* q = p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31);
-                            q[0] = h;
-                            q[32] = (_Float16)(x - (float)h);
-                        }
-                    }
-                }
-                if (p.outT && col < p.N) {
-                    float y[4];
-                    bool all = row0 + 3 < padM;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        y[e] = row0 + e < p.M ? v[e] * p.so : 0.0f;
-                        if (p.sym && row0 + e <= col) all = false;        // (row == col was written above)
-                    }
-                    if (all) put_planes(p.outT, col, p.otc, row0, y, 4);
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (row0 + e < padM && (!p.sym || row0 + e > col)) {
-                                const _Float16 h = (_Float16)y[e];
-                                _Float16* q = p.outT + ((size_t)col * p.otc + ((row0 + e) >> 5)) * 64 + ((row0 + e) & 31);
-                                q[0] = h;
-                                q[32] = (_Float16)(y[e] - (float)h);
-                            }
-                }
-            }
+            for (int e = 0; e < 8; ++e) v[e] += p.cb * ((float)h[e] + (float)l[e]);
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (row == col + e) v[e] += p.ca;
+        if (p.fin) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < p.N) {
+                    const size_t at = (size_t)row * p.N + col + e;
+                    float x = v[e];
+                    if (a.fin_update) x = p.fdecay * load_any(p.fin, a.fin_dtype, at) - p.fmul * x;
+                    store_fin(p.fin, a.fin_dtype, at, x);
+                }
+        }
+        // columns N .. padN - 1 are written as zeros.  A symmetric result takes its lower half: row >= column here, mirrored below.
+        if (p.out && col < padN && (!p.sym || row >= col)) {
+            half8 h, l;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = col + e < p.N ? v[e] * p.so : 0.0f;
+                h[e] = (_Float16)x;
+                l[e] = (_Float16)(x - (float)h[e]);
+            }
+            _Float16* o = p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31);
+            if (!p.sym || row >= col + 7) {
+                *reinterpret_cast<half8*>(o) = h;
+                *reinterpret_cast<half8*>(o + 32) = l;
+            } else
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (row >= col + e) {
+                        o[e] = h[e];
+                        o[32 + e] = l[e];
+                    }
+        }
+        if (p.outT)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tt[e] = v[e];
+    }
+    if (!p.outT) return;
+    __syncthreads();
+    for (int q = threadIdx.x; q < rows / 8 * TN; q += 256) {
+        const int cl = (q >> 2) % TN, rl = (q / (4 * TN)) * 32 + (q & 3) * 8, row = r0 + rl, col = c0 + cl;
+        if (col >= p.N || row >= padM) continue;
+        half8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = row + e < p.M ? t[(rl + e) * (TN + 1) + cl] * p.so : 0.0f;
+            h[e] = (_Float16)x;
+            l[e] = (_Float16)(x - (float)h[e]);
+        }
+        _Float16* o = p.outT + ((size_t)col * p.otc + (row >> 5)) * 64 + (row & 31);
+        if (!p.sym || row > col) {
+            *reinterpret_cast<half8*>(o) = h;
+            *reinterpret_cast<half8*>(o + 32) = l;
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (row + e > col) {        // (row + e == col was written above)
+                    o[e] = h[e];
+                    o[32 + e] = l[e];
+                }
+    }
 }
 
-// One tile of (64 WM) x (64 WN), four waves, two LDS buffers of one 32-k chunk: chunk c + 1 is on its way into one while c is multiplied
-// out of the other (one barrier a chunk: whoever passed it has finished with the buffer that is filled next).  A row of a buffer is 128
-// bytes; its 16-byte unit u lies at u ^ (row & 7), so that the 32 rows a fragment read touches meet each bank group equally often.
-template <int WM, int WN>
-__global__ __launch_bounds__(256) void ns_gemm_kernel(Probs a)
+// A tile of (64 WM) x (64 WN), four waves (2 x 2), NS LDS buffers of one 32-k chunk.  Halfway through chunk c (its second 16 k are in
+// registers by then) the workgroup meets: chunk c + 1 has arrived for everybody, buffer c is free and takes chunk c + NS; the first fragments
+// of c + 1 are read while the second half of c is multiplied.  One barrier a chunk, NS - 1 chunks of latency covered.
+// An operand row of a buffer is 64 bytes per plane (PL, PR planes); its 16-byte unit u lies at u ^ swz(row), the swizzle applied to the
+// source address of the load, so that the 32 rows of a fragment read meet each bank group equally often.
+template <int PL> __device__ __forceinline__ int swz(int row) { return PL == 2 ? row & 7 : (row >> 1) & 3; }
+
+template <int WM, int WN, int PL, int PR, int NS>
+__global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Probs a)
 {
-    constexpr int TM = 64 * WM, TN = 64 * WN, STAGE = (TM + TN) * 128;
-    __shared__ __align__(16) char lds[2 * STAGE];
-    const TileAt t = find_tile(a, blockIdx.x, TM, TN);
-    const Prob& p = a.p[t.prob];
+    constexpr int TM = 64 * WM, TN = 64 * WN, BL = TM * 64 * PL, BR = TN * 64 * PR, STAGE = BL + BR;
+    constexpr int NL = BL / 4096, NR = BR / 4096;                  // load instructions a wave and stage
+    extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c0 = t.split * a.kper, c1 = a.splits == 1 ? p.kc : (c0 + a.kper < p.kc ? c0 + a.kper : p.kc);
+    const int fr = lane & 31, fh = lane >> 5;                      // fragment row, k half
+    const int wm = (wave >> 1) * WM * 32, wn = (wave & 1) * WN * 32;
 
-    // load unit of this lane: rows (8 a wave and instruction), 16-byte unit of the row's chunk (swizzled at the source)
-    const int lr = wave * 8 + (lane >> 3), lu = (lane & 7) ^ (lr & 7);
-    const char* srcL[2 * WM];
-    const char* srcR[2 * WN];
-#pragma unroll
-    for (int i = 0; i < 2 * WM; ++i) {
-        int row = t.m0 + lr + 32 * i;
-        row = row < p.M ? row : p.M - 1;
-        srcL[i] = reinterpret_cast<const char*>(p.L) + ((size_t)row * p.kc + c0) * 128 + lu * 16;
+    // the workgroups of one XCD (every eighth) take consecutive tiles / ranges: they share operand rows through its L2
+    const int total = a.whole + a.cuts, bid = blockIdx.x;
+    int w = bid;
+    {
+        const int base = bid < a.whole ? 0 : a.whole, n = bid < a.whole ? a.whole : total - a.whole, b = bid - base;
+        const int per = n >> 3, rest = n & 7, x = b & 7, y = b >> 3;
+        w = base + x * per + (x < rest ? x : rest) + y;
     }
-#pragma unroll
-    for (int i = 0; i < 2 * WN; ++i) {
-        int row = t.n0 + lr + 32 * i;
-        row = row < p.N ? row : p.N - 1;
-        srcR[i] = reinterpret_cast<const char*>(p.R) + ((size_t)row * p.kc + c0) * 128 + lu * 16;
+    int u, uend;            // this workgroup's units
+    if (w < a.whole) {
+        int i = 0;
+        while (i + 1 < a.count && w >= a.p[i + 1].tile0) ++i;
+        u = a.p[i].unit0 + (w - a.p[i].tile0) * a.p[i].kc;
+        uend = u + a.p[i].kc;
+    } else {
+        u = a.cut0 + (w - a.whole) * a.cut;
+        uend = u + a.cut < a.units ? u + a.cut : a.units;
     }
-    auto fetch = [&](int buf) {
-        char* d = lds + buf * STAGE + wave * 1024;
+    for (int piece = 0; u < uend; ++piece) {
+        int i = 0;
+        while (i + 1 < a.count && u >= a.p[i + 1].unit0) ++i;      // uniform: scalar loop over <= 24 entries
+        const Prob& p = a.p[i];
+        const int tile = (u - p.unit0) / p.kc, c0 = (u - p.unit0) - tile * p.kc;
+        const int n = uend - u < p.kc - c0 ? uend - u : p.kc - c0;      // chunks of this piece (>= 1)
+        int m0, n0;
+        tile_at(p, tile, TM, TN, m0, n0);
+
+        const char* srcL[NL];
+        const char* srcR[NR];
+        constexpr int UL = 4 * PL, UR = 4 * PR;        // 16-byte units a row
 #pragma unroll
-        for (int i = 0; i < 2 * WM; ++i) {
-            to_lds16(srcL[i], d + i * 4096);
-            srcL[i] += 128;
+        for (int k = 0; k < NL; ++k) {
+            const int lr = (k * 256 + threadIdx.x) / UL;
+            const int row = m0 + lr < p.M ? m0 + lr : p.M - 1;
+            srcL[k] = reinterpret_cast<const char*>(p.L) + ((size_t)row * p.kc + c0) * (64 * PL) + ((lane % UL) ^ swz<PL>(lr)) * 16;
         }
 #pragma unroll
-        for (int i = 0; i < 2 * WN; ++i) {
-            to_lds16(srcR[i], d + TM * 128 + i * 4096);
-            srcR[i] += 128;
+        for (int k = 0; k < NR; ++k) {
+            const int lr = (k * 256 + threadIdx.x) / UR;
+            const int row = n0 + lr < p.N ? n0 + lr : p.N - 1;
+            srcR[k] = reinterpret_cast<const char*>(p.R) + ((size_t)row * p.kc + c0) * (64 * PR) + ((lane % UR) ^ swz<PR>(lr)) * 16;
         }
-    };
-    float16v acc[WM][WN];
+        auto fetch = [&](int buf) {
+            char* d = lds + buf * STAGE + wave * 1024;
 #pragma unroll
-    for (int i = 0; i < WM; ++i)
-#pragma unroll
-        for (int j = 0; j < WN; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-
-    const int fr = lane & 31, fh = lane >> 5;                  // fragment row, k half
-    const int rowL = (wave >> 1) * WM * 32 + fr, rowR = (wave & 1) * WN * 32 + fr;      // (32 i more: same row & 7)
-    if (c0 < c1) fetch(0);
-    for (int c = c0; c < c1; ++c) {
-        wait_vm0();
-        lds_barrier();
-        const char* s = lds + ((c - c0) & 1) * STAGE;
-        if (c + 1 < c1) fetch((c - c0 + 1) & 1);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            half8 fl[WM][2], fq[WN][2];
-#pragma unroll
-            for (int pl = 0; pl < 2; ++pl) {
-                const int u = pl * 4 + ks * 2 + fh;
-#pragma unroll
-                for (int i = 0; i < WM; ++i) fl[i][pl] = *reinterpret_cast<const half8*>(s + (rowL + 32 * i) * 128 + ((u ^ (rowL & 7)) * 16));
-#pragma unroll
-                for (int j = 0; j < WN; ++j) fq[j][pl] = *reinterpret_cast<const half8*>(s + TM * 128 + (rowR + 32 * j) * 128 + ((u ^ (rowR & 7)) * 16));
+            for (int k = 0; k < NL; ++k) {
+                to_lds16(srcL[k], d + k * 4096);
+                srcL[k] += 64 * PL;
             }
-            // the small products first; a block's three stay WM * WN apart (independent accumulators between them)
 #pragma unroll
-            for (int k = 0; k < 3; ++k)
+            for (int k = 0; k < NR; ++k) {
+                to_lds16(srcR[k], d + BL + k * 4096);
+                srcR[k] += 64 * PR;
+            }
+        };
+        float16v acc[WM][WN];
 #pragma unroll
-                for (int i = 0; i < WM; ++i)
+        for (int x = 0; x < WM; ++x)
 #pragma unroll
-                    for (int j = 0; j < WN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[i][k == 0], fq[j][k == 1], acc[i][j], 0, 0, 0);
+            for (int y = 0; y < WN; ++y)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+
+        const int rowL = wm + fr, rowR = wn + fr;        // (32 rows on: the same swizzle)
+        half8 fl[2][WM][PL], fq[2][WN][PR];
+        auto read = [&](int buf, int ks) {
+            const char* s = lds + buf * STAGE;
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+                for (int x = 0; x < WM; ++x)
+                    fl[ks][x][pl] = *reinterpret_cast<const half8*>(s + (rowL + 32 * x) * (64 * PL) + (((pl * 4 + ks * 2 + fh) ^ swz<PL>(rowL)) * 16));
+#pragma unroll
+            for (int pl = 0; pl < PR; ++pl)
+#pragma unroll
+                for (int y = 0; y < WN; ++y)
+                    fq[ks][y][pl] = *reinterpret_cast<const half8*>(s + BL + (rowR + 32 * y) * (64 * PR) + (((pl * 4 + ks * 2 + fh) ^ swz<PR>(rowR)) * 16));
+        };
+        auto multiply = [&](int ks) {       // the small products first; a block's stay WM * WN apart
+            if constexpr (PL == 2)
+#pragma unroll
+                for (int x = 0; x < WM; ++x)
+#pragma unroll
+                    for (int y = 0; y < WN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][PL - 1], fq[ks][y][0], acc[x][y], 0, 0, 0);
+            if constexpr (PR == 2)
+#pragma unroll
+                for (int x = 0; x < WM; ++x)
+#pragma unroll
+                    for (int y = 0; y < WN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][0], fq[ks][y][PR - 1], acc[x][y], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < WM; ++x)
+#pragma unroll
+                for (int y = 0; y < WN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][0], fq[ks][y][0], acc[x][y], 0, 0, 0);
+        };
+        const int ahead = n < NS ? n : NS;
+        for (int k = 0; k < ahead; ++k) fetch(k);
+        if (n >= NS) wait_vm<(NS - 1) * (NL + NR)>();
+        else wait_vm<0>();
+        lds_barrier();
+        read(0, 0);
+        int buf = 0;
+        for (int c = 0; c < n; ++c) {
+            read(buf, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (c + NS <= n) wait_vm<(NS - 2) * (NL + NR)>();     // chunks up to c + NS - 1 are on their way: all but c + 1's followers
+            else wait_vm<0>();
+            lds_barrier();
+            const int next = buf + 1 < NS ? buf + 1 : 0;
+            if (c + NS < n) fetch(buf);
+            if (c + 1 < n) read(next, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(1);
+            __builtin_amdgcn_sched_barrier(0);
+            buf = next;
         }
+        // (nobody reads the buffers any more: the last meeting was behind the last fragment reads)
+        float* t = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int x = 0; x < WM; ++x)
+#pragma unroll
+            for (int y = 0; y < WN; ++y)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)      // register r of lane q: row (r & 3) + 8 (r >> 2) + 4 (q >> 5), column q & 31
+                    t[(wm + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * fh) * (TN + 1) + wn + 32 * y + fr] = acc[x][y][r];
+        __syncthreads();
+        if (n == p.kc) epilogue<TN>(a, p, t, TM, m0, n0);
+        else {        // a range's first piece and its last one may be parts of tiles: two slots a range
+            float* o = a.part + (size_t)(2 * (w - a.whole) + (piece > 0)) * (TM * TN);
+            for (int q = threadIdx.x; q < TM * TN; q += 256) o[q] = t[q / TN * (TN + 1) + q % TN];
+        }
+        __syncthreads();
+        u += n;
     }
-    if (a.splits > 1) {
-        float4* o = reinterpret_cast<float4*>(a.part) + (size_t)blockIdx.x * (WM * WN * 4 * 256) + threadIdx.x;
-#pragma unroll
-        for (int i = 0; i < WM; ++i)
-#pragma unroll
-            for (int j = 0; j < WN; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    o[((i * WN + j) * 4 + r) * 256] = make_float4(acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]);
-        return;
-    }
-    epilogue<WM, WN>(a, p, t, acc);
 }
 
-// the split tiles' accumulators added in the order of the splits, then the same epilogue
+// Tiles that the ranges cut: the parts' accumulators added in the order of the ranges, then the same epilogue.  A workgroup takes 32 rows.
 template <int WM, int WN>
-__global__ __launch_bounds__(256) void ns_join_kernel(Probs a)
+__global__ __launch_bounds__(256) void ns_join_kernel(Probs a, int tile_first)
 {
-    const TileAt t = find_tile(a, blockIdx.x * a.splits, 64 * WM, 64 * WN);
-    float16v acc[WM][WN];
+    constexpr int TM = 64 * WM, TN = 64 * WN, STRIPS = TM / 32, PER = 32 * TN / 1024;
+    __shared__ float t[32 * (TN + 1)];
+    const int strip = blockIdx.x % STRIPS, tile = tile_first + blockIdx.x / STRIPS;
+    int i = 0;
+    while (i + 1 < a.count && tile >= a.p[i + 1].tile0) ++i;
+    const Prob& p = a.p[i];
+    const int u0 = p.unit0 + (tile - p.tile0) * p.kc;
+    const int w0 = (u0 - a.cut0) / a.cut, w1 = (u0 + p.kc - 1 - a.cut0) / a.cut;
+    if (w0 == w1) return;           // one range had it whole
+    float4 acc[PER];
 #pragma unroll
-    for (int i = 0; i < WM; ++i)
+    for (int k = 0; k < PER; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int w = w0; w <= w1; ++w) {
+        const int slot = 2 * w + (a.cut0 + w * a.cut < u0);
+        const float4* o = reinterpret_cast<const float4*>(a.part + (size_t)slot * (TM * TN) + strip * 32 * TN) + threadIdx.x;
 #pragma unroll
-        for (int j = 0; j < WN; ++j)
+        for (int k = 0; k < PER; ++k) {
+            const float4 v = o[k * 256];
+            acc[k].x += v.x;
+            acc[k].y += v.y;
+            acc[k].z += v.z;
+            acc[k].w += v.w;
+        }
+    }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    const float4* o = reinterpret_cast<const float4*>(a.part) + (size_t)blockIdx.x * a.splits * (WM * WN * 4 * 256) + threadIdx.x;
-    for (int s = 0; s < a.splits; ++s, o += WM * WN * 4 * 256)
-#pragma unroll
-        for (int i = 0; i < WM; ++i)
-#pragma unroll
-            for (int j = 0; j < WN; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float4 v = o[((i * WN + j) * 4 + r) * 256];
-                    acc[i][j][4 * r] += v.x;
-                    acc[i][j][4 * r + 1] += v.y;
-                    acc[i][j][4 * r + 2] += v.z;
-                    acc[i][j][4 * r + 3] += v.w;
-                }
-    epilogue<WM, WN>(a, a.p[t.prob], t, acc);
+    for (int k = 0; k < PER; ++k) {
+        const int at = (k * 256 + threadIdx.x) * 4;
+        float* d = t + at / TN * (TN + 1) + at % TN;
+        d[0] = acc[k].x;
+        d[1] = acc[k].y;
+        d[2] = acc[k].z;
+        d[3] = acc[k].w;
+    }
+    __syncthreads();
+    int m0, n0;
+    tile_at(p, tile - p.tile0, TM, TN, m0, n0);
+    epilogue<TN>(a, p, t, 32, m0 + strip * 32, n0);
 }
 
 // ---- momentum, norm, planes -------------------------------------------------------------------------------------------------------
@@ -355,15 +463,25 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Mats a)
     const size_t n = (size_t)m.rows * m.cols;
     const int b = blockIdx.x - m.blk0;
     double s = 0.0;
-    for (size_t e = (size_t)b * 256 + threadIdx.x; e < n; e += (size_t)m.blocks * 256) {
-        float u = load_any(m.g, a.dtype, e);
+#pragma unroll 4
+    for (size_t e = ((size_t)b * 256 + threadIdx.x) * 4; e < n; e += (size_t)m.blocks * 1024) {
+        const int64_t left = (int64_t)(n - e);
+        float u[4];
+        load4(m.g, a.dtype, e, left, u);
         if (m.mom) {
-            float v = m.mom[e];
-            v = v + (1.0f - a.mu) * (u - v);
-            m.mom[e] = v;
-            u = a.nesterov ? u + a.mu * (v - u) : v;
+            float v[4];
+            load4(m.mom, MP_DTYPE_F32, e, left, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[k] = v[k] + (1.0f - a.mu) * (u[k] - v[k]);
+                u[k] = a.nesterov ? u[k] + a.mu * (v[k] - u[k]) : v[k];
+            }
+            if (left >= 4) __builtin_memcpy(m.mom + e, v, 16);
+            else
+                for (int k = 0; k < (int)left; ++k) m.mom[e + k] = v[k];
         }
-        s += (double)u * (double)u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += (double)u[k] * (double)u[k];
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -396,20 +514,23 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
     const int local = blockIdx.x - m.tile0, tn = (m.cols + 63) / 64;
     const int r0 = (local / tn) * 64, c0 = (local % tn) * 64;
     if (local == 0 && threadIdx.x == 0) *m.r = (float)(1.0 / ldexp(norm > a.eps || norm != norm ? norm : a.eps, e));
-    const int tc = threadIdx.x & 63, tr = threadIdx.x >> 6;
-    for (int k = 0; k < 64; k += 4) {
+    const int tc = (threadIdx.x & 15) * 4, tr = threadIdx.x >> 4;
+#pragma unroll
+    for (int k = 0; k < 64; k += 16) {
         const int r = r0 + k + tr, c = c0 + tc;
-        float u = 0.0f;
-        if (r < m.rows && c < m.cols) {
+        float u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < m.rows) {
             const size_t at = (size_t)r * m.cols + c;
-            u = load_any(m.g, a.dtype, at);
+            load4(m.g, a.dtype, at, (int64_t)m.cols - c, u);
             if (m.mom) {
-                const float v = m.mom[at];
-                u = a.nesterov ? u + a.mu * (v - u) : v;
+                float v[4];
+                load4(m.mom, MP_DTYPE_F32, at, (int64_t)m.cols - c, v);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) u[q] = a.nesterov ? u[q] + a.mu * (v[q] - u[q]) : v[q];
             }
-            u = ldexpf(u, e);
         }
-        tile[k + tr][tc] = u;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tile[k + tr][tc + q] = ldexpf(u[q], e);
     }
     __syncthreads();
     const int pc = chunks(m.cols), ptc = chunks(m.rows);
@@ -419,12 +540,12 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
         if (r0 + b < m.rows && c0 + a4 < pc * 32) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = tile[b][a4 + k];
-            put_planes(m.P, r0 + b, pc, c0 + a4, v, 4);
+            put_planes(m.P, r0 + b, pc, c0 + a4, v);
         }
         if (c0 + b < m.cols && r0 + a4 < ptc * 32) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = tile[a4 + k][b];
-            put_planes(m.PT, c0 + b, ptc, r0 + a4, v, 4);
+            put_planes(m.PT, c0 + b, ptc, r0 + a4, v);
         }
     }
 }
@@ -479,7 +600,9 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
 int hop_plan(const Shape& s, int steps, int dtype)
 {
     // steps of a hop: cheapest of the allowed lengths (a hop of h: 3 m^2 n + (4 h - 3) m^3 against h (3 m^2 n + m^3)); ties to the short one
-    const int most = dtype == MP_DTYPE_F32 ? 2 : steps;
+    // (fp32: two steps a hop only from n = 2 m on, where it saves a fifth; nearer to square it saves less than 15 % and the error
+    // doubles: 128 x 131: 2.6e-6 of the exact result against 1.4e-6 step by step)
+    const int most = dtype == MP_DTYPE_F32 ? (s.n >= 2 * s.m ? 2 : 1) : steps;
     int best = 1;
     double cost = 1e300;
     for (int h = 1; h <= most; ++h) {
@@ -533,77 +656,99 @@ size_t layout(const Shape& s, int steps, int dtype, char* base, Buffers* b)
 }
 
 constexpr int CUS = 256;
-constexpr int SPLIT_FROM = 32;       // chunks of K from which a split pays for its trip through memory
 
-// tiles of a product in TM x TM pieces
-int64_t tiles_of(const Prob& p, int T)
-{
-    const int64_t tm = (p.M + T - 1) / T, tn = (p.N + T - 1) / T;
-    return p.sym ? tm * (tm + 1) / 2 : tm * tn;
-}
+// What a launch does: tile size, tiles taken whole (one a workgroup) and the rest cut into equal ranges of (tile, chunk) units.
+struct Plan { int shape, whole, cuts, cut; };
+// Tile shapes.  cyc: cycles of a chunk on one CU (three plane products), from the MFMA time of 256 x 128, LDS traffic of the others
+// (reads and arrivals: 256 x 128 3/4 of its MFMA time, 128 x 128 1.0, 64 x 64 1.5).
+struct TileShape { int tm, tn; double cyc; };
+constexpr TileShape SHAPES[3] = {{256, 128, 1900.0}, {128, 128, 1100.0}, {64, 64, 420.0}};
+constexpr int MAX_CUTS = CUS;
+// accumulators of the cut tiles: two slots a range
+constexpr size_t PART_BYTES = (size_t)MAX_CUTS * 2 * 256 * 128 * sizeof(float);
 
-// The launch's tile size and split.  128 x 128 tiles read each operand half as often as 64 x 64 ones but are a quarter as many: they are
-// taken when the launch has at least 3/4 of a tile per CU.  Fewer tiles than CUs and a long K: the K axis is split so that the launch has
-// about one workgroup per CU, at least 8 chunks each (a split's accumulators pass through memory once).
-struct Plan { int T, splits, kper; };
-Plan plan_of(const Prob* p, int count, bool may_split)
+// Estimated cycles of the launch in every shape, tiles whole or cut; the cheapest is taken.
+Plan plan_of(const Prob* p, int count)
 {
-    int64_t t128 = 0, t64 = 0;
-    int kc = 0;
-    for (int i = 0; i < count; ++i) {
-        t128 += tiles_of(p[i], 128);
-        t64 += tiles_of(p[i], 64);
-        kc = p[i].kc > kc ? p[i].kc : kc;
-    }
-    Plan r{128, 1, kc};
-    int64_t tiles = t128;
-    if (may_split && t128 < CUS * 3 / 4 && kc >= 64) {       // long K: keep the large tiles and split
-        r.T = t128 * 8 >= CUS / 4 ? 128 : 64;
-    } else if (t128 < CUS * 3 / 4)
-        r.T = 64;
-    if (r.T == 64) tiles = t64;
-    if (may_split && tiles < CUS && kc >= SPLIT_FROM) {
-        int64_t s = (CUS + tiles / 2) / tiles;
-        if (s > kc / 8) s = kc / 8;
-        if (s > 32) s = 32;
-        if (s > 1) {
-            r.kper = (int)((kc + s - 1) / s);
-            r.splits = (kc + r.kper - 1) / r.kper;
+    Plan best{0, 0, 0, 0};
+    double best_cost = 1e300;
+    for (int s = 0; s < 3; ++s) {
+        int64_t tiles = 0, units = 0;
+        int kmin = 1 << 30, kmax = 0;
+        for (int i = 0; i < count; ++i) {
+            const int t = tiles_of(p[i].M, p[i].N, p[i].sym, SHAPES[s].tm, SHAPES[s].tn);
+            tiles += t;
+            units += (int64_t)t * p[i].kc;
+            kmin = p[i].kc < kmin ? p[i].kc : kmin;
+            kmax = p[i].kc > kmax ? p[i].kc : kmax;
+        }
+        if (tiles > (1 << 28) || units > (1 << 30)) continue;
+        const double cyc = SHAPES[s].cyc, epi = SHAPES[s].tm * SHAPES[s].tn / 8.0;
+        // whole tiles only: as many rounds as it takes (unequal lengths: at least the longest one)
+        const double rounds = (double)((tiles + CUS - 1) / CUS);
+        double c = kmin == kmax ? rounds * (kmax * cyc + epi) : (double)units / CUS * cyc + kmax * cyc + rounds * epi;
+        if (tiles <= CUS) c = kmax * cyc + epi;
+        if (c < best_cost) { best_cost = c; best = Plan{s, (int)tiles, 0, 0}; }
+        // full rounds whole (equal lengths), the rest cut over all CUs, at least 4 chunks a range; partial accumulators there and back
+        // at ~2000 bytes a cycle of the chip, and one more launch
+        const int64_t whole = kmin == kmax ? tiles / CUS * CUS : 0, rest = tiles - whole;
+        const int64_t ru = kmin == kmax ? rest * kmax : units;
+        if (rest > 0) {
+            int64_t cut = (ru + CUS - 1) / CUS;
+            if (cut < 4) cut = 4;
+            const int64_t cuts = (ru + cut - 1) / cut;
+            const double bytes = 2.0 * (double)(cuts + rest < 2 * cuts ? cuts + rest : 2 * cuts) * SHAPES[s].tm * SHAPES[s].tn * 4.0;
+            c = (double)whole / CUS * (kmax * cyc + epi) + cut * cyc + epi + bytes / 2000.0 + 12000.0;
+            if (c < best_cost) { best_cost = c; best = Plan{s, (int)whole, (int)cuts, (int)cut}; }
         }
     }
-    return r;
+    return best;
 }
 
-// Accumulators of a split launch: tiles * splits <= CUS + tiles / 2 < 1.5 CUS whatever set of matrices the launch has.
-constexpr size_t PART_BYTES = (size_t)(CUS + CUS / 2) * 128 * 128 * sizeof(float);
+template <int WM, int WN, int PL, int PR, int NS>
+int launch_as(const Probs& a, const char* tag, double flops, hipStream_t stream)
+{
+    static mp::DynLds dyn;
+    constexpr size_t ring = (size_t)NS * (64 * WM * 64 * PL + 64 * WN * 64 * PR), tile = (size_t)64 * WM * (64 * WN + 1) * sizeof(float);
+    constexpr size_t smem = ring > tile ? ring : tile;
+    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS>), smem)) return MP_ELAUNCH;
+    MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS>), dim3((unsigned)(a.whole + a.cuts)), dim3(256), smem, stream, a);
+    MP_CHECK_LAUNCH();
+    if (a.cuts) {
+        int first = a.whole;        // (whole > 0 only with equal lengths: tile and unit order agree)
+        MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<WM, WN>), dim3((unsigned)(a.tiles - first) * 2 * WM), dim3(256), 0, stream, a, first);
+        MP_CHECK_LAUNCH();
+    }
+    return MP_OK;
+}
 
-int launch(Probs& a, bool may_split, const char* tag, hipStream_t stream)
+int launch(Probs& a, const char* tag, hipStream_t stream)
 {
     if (a.count == 0) return MP_OK;
-    const Plan pl = plan_of(a.p, a.count, may_split);
-    a.splits = pl.splits;
-    a.kper = pl.kper;
-    int64_t blocks = 0;
+    const Plan pl = plan_of(a.p, a.count);
+    const TileShape ts = SHAPES[pl.shape];
+    if (pl.whole + pl.cuts == 0) return MP_EUNSUPPORTED;
+    int64_t tiles = 0, units = 0;
     double flops = 0.0;
     for (int i = 0; i < a.count; ++i) {
         Prob& p = a.p[i];
-        p.tiles_n = (p.N + pl.T - 1) / pl.T;
-        p.tile0 = (int)blocks;
-        blocks += tiles_of(p, pl.T) * pl.splits;
+        p.tiles_n = (p.N + ts.tn - 1) / ts.tn;
+        p.tile0 = (int)tiles;
+        p.unit0 = (int)units;
+        const int t = tiles_of(p.M, p.N, p.sym, ts.tm, ts.tn);
+        tiles += t;
+        units += (int64_t)t * p.kc;
         flops += 6.0 * p.M * p.N * 32.0 * p.kc * (p.sym ? 0.5 : 1.0);
-        if (blocks > 0x7fffffff) return MP_EUNSUPPORTED;
     }
-    if (pl.T == 128) {
-        MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<2, 2>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-        MP_CHECK_LAUNCH();
-        if (pl.splits > 1) MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<2, 2>), dim3((unsigned)(blocks / pl.splits)), dim3(256), 0, stream, a);
-    } else {
-        MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<1, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-        MP_CHECK_LAUNCH();
-        if (pl.splits > 1) MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<1, 1>), dim3((unsigned)(blocks / pl.splits)), dim3(256), 0, stream, a);
-    }
-    MP_CHECK_LAUNCH();
-    return MP_OK;
+    a.tiles = (int)tiles;
+    a.units = (int)units;
+    a.whole = pl.whole;
+    a.cuts = pl.cuts;
+    a.cut = pl.cut;
+    a.cut0 = pl.whole == 0 ? 0 : pl.whole * a.p[0].kc;
+    if (pl.shape == 0) return launch_as<4, 2, 2, 2, 3>(a, tag, flops, stream);
+    if (pl.shape == 1) return launch_as<2, 2, 2, 2, 2>(a, tag, flops, stream);
+    return launch_as<1, 1, 2, 2, 4>(a, tag, flops, stream);
 }
 
 struct Update { int on; double lr, mu, decay; int nesterov, scale; };
@@ -620,13 +765,11 @@ int next_chunk(int64_t count, const int64_t* rows, const int64_t* cols, int64_t&
 size_t chunk_bytes(const int64_t* rows, const int64_t* cols, const int64_t* idx, int k, int steps, int dtype)
 {
     size_t bytes = 0;
-    bool split = false;
     for (int q = 0; q < k; ++q) {
         const Shape s = shape_of(rows[idx[q]], cols[idx[q]]);
         bytes += layout(s, steps, dtype, nullptr, nullptr);
-        split = split || chunks(s.n) >= SPLIT_FROM;
     }
-    return bytes + (split ? PART_BYTES : 0);
+    return bytes + PART_BYTES;
 }
 
 int check_args(int64_t count, const int64_t* rows, const int64_t* cols, int dtype, int steps)
@@ -637,7 +780,8 @@ int check_args(int64_t count, const int64_t* rows, const int64_t* cols, int dtyp
     for (int64_t i = 0; i < count; ++i) {
         if (rows[i] < 0 || cols[i] < 0) return MP_EINVAL;
         const int64_t m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
-        if (m > 65536 || n > ((int64_t)1 << 30)) return MP_EUNSUPPORTED;
+        // (the last: units of a product are counted in 31 bits; such a matrix and its planes do not fit the card)
+        if (m > 65536 || n > ((int64_t)1 << 30) || (double)m * (double)m * (double)n > 1125899906842624.0) return MP_EUNSUPPORTED;
     }
     return MP_OK;
 }
@@ -713,7 +857,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
             if (first[q]) { p.rdev = bf[q].r; p.rpow = 2; }
             g.p[g.count++] = p;
         }
-        int rc = launch(g, true, "ns_gemm_kernel (gram)", stream);
+        int rc = launch(g, "ns_gemm_kernel (gram)", stream);
         if (rc) return rc;
         for (int s = 0; s < longest; ++s) {
             g.count = 0;
@@ -727,7 +871,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                 p.ca = (float)coef[0];
                 g.p[g.count++] = p;
             }
-            rc = launch(g, false, "ns_gemm_kernel (square)", stream);
+            rc = launch(g, "ns_gemm_kernel (square)", stream);
             if (rc) return rc;
             g.count = 0;
             for (int q = 0; q < k; ++q) {      // T = A Q (another step follows), R = Q R: independent, one launch
@@ -744,12 +888,12 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                     sR[q] = so;
                 }
             }
-            rc = launch(g, false, "ns_gemm_kernel (step)", stream);
+            rc = launch(g, "ns_gemm_kernel (step)", stream);
             if (rc) return rc;
             g.count = 0;
             for (int q = 0; q < k; ++q)        // A = T Q
                 if (s + 1 < len[q]) g.p[g.count++] = sym_prob(q, bf[q].T, bf[q].P[qbuf[q]], sT, sQ, bf[q].A, sA);
-            rc = launch(g, false, "ns_gemm_kernel (step)", stream);
+            rc = launch(g, "ns_gemm_kernel (step)", stream);
             if (rc) return rc;
         }
         g.count = 0;
@@ -790,7 +934,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
             first[q] = false;
             g.p[g.count++] = p;
         }
-        rc = launch(g, false, "ns_gemm_kernel (apply)", stream);
+        rc = launch(g, "ns_gemm_kernel (apply)", stream);
         if (rc) return rc;
     }
     return MP_OK;
