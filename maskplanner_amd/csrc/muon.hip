@@ -57,11 +57,11 @@ static_assert(sizeof(Probs) <= 3584, "travels in the kernel arguments");
 
 __host__ __device__ inline int chunks(int64_t k) { return (int)((k + 31) / 32); }
 
-// 16 bytes a lane straight into LDS (lane i at dst + 16 i); waited for by wait_vm in front of a barrier
-__device__ __forceinline__ void to_lds16(const void* src, void* dst)
+// 16 bytes a lane straight into LDS: from base + off (base the same for the wave) to the LDS address dst + 16 * lane; waited for by
+// wait_vm in front of a barrier
+__device__ __forceinline__ void to_lds16(const char* base, unsigned off, unsigned dst)
 {
-    const unsigned l = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) void*)dst);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(l) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_vm()
 {
@@ -253,6 +253,7 @@ __global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Prob
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int fr = lane & 31, fh = lane >> 5;                      // fragment row, k half
     const int wm = (wave >> 1) * WM * 32, wn = (wave & 1) * WN * 32;
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)lds + wave * 1024);
 
     // the workgroups of one XCD (every eighth) take consecutive tiles / ranges: they share operand rows through its L2
     const int total = a.whole + a.cuts, bid = blockIdx.x;
@@ -281,32 +282,28 @@ __global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Prob
         int m0, n0;
         tile_at(p, tile, TM, TN, m0, n0);
 
-        const char* srcL[NL];
-        const char* srcR[NR];
+        // source offsets of this lane from the tile's first row (below 2^32: rows <= 256, K <= 2^21)
+        unsigned offL[NL], offR[NR];
         constexpr int UL = 4 * PL, UR = 4 * PR;        // 16-byte units a row
 #pragma unroll
         for (int k = 0; k < NL; ++k) {
-            const int lr = (k * 256 + threadIdx.x) / UL;
-            const int row = m0 + lr < p.M ? m0 + lr : p.M - 1;
-            srcL[k] = reinterpret_cast<const char*>(p.L) + ((size_t)row * p.kc + c0) * (64 * PL) + ((lane % UL) ^ swz<PL>(lr)) * 16;
+            const int lr = (k * 256 + threadIdx.x) / UL, row = m0 + lr < p.M ? lr : p.M - 1 - m0;
+            offL[k] = (unsigned)row * (unsigned)(p.kc * 64 * PL) + ((lane % UL) ^ swz<PL>(lr)) * 16;
         }
 #pragma unroll
         for (int k = 0; k < NR; ++k) {
-            const int lr = (k * 256 + threadIdx.x) / UR;
-            const int row = n0 + lr < p.N ? n0 + lr : p.N - 1;
-            srcR[k] = reinterpret_cast<const char*>(p.R) + ((size_t)row * p.kc + c0) * (64 * PR) + ((lane % UR) ^ swz<PR>(lr)) * 16;
+            const int lr = (k * 256 + threadIdx.x) / UR, row = n0 + lr < p.N ? lr : p.N - 1 - n0;
+            offR[k] = (unsigned)row * (unsigned)(p.kc * 64 * PR) + ((lane % UR) ^ swz<PR>(lr)) * 16;
         }
-        auto fetch = [&](int buf) {
-            char* d = lds + buf * STAGE + wave * 1024;
-#pragma unroll
-            for (int k = 0; k < NL; ++k) {
-                to_lds16(srcL[k], d + k * 4096);
-                srcL[k] += 64 * PL;
-            }
-#pragma unroll
-            for (int k = 0; k < NR; ++k) {
-                to_lds16(srcR[k], d + BL + k * 4096);
-                srcR[k] += 64 * PR;
+        const char* srcL = reinterpret_cast<const char*>(p.L) + ((size_t)m0 * p.kc + c0) * (64 * PL);
+        const char* srcR = reinterpret_cast<const char*>(p.R) + ((size_t)n0 * p.kc + c0) * (64 * PR);
+        auto fetch_one = [&](int buf, int k) {         // instruction k of NL + NR; the last one moves on to the next chunk
+            const unsigned d = lds0 + buf * STAGE;
+            if (k < NL) to_lds16(srcL, offL[k < NL ? k : 0], d + k * 4096);
+            else to_lds16(srcR, offR[k >= NL ? k - NL : 0], d + BL + (k - NL) * 4096);
+            if (k == NL + NR - 1) {
+                srcL += 64 * PL;
+                srcR += 64 * PR;
             }
         };
         float16v acc[WM][WN];
@@ -319,56 +316,59 @@ __global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Prob
 
         const int rowL = wm + fr, rowR = wn + fr;        // (32 rows on: the same swizzle)
         half8 fl[2][WM][PL], fq[2][WN][PR];
-        auto read = [&](int buf, int ks) {
+        constexpr int READS = WM * PL + WN * PR, PRODS = (PL + PR - 1) * WM * WN, FETCHES = NL + NR;
+        auto read_one = [&](int buf, int ks, int k) {
             const char* s = lds + buf * STAGE;
-#pragma unroll
-            for (int pl = 0; pl < PL; ++pl)
-#pragma unroll
-                for (int x = 0; x < WM; ++x)
-                    fl[ks][x][pl] = *reinterpret_cast<const half8*>(s + (rowL + 32 * x) * (64 * PL) + (((pl * 4 + ks * 2 + fh) ^ swz<PL>(rowL)) * 16));
-#pragma unroll
-            for (int pl = 0; pl < PR; ++pl)
-#pragma unroll
-                for (int y = 0; y < WN; ++y)
-                    fq[ks][y][pl] = *reinterpret_cast<const half8*>(s + BL + (rowR + 32 * y) * (64 * PR) + (((pl * 4 + ks * 2 + fh) ^ swz<PR>(rowR)) * 16));
+            if (k < WM * PL) {
+                const int x = k % WM, pl = k / WM % PL;
+                fl[ks][x][pl] = *reinterpret_cast<const half8*>(s + (rowL + 32 * x) * (64 * PL) + (((pl * 4 + ks * 2 + fh) ^ swz<PL>(rowL)) * 16));
+            } else {
+                const int y = (k - WM * PL) % WN, pl = (k - WM * PL) / WN % PR;
+                fq[ks][y][pl] = *reinterpret_cast<const half8*>(s + BL + (rowR + 32 * y) * (64 * PR) + (((pl * 4 + ks * 2 + fh) ^ swz<PR>(rowR)) * 16));
+            }
         };
-        auto multiply = [&](int ks) {       // the small products first; a block's stay WM * WN apart
-            if constexpr (PL == 2)
+        // The PRODS matrix instructions of 16 k, the small products first, a block's WM * WN apart; in the shadow of each (32 cycles) go its
+        // share of the reads of the other half's fragments and of the loads of a chunk to come: with one wave a SIMD nothing else fills it.
+        auto multiply = [&](int ks, bool reads, int rbuf, bool fetches, int fbuf) {
 #pragma unroll
-                for (int x = 0; x < WM; ++x)
+            for (int g = 0; g < PRODS; ++g) {
+                const int k = g / (WM * WN), x = g / WN % WM, y = g % WN;
+                const int pl = PL == 2 && k == 0 ? 1 : 0, pr = PR == 2 && k == PL - 1 ? 1 : 0;
+                acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][pl], fq[ks][y][pr], acc[x][y], 0, 0, 0);
+                if (reads)
 #pragma unroll
-                    for (int y = 0; y < WN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][PL - 1], fq[ks][y][0], acc[x][y], 0, 0, 0);
-            if constexpr (PR == 2)
+                    for (int r = g * READS * 2 / PRODS; r < (g + 1) * READS * 2 / PRODS; ++r)        // (in the first half: in time for the next)
+                        if (r < READS) read_one(rbuf, ks ^ 1, r);
+                if (fetches)
 #pragma unroll
-                for (int x = 0; x < WM; ++x)
-#pragma unroll
-                    for (int y = 0; y < WN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][0], fq[ks][y][PR - 1], acc[x][y], 0, 0, 0);
-#pragma unroll
-            for (int x = 0; x < WM; ++x)
-#pragma unroll
-                for (int y = 0; y < WN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][0], fq[ks][y][0], acc[x][y], 0, 0, 0);
+                    for (int r = g * FETCHES / PRODS; r < (g + 1) * FETCHES / PRODS; ++r) fetch_one(fbuf, r);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         const int ahead = n < NS ? n : NS;
-        for (int k = 0; k < ahead; ++k) fetch(k);
-        if (n >= NS) wait_vm<(NS - 1) * (NL + NR)>();
+        for (int k = 0; k < ahead; ++k)
+#pragma unroll
+            for (int r = 0; r < FETCHES; ++r) fetch_one(k, r);
+        if (n >= NS) wait_vm<(NS - 1) * FETCHES>();
         else wait_vm<0>();
         lds_barrier();
-        read(0, 0);
-        int buf = 0;
-        for (int c = 0; c < n; ++c) {
-            read(buf, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (c + NS <= n) wait_vm<(NS - 2) * (NL + NR)>();     // chunks up to c + NS - 1 are on their way: all but c + 1's followers
-            else wait_vm<0>();
+#pragma unroll
+        for (int r = 0; r < READS; ++r) read_one(0, 0, r);
+        int buf = 0, c = 0;
+        for (; c + NS < n; ++c) {       // chunks up to c + NS - 1 are on their way
+            multiply(0, true, buf, false, 0);
+            wait_vm<(NS - 2) * FETCHES>();
             lds_barrier();
             const int next = buf + 1 < NS ? buf + 1 : 0;
-            if (c + NS < n) fetch(buf);
-            if (c + 1 < n) read(next, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(1);
-            __builtin_amdgcn_sched_barrier(0);
+            multiply(1, true, next, true, buf);
+            buf = next;
+        }
+        for (; c < n; ++c) {            // the last NS: nothing more to load
+            multiply(0, true, buf, false, 0);
+            wait_vm<0>();
+            lds_barrier();
+            const int next = buf + 1 < NS ? buf + 1 : 0;
+            multiply(1, c + 1 < n, next, false, 0);
             buf = next;
         }
         // (nobody reads the buffers any more: the last meeting was behind the last fragment reads)
@@ -781,7 +781,7 @@ int check_args(int64_t count, const int64_t* rows, const int64_t* cols, int dtyp
         if (rows[i] < 0 || cols[i] < 0) return MP_EINVAL;
         const int64_t m = rows[i] < cols[i] ? rows[i] : cols[i], n = rows[i] < cols[i] ? cols[i] : rows[i];
         // (the last: units of a product are counted in 31 bits; such a matrix and its planes do not fit the card)
-        if (m > 65536 || n > ((int64_t)1 << 30) || (double)m * (double)m * (double)n > 1125899906842624.0) return MP_EUNSUPPORTED;
+        if (m > 65536 || n > ((int64_t)1 << 21) || (double)m * (double)m * (double)n > 1125899906842624.0) return MP_EUNSUPPORTED;
     }
     return MP_OK;
 }
