@@ -31,7 +31,7 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int MAX_MAT = 12;            // matrices of one pass through the stages
 constexpr int MAX_PROB = 2 * MAX_MAT;  // products of one launch (a hop's step has two independent ones per matrix)
-constexpr int MAX_NORM_BLOCKS = 512;   // partial sums of squares per matrix
+constexpr int MAX_NORM_BLOCKS = 2048;   // partial sums of squares per matrix
 
 struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T over kc chunks of 32
     const _Float16* L;
@@ -39,9 +39,9 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     const _Float16* C;       // planes [M][oc] or NULL
     _Float16* out;           // planes [M][oc] or NULL
     _Float16* outT;          // planes [N][otc] or NULL
-    void* fin;               // [M, N] of the result type or NULL
+    void* fin;               // [M, N] of the result type, or [N, M] (fin_t), or NULL
     const float* rdev;       // alpha is multiplied by rdev^rpow
-    int M, N, kc, oc, otc, rpow, sym, tiles_n;
+    int M, N, kc, oc, otc, rpow, sym, tiles_n, fin_t;
     float alpha, cb, ca, so, fmul, fdecay;
     int tile0, unit0;        // first tile, first unit (a unit: one chunk of one tile) of the launch
 };
@@ -152,6 +152,35 @@ __device__ __forceinline__ float alpha_of(const Prob& p)
     return p.alpha * (p.rpow == 2 ? r * r : r);
 }
 
+// up to eight consecutive elements of the result, at any element address
+__device__ __forceinline__ void put_fin(const Probs& a, const Prob& p, size_t at, int left, float (&v)[8])
+{
+    if (a.fin_update) {
+        float w[8];
+        load4(p.fin, a.fin_dtype, at, left, reinterpret_cast<float(&)[4]>(w[0]));
+        load4(p.fin, a.fin_dtype, at + 4, left - 4, reinterpret_cast<float(&)[4]>(w[4]));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = p.fdecay * w[e] - p.fmul * v[e];
+    }
+    if (left >= 8) {
+        if (a.fin_dtype == MP_DTYPE_F32) __builtin_memcpy(static_cast<float*>(p.fin) + at, v, 32);
+        else if (a.fin_dtype == MP_DTYPE_F16) {
+            _Float16 h[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = (_Float16)v[e];
+            __builtin_memcpy(static_cast<_Float16*>(p.fin) + at, h, 16);
+        } else {
+            __bf16 h[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = (__bf16)v[e];
+            __builtin_memcpy(static_cast<__bf16*>(p.fin) + at, h, 16);
+        }
+    } else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < left) store_fin(p.fin, a.fin_dtype, at + e, v[e]);
+}
+
 // `rows` (a multiple of 32) x TN accumulators at (r0, c0) of the product, in LDS with row stride TN + 1, to wherever the problem wants
 // them.  Through LDS because a result goes out in two orientations: eight consecutive elements a lane (16 bytes of each plane, 64-byte
 // runs) either way.
@@ -176,16 +205,7 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (row == col + e) v[e] += p.ca;
-        if (p.fin) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (col + e < p.N) {
-                    const size_t at = (size_t)row * p.N + col + e;
-                    float x = v[e];
-                    if (a.fin_update) x = p.fdecay * load_any(p.fin, a.fin_dtype, at) - p.fmul * x;
-                    store_fin(p.fin, a.fin_dtype, at, x);
-                }
-        }
+        if (p.fin && !p.fin_t) put_fin(a, p, (size_t)row * p.N + col, p.N - col, v);
         // columns N .. padN - 1 are written as zeros.  A symmetric result takes its lower half: row >= column here, mirrored below.
         if (p.out && col < padN && (!p.sym || row >= col)) {
             half8 h, l;
@@ -207,15 +227,21 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
                         o[32 + e] = l[e];
                     }
         }
-        if (p.outT)
+        if (p.outT || p.fin_t)
 #pragma unroll
             for (int e = 0; e < 8; ++e) tt[e] = v[e];
     }
-    if (!p.outT) return;
+    if (!p.outT && !p.fin_t) return;
     __syncthreads();
     for (int q = threadIdx.x; q < rows / 8 * TN; q += 256) {
         const int cl = (q >> 2) % TN, rl = (q / (4 * TN)) * 32 + (q & 3) * 8, row = r0 + rl, col = c0 + cl;
-        if (col >= p.N || row >= padM) continue;
+        if (p.fin_t && col < p.N && row < p.M) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = t[(rl + e) * (TN + 1) + cl];
+            put_fin(a, p, (size_t)col * p.M + row, p.M - row, v);
+        }
+        if (!p.outT || col >= p.N || row >= padM) continue;
         half8 h, l;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -446,7 +472,7 @@ struct Mat {
 };
 struct Mats {
     Mat m[MAX_MAT];
-    int count, dtype, nesterov;
+    int count, dtype, nesterov, planes;
     float mu;
     double eps;
 };
@@ -490,8 +516,17 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Mats a)
     if (threadIdx.x == 0) m.sums[b] = (s_acc[0] + s_acc[1]) + (s_acc[2] + s_acc[3]);
 }
 
+__device__ __forceinline__ void put_plane(_Float16* img, int row, int nchunk, int col, const float (&v)[4])
+{
+    half4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (_Float16)v[e];
+    *reinterpret_cast<half4*>(img + ((size_t)row * nchunk + (col >> 5)) * 32 + (col & 31)) = h;
+}
+
 // 64 x 64 elements of a matrix into both plane images.  The power of two 2^e takes the norm into [2^13, 2^14): exact, and every entry
-// below 2^14; the division by the norm itself waits for the products' epilogues (r).
+// below 2^14; the division by the norm itself waits for the products' epilogues (r).  A 16-bit matrix without momentum is one plane: fp16
+// holds the 8 or 11 bits of an entry exactly (down to 2^-38 of the norm, where the polynomial's slope of 485 is still far below half a step).
 __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
 {
     __shared__ double s_acc[4];
@@ -540,12 +575,14 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
         if (r0 + b < m.rows && c0 + a4 < pc * 32) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = tile[b][a4 + k];
-            put_planes(m.P, r0 + b, pc, c0 + a4, v);
+            if (a.planes == 1) put_plane(m.P, r0 + b, pc, c0 + a4, v);
+            else put_planes(m.P, r0 + b, pc, c0 + a4, v);
         }
         if (c0 + b < m.cols && r0 + a4 < ptc * 32) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = tile[a4 + k][b];
-            put_planes(m.PT, c0 + b, ptc, r0 + a4, v);
+            if (a.planes == 1) put_plane(m.PT, c0 + b, ptc, r0 + a4, v);
+            else put_planes(m.PT, c0 + b, ptc, r0 + a4, v);
         }
     }
 }
@@ -597,7 +634,7 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
     return ldexpf(1.0f, 15 - e);
 }
 
-int hop_plan(const Shape& s, int steps, int dtype)
+int hop_plan(const Shape& s, int steps, int dtype, int planes)
 {
     // steps of a hop: cheapest of the allowed lengths (a hop of h: 3 m^2 n + (4 h - 3) m^3 against h (3 m^2 n + m^3)); ties to the short one
     // (fp32: two steps a hop only from n = 2 m on, where it saves a fifth; nearer to square it saves less than 15 % and the error
@@ -609,7 +646,9 @@ int hop_plan(const Shape& s, int steps, int dtype)
         double c = 0.0;
         for (int left = steps; left > 0;) {
             const int k = left < h ? left : h;
-            c += 3.0 * (double)s.n + (4.0 * k - 3.0) * (double)s.m;
+            // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
+            c += left == steps && planes == 1 ? (1.0 + 2.0 * 2.0) * (double)s.n : 3.0 * 3.0 * (double)s.n;
+            c += 3.0 * (4.0 * k - 3.0) * (double)s.m;
             left -= k;
         }
         if (c < cost * 0.999) {
@@ -631,9 +670,9 @@ int norm_blocks(const Shape& s)
     return (int)(b < MAX_NORM_BLOCKS ? (b > 0 ? b : 1) : MAX_NORM_BLOCKS);
 }
 
-size_t layout(const Shape& s, int steps, int dtype, char* base, Buffers* b)
+size_t layout(const Shape& s, int steps, int dtype, int planes, char* base, Buffers* b)
 {
-    const int hop = hop_plan(s, steps, dtype);
+    const int hop = hop_plan(s, steps, dtype, planes);
     size_t at = 0;
     auto take = [&](size_t n) {
         char* p = base ? base + at : nullptr;
@@ -668,7 +707,7 @@ constexpr int MAX_CUTS = CUS;
 constexpr size_t PART_BYTES = (size_t)MAX_CUTS * 2 * 256 * 128 * sizeof(float);
 
 // Estimated cycles of the launch in every shape, tiles whole or cut; the cheapest is taken.
-Plan plan_of(const Prob* p, int count)
+Plan plan_of(const Prob* p, int count, int products)
 {
     Plan best{0, 0, 0, 0};
     double best_cost = 1e300;
@@ -683,7 +722,7 @@ Plan plan_of(const Prob* p, int count)
             kmax = p[i].kc > kmax ? p[i].kc : kmax;
         }
         if (tiles > (1 << 28) || units > (1 << 30)) continue;
-        const double cyc = SHAPES[s].cyc, epi = SHAPES[s].tm * SHAPES[s].tn / 8.0;
+        const double cyc = SHAPES[s].cyc * products / 3.0, epi = SHAPES[s].tm * SHAPES[s].tn / 8.0;
         // whole tiles only: as many rounds as it takes (unequal lengths: at least the longest one)
         const double rounds = (double)((tiles + CUS - 1) / CUS);
         double c = kmin == kmax ? rounds * (kmax * cyc + epi) : (double)units / CUS * cyc + kmax * cyc + rounds * epi;
@@ -706,7 +745,7 @@ Plan plan_of(const Prob* p, int count)
 }
 
 template <int WM, int WN, int PL, int PR, int NS>
-int launch_as(const Probs& a, const char* tag, double flops, hipStream_t stream)
+int launch_ring(const Probs& a, const char* tag, double flops, hipStream_t stream)
 {
     static mp::DynLds dyn;
     constexpr size_t ring = (size_t)NS * (64 * WM * 64 * PL + 64 * WN * 64 * PR), tile = (size_t)64 * WM * (64 * WN + 1) * sizeof(float);
@@ -722,10 +761,23 @@ int launch_as(const Probs& a, const char* tag, double flops, hipStream_t stream)
     return MP_OK;
 }
 
-int launch(Probs& a, const char* tag, hipStream_t stream)
+// Depth of the ring: what 144 KB hold (at most 8 chunks) where the launch has one workgroup a CU at most, else half of that so that two
+// share a CU (256 x 128: always one).
+template <int WM, int WN, int PL, int PR>
+int launch_as(const Probs& a, const char* tag, double flops, hipStream_t stream)
+{
+    constexpr int stage = 64 * WM * 64 * PL + 64 * WN * 64 * PR, deep = 147456 / stage < 8 ? 147456 / stage : 8;
+    constexpr int half = WM * WN >= 8 ? deep : (73728 / stage < 8 ? 73728 / stage : 8);
+    if (a.whole + a.cuts <= CUS) return launch_ring<WM, WN, PL, PR, deep>(a, tag, flops, stream);
+    return launch_ring<WM, WN, PL, PR, half>(a, tag, flops, stream);
+}
+
+// planes of the left and the right operands: (2, 2), (2, 1) or (1, 1)
+int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
 {
     if (a.count == 0) return MP_OK;
-    const Plan pl = plan_of(a.p, a.count);
+    const int products = left + right - 1;
+    const Plan pl = plan_of(a.p, a.count, products);
     const TileShape ts = SHAPES[pl.shape];
     if (pl.whole + pl.cuts == 0) return MP_EUNSUPPORTED;
     int64_t tiles = 0, units = 0;
@@ -738,7 +790,7 @@ int launch(Probs& a, const char* tag, hipStream_t stream)
         const int t = tiles_of(p.M, p.N, p.sym, ts.tm, ts.tn);
         tiles += t;
         units += (int64_t)t * p.kc;
-        flops += 6.0 * p.M * p.N * 32.0 * p.kc * (p.sym ? 0.5 : 1.0);
+        flops += 2.0 * products * p.M * p.N * 32.0 * p.kc * (p.sym ? 0.5 : 1.0);
     }
     a.tiles = (int)tiles;
     a.units = (int)units;
@@ -746,9 +798,14 @@ int launch(Probs& a, const char* tag, hipStream_t stream)
     a.cuts = pl.cuts;
     a.cut = pl.cut;
     a.cut0 = pl.whole == 0 ? 0 : pl.whole * a.p[0].kc;
-    if (pl.shape == 0) return launch_as<4, 2, 2, 2, 3>(a, tag, flops, stream);
-    if (pl.shape == 1) return launch_as<2, 2, 2, 2, 2>(a, tag, flops, stream);
-    return launch_as<1, 1, 2, 2, 4>(a, tag, flops, stream);
+#define NS_SHAPES(PL, PR)                                                                  \
+    return pl.shape == 0   ? launch_as<4, 2, PL, PR>(a, tag, flops, stream)                \
+           : pl.shape == 1 ? launch_as<2, 2, PL, PR>(a, tag, flops, stream)                \
+                           : launch_as<1, 1, PL, PR>(a, tag, flops, stream)
+    if (left == 2 && right == 2) NS_SHAPES(2, 2);
+    if (left == 2) NS_SHAPES(2, 1);
+    NS_SHAPES(1, 1);
+#undef NS_SHAPES
 }
 
 struct Update { int on; double lr, mu, decay; int nesterov, scale; };
@@ -767,7 +824,9 @@ size_t chunk_bytes(const int64_t* rows, const int64_t* cols, const int64_t* idx,
     size_t bytes = 0;
     for (int q = 0; q < k; ++q) {
         const Shape s = shape_of(rows[idx[q]], cols[idx[q]]);
-        bytes += layout(s, steps, dtype, nullptr, nullptr);
+        // (one size for both uses of 16-bit matrices: as they are, or with a momentum)
+        const size_t one = layout(s, steps, dtype, 1, nullptr, nullptr), two = layout(s, steps, dtype, 2, nullptr, nullptr);
+        bytes += one > two ? one : two;
     }
     return bytes + PART_BYTES;
 }
@@ -794,12 +853,13 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     int hop[MAX_MAT];
     Mats a;
     a.count = k; a.dtype = dtype; a.nesterov = up_.nesterov; a.mu = (float)up_.mu; a.eps = eps;
+    a.planes = dtype != MP_DTYPE_F32 && !mom ? 1 : 2;
     int64_t blocks = 0, tiles = 0;
     double elems = 0.0;
     for (int q = 0; q < k; ++q) {
         sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
-        hop[q] = hop_plan(sh[q], steps, dtype);
-        ws += layout(sh[q], steps, dtype, ws, &bf[q]);
+        hop[q] = hop_plan(sh[q], steps, dtype, a.planes);
+        ws += layout(sh[q], steps, dtype, a.planes, ws, &bf[q]);
         Mat& m = a.m[q];
         const bool tall = sh[q].rows > sh[q].cols;
         m.g = in[idx[q]];
@@ -857,7 +917,8 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
             if (first[q]) { p.rdev = bf[q].r; p.rpow = 2; }
             g.p[g.count++] = p;
         }
-        int rc = launch(g, "ns_gemm_kernel (gram)", stream);
+        const int xp = left == k && done[0] == 0 ? a.planes : 2;       // planes of X in this round of hops
+        int rc = launch(g, xp, xp, "ns_gemm_kernel (gram)", stream);
         if (rc) return rc;
         for (int s = 0; s < longest; ++s) {
             g.count = 0;
@@ -871,7 +932,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                 p.ca = (float)coef[0];
                 g.p[g.count++] = p;
             }
-            rc = launch(g, "ns_gemm_kernel (square)", stream);
+            rc = launch(g, 2, 2, "ns_gemm_kernel (square)", stream);
             if (rc) return rc;
             g.count = 0;
             for (int q = 0; q < k; ++q) {      // T = A Q (another step follows), R = Q R: independent, one launch
@@ -888,12 +949,12 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                     sR[q] = so;
                 }
             }
-            rc = launch(g, "ns_gemm_kernel (step)", stream);
+            rc = launch(g, 2, 2, "ns_gemm_kernel (step)", stream);
             if (rc) return rc;
             g.count = 0;
             for (int q = 0; q < k; ++q)        // A = T Q
                 if (s + 1 < len[q]) g.p[g.count++] = sym_prob(q, bf[q].T, bf[q].P[qbuf[q]], sT, sQ, bf[q].A, sA);
-            rc = launch(g, "ns_gemm_kernel (step)", stream);
+            rc = launch(g, 2, 2, "ns_gemm_kernel (step)", stream);
             if (rc) return rc;
         }
         g.count = 0;
@@ -904,16 +965,16 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
             Prob p{};
             const _Float16* R = reinterpret_cast<const _Float16*>(bf[q].P[rbuf[q]]);
             const _Float16* XT = reinterpret_cast<const _Float16*>(bf[q].XT);
-            const bool flip = last && tall;        // the result in the matrix's own orientation: X^T R
-            p.L = flip ? XT : R;
-            p.R = flip ? R : XT;
-            p.M = (int)(flip ? sh[q].n : sh[q].m);
-            p.N = (int)(flip ? sh[q].m : sh[q].n);
+            p.L = R;
+            p.R = XT;
+            p.M = (int)sh[q].m;
+            p.N = (int)sh[q].n;
             p.kc = chunks(sh[q].m);
             p.alpha = 1.0f / (sR[q] * (first[q] ? 1.0f : sX));
             if (first[q]) { p.rdev = bf[q].r; p.rpow = 1; }
             if (last) {
                 p.fin = out[idx[q]];
+                p.fin_t = tall;
                 if (up_.on) {
                     const double rr = (double)sh[q].rows, cc = (double)sh[q].cols;
                     const double sc = up_.scale == MP_MUON_SCALE_MATCH_RMS ? 0.2 * sqrt(rr > cc ? rr : cc) : up_.scale == MP_MUON_SCALE_ORIGINAL ? sqrt(rr > cc ? rr / cc : 1.0) : 1.0;
@@ -934,7 +995,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
             first[q] = false;
             g.p[g.count++] = p;
         }
-        rc = launch(g, "ns_gemm_kernel (apply)", stream);
+        rc = launch(g, 2, xp, "ns_gemm_kernel (apply)", stream);
         if (rc) return rc;
     }
     return MP_OK;
