@@ -43,16 +43,27 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     const float* rdev;       // alpha is multiplied by rdev^rpow
     int M, N, kc, oc, otc, rpow, sym, tiles_n, fin_t;
     float alpha, cb, ca, so, fmul, fdecay;
-    int tile0, unit0;        // first tile, first unit (a unit: one chunk of one tile) of the launch
 };
 struct Probs {
-    Prob p[MAX_PROB];
-    int count, tiles, units;      // totals
+    int tile0[MAX_PROB], unit0[MAX_PROB];      // first tile and first unit (one chunk of one tile) of every problem; behind the last: INT_MAX
+    int tiles, units;             // totals
     int whole;                    // tiles of the first `whole` workgroups, one each; the rest is cut into equal ranges of units
     int cut0, cut, cuts;          // the ranges: first unit, units a range, how many
     int fin_dtype, fin_update;    // fin_update: fin = fdecay * fin - fmul * value
     float* part;
+    int count;
+    Prob p[MAX_PROB];
 };
+
+// The entry of `starts` (ascending, INT_MAX behind the last) that `at` belongs to: one load by all lanes and a ballot.  The arguments come
+// from host memory, ~1 us a dependent read: a scalar search would pay that per entry.
+template <int N> __device__ __forceinline__ int which(const int (&starts)[N], int at)
+{
+    static_assert(N <= 64, "one entry a lane");
+    const int lane = threadIdx.x & 63;
+    const int v = lane < N ? starts[lane] : 0x7fffffff;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(v <= at)) - 1);
+}
 static_assert(sizeof(Probs) <= 3584, "travels in the kernel arguments");
 
 __host__ __device__ inline int chunks(int64_t k) { return (int)((k + 31) / 32); }
@@ -181,85 +192,124 @@ __device__ __forceinline__ void put_fin(const Probs& a, const Prob& p, size_t at
             if (e < left) store_fin(p.fin, a.fin_dtype, at + e, v[e]);
 }
 
-// `rows` (a multiple of 32) x TN accumulators at (r0, c0) of the product, in LDS with row stride TN + 1, to wherever the problem wants
-// them.  Through LDS because a result goes out in two orientations: eight consecutive elements a lane (16 bytes of each plane, 64-byte
-// runs) either way.
-template <int TN>
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+
+// fp16 planes of x packed into 32 bits: h below, l above
+__device__ __forceinline__ unsigned planes_of(float x)
+{
+    const _Float16 h = (_Float16)x, l = (_Float16)(x - (float)h);
+    unsigned short hb, lb;
+    __builtin_memcpy(&hb, &h, 2);
+    __builtin_memcpy(&lb, &l, 2);
+    return (unsigned)hb | ((unsigned)lb << 16);
+}
+// eight packed elements to the h and l runs of an image (16 bytes each)
+__device__ __forceinline__ void put_packed(_Float16* o, const unsigned (&w)[8])
+{
+    uint4v h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        h[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x05040100);
+        l[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302);
+    }
+    *reinterpret_cast<uint4v*>(o) = h;
+    *reinterpret_cast<uint4v*>(o + 32) = l;
+}
+__device__ __forceinline__ void put_one(_Float16* o, unsigned w)
+{
+    reinterpret_cast<unsigned short*>(o)[0] = (unsigned short)w;
+    reinterpret_cast<unsigned short*>(o)[32] = (unsigned short)(w >> 16);
+}
+
+constexpr int TPAD = 4;      // a tile's rows in LDS are TN + 4 floats apart: 16-byte pieces, columns spread over the banks
+
+// `rows` (a multiple of 32) x TN accumulators at (r0, c0) of the product, in LDS (COPIES of them, to be added in order), to wherever the
+// problem wants them.  Through LDS because a result goes out in two orientations: eight consecutive elements a lane (16 bytes of each
+// plane, 64-byte runs) either way.  The first pass forms the values, writes the row orientation and leaves them packed for the second.
+// (With one wave a SIMD this is instruction time: 64 x 64 took 5.6 us with values formed and rounded in both passes.)
+template <int TN, int COPIES>
 __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t, int rows, int r0, int c0)
 {
-    const float alpha = alpha_of(p);
-    const int padN = p.oc * 32, padM = p.otc * 32;
+    constexpr int S = TN + TPAD;
+    const float so = p.fin ? 1.0f : p.so, alpha = alpha_of(p) * so, cb = p.cb * so, ca = p.ca * so;
+    const int padN = p.oc * 32, padM = p.otc * 32, copy = rows * S;
+    const bool diagonal = p.ca != 0.0f && r0 < c0 + TN && c0 < r0 + rows, edge = c0 + TN > p.N;
+#pragma unroll 2
     for (int q = threadIdx.x; q < rows * (TN / 8); q += 256) {
         const int rl = q / (TN / 8), cl = q % (TN / 8) * 8, row = r0 + rl, col = c0 + cl;
-        if (row >= p.M) continue;
-        float* tt = t + rl * (TN + 1) + cl;
+        float* tt = t + rl * S + cl;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = alpha * tt[e];
-        if (p.C && col < padN) {
+        for (int k = 0; k < COPIES; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(tt + k * copy), y = *reinterpret_cast<const float4*>(tt + k * copy + 4);
+            const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k == 0 ? w[e] : v[e] + w[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= alpha;
+        if (p.C && row < p.M && col < padN) {
             const half8* c = reinterpret_cast<const half8*>(p.C + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31));
             const half8 h = c[0], l = c[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += p.cb * ((float)h[e] + (float)l[e]);
+            for (int e = 0; e < 8; ++e) v[e] += cb * ((float)h[e] + (float)l[e]);
         }
+        if (diagonal)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (row == col + e) v[e] += p.ca;
-        if (p.fin && !p.fin_t) put_fin(a, p, (size_t)row * p.N + col, p.N - col, v);
-        // columns N .. padN - 1 are written as zeros.  A symmetric result takes its lower half: row >= column here, mirrored below.
-        if (p.out && col < padN && (!p.sym || row >= col)) {
-            half8 h, l;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = col + e < p.N ? v[e] * p.so : 0.0f;
-                h[e] = (_Float16)x;
-                l[e] = (_Float16)(x - (float)h[e]);
+            for (int e = 0; e < 8; ++e) v[e] += row == col + e ? ca : 0.0f;
+        if (p.fin) {
+            if (!p.fin_t) {
+                if (row < p.M) put_fin(a, p, (size_t)row * p.N + col, p.N - col, v);
+            } else {
+                *reinterpret_cast<float4*>(tt) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(tt + 4) = make_float4(v[4], v[5], v[6], v[7]);
             }
+            continue;
+        }
+        // columns N .. padN - 1 and rows M .. padM - 1 are zeros
+        if (edge)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = col + e < p.N ? v[e] : 0.0f;
+        unsigned w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = row < p.M ? planes_of(v[e]) : 0u;
+        uint4v* wt = reinterpret_cast<uint4v*>(tt);
+        wt[0] = uint4v{w[0], w[1], w[2], w[3]};
+        wt[1] = uint4v{w[4], w[5], w[6], w[7]};
+        // a symmetric result takes its lower half: row >= column here, mirrored below
+        if (row < p.M && col < padN && (!p.sym || row >= col)) {
             _Float16* o = p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31);
-            if (!p.sym || row >= col + 7) {
-                *reinterpret_cast<half8*>(o) = h;
-                *reinterpret_cast<half8*>(o + 32) = l;
-            } else
+            if (!p.sym || row >= col + 7) put_packed(o, w);
+            else
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (row >= col + e) {
-                        o[e] = h[e];
-                        o[32 + e] = l[e];
-                    }
+                    if (row >= col + e) put_one(o + e, w[e]);
         }
-        if (p.outT || p.fin_t)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) tt[e] = v[e];
     }
-    if (!p.outT && !p.fin_t) return;
+    if (p.fin && !p.fin_t) return;
     __syncthreads();
+#pragma unroll 2
     for (int q = threadIdx.x; q < rows / 8 * TN; q += 256) {
         const int cl = (q >> 2) % TN, rl = (q / (4 * TN)) * 32 + (q & 3) * 8, row = r0 + rl, col = c0 + cl;
-        if (p.fin_t && col < p.N && row < p.M) {
+        if (col >= p.N) continue;
+        const float* tt = t + rl * S + cl;
+        if (p.fin) {
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = t[(rl + e) * (TN + 1) + cl];
-            put_fin(a, p, (size_t)col * p.M + row, p.M - row, v);
+            for (int e = 0; e < 8; ++e) v[e] = tt[e * S];
+            if (row < p.M) put_fin(a, p, (size_t)col * p.M + row, p.M - row, v);
+            continue;
         }
-        if (!p.outT || col >= p.N || row >= padM) continue;
-        half8 h, l;
+        if (row >= padM) continue;
+        unsigned w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x = row + e < p.M ? t[(rl + e) * (TN + 1) + cl] * p.so : 0.0f;
-            h[e] = (_Float16)x;
-            l[e] = (_Float16)(x - (float)h[e]);
-        }
+        for (int e = 0; e < 8; ++e) w[e] = reinterpret_cast<const unsigned*>(tt)[e * S];
         _Float16* o = p.outT + ((size_t)col * p.otc + (row >> 5)) * 64 + (row & 31);
-        if (!p.sym || row > col) {
-            *reinterpret_cast<half8*>(o) = h;
-            *reinterpret_cast<half8*>(o + 32) = l;
-        } else
+        if (!p.sym || row > col) put_packed(o, w);
+        else
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (row + e > col) {        // (row + e == col was written above)
-                    o[e] = h[e];
-                    o[32 + e] = l[e];
-                }
+                if (row + e > col) put_one(o + e, w[e]);        // (row + e == col was written above)
     }
 }
 
@@ -270,16 +320,26 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
 // source address of the load, so that the 32 rows of a fragment read meet each bank group equally often.
 template <int PL> __device__ __forceinline__ int swz(int row) { return PL == 2 ? row & 7 : (row >> 1) & 3; }
 
-template <int WM, int WN, int PL, int PR, int NS>
-__global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Probs a)
+// KW: the four waves share a (32 WM) x (32 WN) tile by K instead, wave v taking chunks v, v + 4, ..: each with a ring of its own and no
+// meeting at all; their sums meet in LDS at the end, added in the order of the waves.  For 64 x 64 tiles, where a wave of the shared form has
+// three products between two meetings (136 tiles of K = 1024: 15 us against <KWTIME>).
+template <int WM, int WN, int PL, int PR, int NS, bool KW>
+__global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 {
-    constexpr int TM = 64 * WM, TN = 64 * WN, BL = TM * 64 * PL, BR = TN * 64 * PR, STAGE = BL + BR;
-    constexpr int NL = BL / 4096, NR = BR / 4096;                  // load instructions a wave and stage
+    constexpr int WAVES = KW ? 1 : 4;                              // waves that load a stage together
+    constexpr int TM = KW ? 32 * WM : 64 * WM, TN = KW ? 32 * WN : 64 * WN, BL = TM * 64 * PL, BR = TN * 64 * PR, STAGE = BL + BR;
+    constexpr int NL = BL / (1024 * WAVES), NR = BR / (1024 * WAVES);      // load instructions a wave and stage
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int fr = lane & 31, fh = lane >> 5;                      // fragment row, k half
-    const int wm = (wave >> 1) * WM * 32, wn = (wave & 1) * WN * 32;
-    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)lds + wave * 1024);
+    const int wm = KW ? 0 : (wave >> 1) * WM * 32, wn = KW ? 0 : (wave & 1) * WN * 32;
+    char* const ring = KW ? lds + wave * (NS * STAGE) : lds;
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)lds + wave * (KW ? NS * STAGE : 1024));
+    const int lt = KW ? lane : (int)threadIdx.x;                   // this lane among those that load a stage
+    auto meet = [&] {       // everybody who reads a stage has it, and has finished with the one before
+        if constexpr (KW) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        else lds_barrier();
+    };
 
     // the workgroups of one XCD (every eighth) take consecutive tiles / ranges: they share operand rows through its L2
     const int total = a.whole + a.cuts, bid = blockIdx.x;
@@ -289,22 +349,20 @@ __global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Prob
         const int per = n >> 3, rest = n & 7, x = b & 7, y = b >> 3;
         w = base + x * per + (x < rest ? x : rest) + y;
     }
-    int u, uend;            // this workgroup's units
-    if (w < a.whole) {
-        int i = 0;
-        while (i + 1 < a.count && w >= a.p[i + 1].tile0) ++i;
-        u = a.p[i].unit0 + (w - a.p[i].tile0) * a.p[i].kc;
-        uend = u + a.p[i].kc;
-    } else {
-        u = a.cut0 + (w - a.whole) * a.cut;
-        uend = u + a.cut < a.units ? u + a.cut : a.units;
-    }
-    for (int piece = 0; u < uend; ++piece) {
-        int i = 0;
-        while (i + 1 < a.count && u >= a.p[i + 1].unit0) ++i;      // uniform: scalar loop over <= 24 entries
-        const Prob& p = a.p[i];
-        const int tile = (u - p.unit0) / p.kc, c0 = (u - p.unit0) - tile * p.kc;
-        const int n = uend - u < p.kc - c0 ? uend - u : p.kc - c0;      // chunks of this piece (>= 1)
+    // this workgroup's work: one tile, or the units [u, uend) piece by piece
+    int u = a.cut0 + (w - a.whole) * a.cut;
+    const int uend = u + a.cut < a.units ? u + a.cut : a.units;
+    for (int piece = 0;; ++piece) {
+        const bool one = w < a.whole;
+        const int i = one ? which(a.tile0, w) : which(a.unit0, u);
+        const Prob p = a.p[i];
+        int tile = w - a.tile0[i], c0 = 0, n = p.kc;                    // chunks [c0, c0 + n) of the tile, n >= 1
+        if (!one) {
+            const int local = u - a.unit0[i];
+            tile = local / p.kc;
+            c0 = local - tile * p.kc;
+            n = uend - u < p.kc - c0 ? uend - u : p.kc - c0;
+        }
         int m0, n0;
         tile_at(p, tile, TM, TN, m0, n0);
 
@@ -313,23 +371,25 @@ __global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Prob
         constexpr int UL = 4 * PL, UR = 4 * PR;        // 16-byte units a row
 #pragma unroll
         for (int k = 0; k < NL; ++k) {
-            const int lr = (k * 256 + threadIdx.x) / UL, row = m0 + lr < p.M ? lr : p.M - 1 - m0;
+            const int lr = (k * 64 * WAVES + lt) / UL, row = m0 + lr < p.M ? lr : p.M - 1 - m0;
             offL[k] = (unsigned)row * (unsigned)(p.kc * 64 * PL) + ((lane % UL) ^ swz<PL>(lr)) * 16;
         }
 #pragma unroll
         for (int k = 0; k < NR; ++k) {
-            const int lr = (k * 256 + threadIdx.x) / UR, row = n0 + lr < p.N ? lr : p.N - 1 - n0;
+            const int lr = (k * 64 * WAVES + lt) / UR, row = n0 + lr < p.N ? lr : p.N - 1 - n0;
             offR[k] = (unsigned)row * (unsigned)(p.kc * 64 * PR) + ((lane % UR) ^ swz<PR>(lr)) * 16;
         }
-        const char* srcL = reinterpret_cast<const char*>(p.L) + ((size_t)m0 * p.kc + c0) * (64 * PL);
-        const char* srcR = reinterpret_cast<const char*>(p.R) + ((size_t)n0 * p.kc + c0) * (64 * PR);
+        const int v = KW ? __builtin_amdgcn_readfirstlane(wave) : 0, step = KW ? 4 : 1;
+        const int nw = KW ? (n - v + 3) / 4 : n;       // chunks of this wave: c0 + v, c0 + v + step, ..
+        const char* srcL = reinterpret_cast<const char*>(p.L) + ((size_t)m0 * p.kc + c0 + v) * (64 * PL);
+        const char* srcR = reinterpret_cast<const char*>(p.R) + ((size_t)n0 * p.kc + c0 + v) * (64 * PR);
         auto fetch_one = [&](int buf, int k) {         // instruction k of NL + NR; the last one moves on to the next chunk
             const unsigned d = lds0 + buf * STAGE;
-            if (k < NL) to_lds16(srcL, offL[k < NL ? k : 0], d + k * 4096);
-            else to_lds16(srcR, offR[k >= NL ? k - NL : 0], d + BL + (k - NL) * 4096);
+            if (k < NL) to_lds16(srcL, offL[k < NL ? k : 0], d + k * (1024 * WAVES));
+            else to_lds16(srcR, offR[k >= NL ? k - NL : 0], d + BL + (k - NL) * (1024 * WAVES));
             if (k == NL + NR - 1) {
-                srcL += 64 * PL;
-                srcR += 64 * PR;
+                srcL += step * 64 * PL;
+                srcR += step * 64 * PR;
             }
         };
         float16v acc[WM][WN];
@@ -344,7 +404,7 @@ __global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Prob
         half8 fl[2][WM][PL], fq[2][WN][PR];
         constexpr int READS = WM * PL + WN * PR, PRODS = (PL + PR - 1) * WM * WN, FETCHES = NL + NR;
         auto read_one = [&](int buf, int ks, int k) {
-            const char* s = lds + buf * STAGE;
+            const char* s = ring + buf * STAGE;
             if (k < WM * PL) {
                 const int x = k % WM, pl = k / WM % PL;
                 fl[ks][x][pl] = *reinterpret_cast<const half8*>(s + (rowL + 32 * x) * (64 * PL) + (((pl * 4 + ks * 2 + fh) ^ swz<PL>(rowL)) * 16));
@@ -371,63 +431,80 @@ __global__ __launch_bounds__(256, WM * WN >= 8 ? 1 : 2) void ns_gemm_kernel(Prob
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        const int ahead = n < NS ? n : NS;
+        const int ahead = nw < NS ? nw : NS;
         for (int k = 0; k < ahead; ++k)
 #pragma unroll
             for (int r = 0; r < FETCHES; ++r) fetch_one(k, r);
-        if (n >= NS) wait_vm<(NS - 1) * FETCHES>();
+        if (nw >= NS) wait_vm<(NS - 1) * FETCHES>();
         else wait_vm<0>();
-        lds_barrier();
+        meet();
+        if (nw > 0)
 #pragma unroll
-        for (int r = 0; r < READS; ++r) read_one(0, 0, r);
+            for (int r = 0; r < READS; ++r) read_one(0, 0, r);
         int buf = 0, c = 0;
-        for (; c + NS < n; ++c) {       // chunks up to c + NS - 1 are on their way
+        for (; c + NS < nw; ++c) {       // chunks up to c + NS - 1 are on their way
             multiply(0, true, buf, false, 0);
             wait_vm<(NS - 2) * FETCHES>();
-            lds_barrier();
+            meet();
             const int next = buf + 1 < NS ? buf + 1 : 0;
             multiply(1, true, next, true, buf);
             buf = next;
         }
-        for (; c < n; ++c) {            // the last NS: nothing more to load
+        for (; c < nw; ++c) {            // the last NS: nothing more to load
             multiply(0, true, buf, false, 0);
             wait_vm<0>();
-            lds_barrier();
+            meet();
             const int next = buf + 1 < NS ? buf + 1 : 0;
-            multiply(1, c + 1 < n, next, false, 0);
+            multiply(1, c + 1 < nw, next, false, 0);
             buf = next;
         }
         // (nobody reads the buffers any more: the last meeting was behind the last fragment reads)
-        float* t = reinterpret_cast<float*>(lds);
+        if constexpr (KW) __syncthreads();
+        float* const t = reinterpret_cast<float*>(lds);
+        float* const mine = KW ? t + wave * (TM * (TN + TPAD)) : t;
 #pragma unroll
         for (int x = 0; x < WM; ++x)
 #pragma unroll
             for (int y = 0; y < WN; ++y)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)      // register r of lane q: row (r & 3) + 8 (r >> 2) + 4 (q >> 5), column q & 31
-                    t[(wm + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * fh) * (TN + 1) + wn + 32 * y + fr] = acc[x][y][r];
+                    mine[(wm + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * fh) * (TN + TPAD) + wn + 32 * y + fr] = acc[x][y][r];
         __syncthreads();
-        if (n == p.kc) epilogue<TN>(a, p, t, TM, m0, n0);
+        if (n == p.kc) epilogue<TN, KW ? 4 : 1>(a, p, t, TM, m0, n0);
         else {        // a range's first piece and its last one may be parts of tiles: two slots a range
-            float* o = a.part + (size_t)(2 * (w - a.whole) + (piece > 0)) * (TM * TN);
-            for (int q = threadIdx.x; q < TM * TN; q += 256) o[q] = t[q / TN * (TN + 1) + q % TN];
+            float4* o = reinterpret_cast<float4*>(a.part + (size_t)(2 * (w - a.whole) + (piece > 0)) * (TM * TN));
+#pragma unroll 4
+            for (int q = threadIdx.x; q < TM * TN / 4; q += 256) {
+                const float* tt = t + q / (TN / 4) * (TN + TPAD) + q % (TN / 4) * 4;
+                float4 x = *reinterpret_cast<const float4*>(tt);
+                if constexpr (KW)
+#pragma unroll
+                    for (int k = 1; k < 4; ++k) {
+                        const float4 y = *reinterpret_cast<const float4*>(tt + k * TM * (TN + TPAD));
+                        x.x += y.x;
+                        x.y += y.y;
+                        x.z += y.z;
+                        x.w += y.w;
+                    }
+                o[q] = x;
+            }
         }
-        __syncthreads();
         u += n;
+        if (one || u >= uend) break;
+        __syncthreads();
     }
 }
 
 // Tiles that the ranges cut: the parts' accumulators added in the order of the ranges, then the same epilogue.  A workgroup takes 32 rows.
-template <int WM, int WN>
+template <int TM, int TN>
 __global__ __launch_bounds__(256) void ns_join_kernel(Probs a, int tile_first)
 {
-    constexpr int TM = 64 * WM, TN = 64 * WN, STRIPS = TM / 32, PER = 32 * TN / 1024;
-    __shared__ float t[32 * (TN + 1)];
+    constexpr int STRIPS = TM / 32, PER = 32 * TN / 1024;
+    __shared__ __align__(16) float t[32 * (TN + TPAD)];
     const int strip = blockIdx.x % STRIPS, tile = tile_first + blockIdx.x / STRIPS;
-    int i = 0;
-    while (i + 1 < a.count && tile >= a.p[i + 1].tile0) ++i;
-    const Prob& p = a.p[i];
-    const int u0 = p.unit0 + (tile - p.tile0) * p.kc;
+    const int i = which(a.tile0, tile);
+    const Prob p = a.p[i];
+    const int u0 = a.unit0[i] + (tile - a.tile0[i]) * p.kc;
     const int w0 = (u0 - a.cut0) / a.cut, w1 = (u0 + p.kc - 1 - a.cut0) / a.cut;
     if (w0 == w1) return;           // one range had it whole
     float4 acc[PER];
@@ -448,16 +525,12 @@ __global__ __launch_bounds__(256) void ns_join_kernel(Probs a, int tile_first)
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         const int at = (k * 256 + threadIdx.x) * 4;
-        float* d = t + at / TN * (TN + 1) + at % TN;
-        d[0] = acc[k].x;
-        d[1] = acc[k].y;
-        d[2] = acc[k].z;
-        d[3] = acc[k].w;
+        *reinterpret_cast<float4*>(t + at / TN * (TN + TPAD) + at % TN) = acc[k];
     }
     __syncthreads();
     int m0, n0;
-    tile_at(p, tile - p.tile0, TM, TN, m0, n0);
-    epilogue<TN>(a, p, t, 32, m0 + strip * 32, n0);
+    tile_at(p, tile - a.tile0[i], TM, TN, m0, n0);
+    epilogue<TN, 1>(a, p, t, 32, m0 + strip * 32, n0);
 }
 
 // ---- momentum, norm, planes -------------------------------------------------------------------------------------------------------
@@ -468,9 +541,10 @@ struct Mat {
     float* r;            // X = (U 2^e) * r
     _Float16* P;         // planes of U 2^e, [rows][chunks(cols)]
     _Float16* PT;        // of its transpose, [cols][chunks(rows)]
-    int rows, cols, blocks, blk0, tile0;
+    int rows, cols, blocks;
 };
 struct Mats {
+    int blk0[MAX_MAT], tile0[MAX_MAT];       // first workgroup of every matrix in ns_norm_kernel / ns_planes_kernel; behind the last: INT_MAX
     Mat m[MAX_MAT];
     int count, dtype, nesterov, planes;
     float mu;
@@ -483,11 +557,10 @@ static_assert(sizeof(Mats) <= 3584, "travels in the kernel arguments");
 __global__ __launch_bounds__(256) void ns_norm_kernel(Mats a)
 {
     __shared__ double s_acc[4];
-    int i = 0;
-    while (i + 1 < a.count && (int)blockIdx.x >= a.m[i + 1].blk0) ++i;
-    const Mat& m = a.m[i];
+    const int i = which(a.blk0, blockIdx.x);
+    const Mat m = a.m[i];
     const size_t n = (size_t)m.rows * m.cols;
-    const int b = blockIdx.x - m.blk0;
+    const int b = blockIdx.x - a.blk0[i];
     double s = 0.0;
 #pragma unroll 4
     for (size_t e = ((size_t)b * 256 + threadIdx.x) * 4; e < n; e += (size_t)m.blocks * 1024) {
@@ -531,9 +604,8 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
 {
     __shared__ double s_acc[4];
     __shared__ float tile[64][65];
-    int i = 0;
-    while (i + 1 < a.count && (int)blockIdx.x >= a.m[i + 1].tile0) ++i;
-    const Mat& m = a.m[i];
+    const int i = which(a.tile0, blockIdx.x);
+    const Mat m = a.m[i];
     double s = 0.0;
     for (int k = threadIdx.x; k < m.blocks; k += 256) s += m.sums[k];
 #pragma unroll
@@ -546,7 +618,7 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
         (void)frexp(norm, &e);        // norm in [2^(e-1), 2^e)
         e = 14 - e;
     }
-    const int local = blockIdx.x - m.tile0, tn = (m.cols + 63) / 64;
+    const int local = blockIdx.x - a.tile0[i], tn = (m.cols + 63) / 64;
     const int r0 = (local / tn) * 64, c0 = (local % tn) * 64;
     if (local == 0 && threadIdx.x == 0) *m.r = (float)(1.0 / ldexp(norm > a.eps || norm != norm ? norm : a.eps, e));
     const int tc = (threadIdx.x & 15) * 4, tr = threadIdx.x >> 4;
@@ -699,9 +771,9 @@ constexpr int CUS = 256;
 // What a launch does: tile size, tiles taken whole (one a workgroup) and the rest cut into equal ranges of (tile, chunk) units.
 struct Plan { int shape, whole, cuts, cut; };
 // Tile shapes.  cyc: cycles of a chunk on one CU (three plane products), from the MFMA time of 256 x 128, LDS traffic of the others
-// (reads and arrivals: 256 x 128 3/4 of its MFMA time, 128 x 128 1.0, 64 x 64 1.5).
+// (reads and arrivals: 256 x 128 3/4 of its MFMA time, 128 x 128 1.0, 64 x 64 1.3).
 struct TileShape { int tm, tn; double cyc; };
-constexpr TileShape SHAPES[3] = {{256, 128, 1900.0}, {128, 128, 1100.0}, {64, 64, 420.0}};
+constexpr TileShape SHAPES[3] = {{256, 128, 1900.0}, {128, 128, 1100.0}, {64, 64, 330.0}};
 constexpr int MAX_CUTS = CUS;
 // accumulators of the cut tiles: two slots a range
 constexpr size_t PART_BYTES = (size_t)MAX_CUTS * 2 * 256 * 128 * sizeof(float);
@@ -744,32 +816,33 @@ Plan plan_of(const Prob* p, int count, int products)
     return best;
 }
 
-template <int WM, int WN, int PL, int PR, int NS>
+template <int WM, int WN, int PL, int PR, int NS, bool KW>
 int launch_ring(const Probs& a, const char* tag, double flops, hipStream_t stream)
 {
     static mp::DynLds dyn;
-    constexpr size_t ring = (size_t)NS * (64 * WM * 64 * PL + 64 * WN * 64 * PR), tile = (size_t)64 * WM * (64 * WN + 1) * sizeof(float);
+    constexpr int TM = KW ? 32 * WM : 64 * WM, TN = KW ? 32 * WN : 64 * WN, RINGS = KW ? 4 : 1;
+    constexpr size_t ring = (size_t)RINGS * NS * 64 * (TM * PL + TN * PR), tile = (size_t)RINGS * TM * (TN + TPAD) * sizeof(float);
     constexpr size_t smem = ring > tile ? ring : tile;
-    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS>), smem)) return MP_ELAUNCH;
-    MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS>), dim3((unsigned)(a.whole + a.cuts)), dim3(256), smem, stream, a);
+    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), smem)) return MP_ELAUNCH;
+    MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), dim3((unsigned)(a.whole + a.cuts)), dim3(256), smem, stream, a);
     MP_CHECK_LAUNCH();
     if (a.cuts) {
-        int first = a.whole;        // (whole > 0 only with equal lengths: tile and unit order agree)
-        MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<WM, WN>), dim3((unsigned)(a.tiles - first) * 2 * WM), dim3(256), 0, stream, a, first);
+        const int first = a.whole;        // (whole > 0 only with equal lengths: tile and unit order agree)
+        MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<TM, TN>), dim3((unsigned)(a.tiles - first) * (TM / 32)), dim3(256), 0, stream, a, first);
         MP_CHECK_LAUNCH();
     }
     return MP_OK;
 }
 
 // Depth of the ring: what 144 KB hold (at most 8 chunks) where the launch has one workgroup a CU at most, else half of that so that two
-// share a CU (256 x 128: always one).
-template <int WM, int WN, int PL, int PR>
+// share a CU (256 x 128 and the K-sharing 64 x 64: always one).
+template <int WM, int WN, int PL, int PR, bool KW>
 int launch_as(const Probs& a, const char* tag, double flops, hipStream_t stream)
 {
-    constexpr int stage = 64 * WM * 64 * PL + 64 * WN * 64 * PR, deep = 147456 / stage < 8 ? 147456 / stage : 8;
-    constexpr int half = WM * WN >= 8 ? deep : (73728 / stage < 8 ? 73728 / stage : 8);
-    if (a.whole + a.cuts <= CUS) return launch_ring<WM, WN, PL, PR, deep>(a, tag, flops, stream);
-    return launch_ring<WM, WN, PL, PR, half>(a, tag, flops, stream);
+    constexpr int lds = 147456, stage = KW ? 4 * 64 * 32 * (WM * PL + WN * PR) : 64 * 64 * (WM * PL + WN * PR);
+    constexpr int deep = lds / stage < 8 ? lds / stage : 8, half = KW || WM * WN >= 8 ? deep : (lds / 2 / stage < 8 ? lds / 2 / stage : 8);
+    if (a.whole + a.cuts <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW>(a, tag, flops, stream);
+    return launch_ring<WM, WN, PL, PR, half, KW>(a, tag, flops, stream);
 }
 
 // planes of the left and the right operands: (2, 2), (2, 1) or (1, 1)
@@ -785,13 +858,14 @@ int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
     for (int i = 0; i < a.count; ++i) {
         Prob& p = a.p[i];
         p.tiles_n = (p.N + ts.tn - 1) / ts.tn;
-        p.tile0 = (int)tiles;
-        p.unit0 = (int)units;
+        a.tile0[i] = (int)tiles;
+        a.unit0[i] = (int)units;
         const int t = tiles_of(p.M, p.N, p.sym, ts.tm, ts.tn);
         tiles += t;
         units += (int64_t)t * p.kc;
         flops += 2.0 * products * p.M * p.N * 32.0 * p.kc * (p.sym ? 0.5 : 1.0);
     }
+    for (int i = a.count; i < MAX_PROB; ++i) a.tile0[i] = a.unit0[i] = 0x7fffffff;
     a.tiles = (int)tiles;
     a.units = (int)units;
     a.whole = pl.whole;
@@ -799,9 +873,9 @@ int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
     a.cut = pl.cut;
     a.cut0 = pl.whole == 0 ? 0 : pl.whole * a.p[0].kc;
 #define NS_SHAPES(PL, PR)                                                                  \
-    return pl.shape == 0   ? launch_as<4, 2, PL, PR>(a, tag, flops, stream)                \
-           : pl.shape == 1 ? launch_as<2, 2, PL, PR>(a, tag, flops, stream)                \
-                           : launch_as<1, 1, PL, PR>(a, tag, flops, stream)
+    return pl.shape == 0   ? launch_as<4, 2, PL, PR, false>(a, tag, flops, stream)         \
+           : pl.shape == 1 ? launch_as<2, 2, PL, PR, false>(a, tag, flops, stream)         \
+                           : launch_as<2, 2, PL, PR, true>(a, tag, flops, stream)
     if (left == 2 && right == 2) NS_SHAPES(2, 2);
     if (left == 2) NS_SHAPES(2, 1);
     NS_SHAPES(1, 1);
@@ -870,13 +944,13 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
         m.PT = reinterpret_cast<_Float16*>(tall ? bf[q].X : bf[q].XT);
         m.rows = (int)sh[q].rows; m.cols = (int)sh[q].cols;
         m.blocks = norm_blocks(sh[q]);
-        m.blk0 = (int)blocks;
-        m.tile0 = (int)tiles;
+        a.blk0[q] = (int)blocks;
+        a.tile0[q] = (int)tiles;
         blocks += m.blocks;
         tiles += ((sh[q].rows + 63) / 64) * ((sh[q].cols + 63) / 64);
         elems += (double)sh[q].rows * (double)sh[q].cols;
     }
-    if (tiles > 0x7fffffff) return MP_EUNSUPPORTED;
+    for (int q = k; q < MAX_MAT; ++q) a.blk0[q] = a.tile0[q] = 0x7fffffff;
     const double esz = dtype == MP_DTYPE_F32 ? 4.0 : 2.0;
     MP_LAUNCH("ns_norm_kernel", 2.0 * elems, elems * (esz + (mom ? 8.0 : 0.0)), ns_norm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
     MP_CHECK_LAUNCH();
