@@ -43,12 +43,14 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     const float* rdev;       // alpha is multiplied by rdev^rpow
     int M, N, kc, oc, otc, rpow, sym, tiles_n, fin_t;
     float alpha, cb, ca, so, fmul, fdecay;
+    int tiles, seg;          // tiles of the result; chunks of a segment of K (kc: not cut)
 };
+// A launch's work items, one a workgroup: the first `whole` tiles uncut, then the rest in segments of K.  Items are ordered by segment, then by
+// tile: neighbours share operand rows, not just the tile.  equal: all problems have one K, the rest is `rest` tiles x segments; else every
+// problem has segments of its own.
 struct Probs {
-    int tile0[MAX_PROB], unit0[MAX_PROB];      // first tile and first unit (one chunk of one tile) of every problem; behind the last: INT_MAX
-    int tiles, units;             // totals
-    int whole;                    // tiles of the first `whole` workgroups, one each; the rest is cut into equal ranges of units
-    int cut0, cut, cuts;          // the ranges: first unit, units a range, how many
+    int tile0[MAX_PROB], item0[MAX_PROB];      // first tile and first item of every problem; behind the last: INT_MAX
+    int tiles, items, whole, rest, equal;
     int fin_dtype, fin_update;    // fin_update: fin = fdecay * fin - fmul * value
     float* part;
     int count;
@@ -287,7 +289,7 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
         }
     }
     if (p.fin && !p.fin_t) return;
-    __syncthreads();
+    lds_barrier();          // (not __syncthreads: it would wait for the stores above)
 #pragma unroll 2
     for (int q = threadIdx.x; q < rows / 8 * TN; q += 256) {
         const int cl = (q >> 2) % TN, rl = (q / (4 * TN)) * 32 + (q & 3) * 8, row = r0 + rl, col = c0 + cl;
@@ -341,28 +343,24 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
         else lds_barrier();
     };
 
-    // the workgroups of one XCD (every eighth) take consecutive tiles / ranges: they share operand rows through its L2
-    const int total = a.whole + a.cuts, bid = blockIdx.x;
-    int w = bid;
+    // the workgroups of one XCD (every eighth) take consecutive items: they share operand rows through its L2
+    const int bid = blockIdx.x;
+    int w;
     {
-        const int base = bid < a.whole ? 0 : a.whole, n = bid < a.whole ? a.whole : total - a.whole, b = bid - base;
+        const int base = bid < a.whole ? 0 : a.whole, n = bid < a.whole ? a.whole : a.items - a.whole, b = bid - base;
         const int per = n >> 3, rest = n & 7, x = b & 7, y = b >> 3;
         w = base + x * per + (x < rest ? x : rest) + y;
     }
-    // this workgroup's work: one tile, or the units [u, uend) piece by piece
-    int u = a.cut0 + (w - a.whole) * a.cut;
-    const int uend = u + a.cut < a.units ? u + a.cut : a.units;
-    for (int piece = 0;; ++piece) {
-        const bool one = w < a.whole;
-        const int i = one ? which(a.tile0, w) : which(a.unit0, u);
+    {
+        const int i = w < a.whole ? which(a.tile0, w) : a.equal ? which(a.tile0, a.whole + (w - a.whole) % a.rest) : which(a.item0, w);
         const Prob p = a.p[i];
-        int tile = w - a.tile0[i], c0 = 0, n = p.kc;                    // chunks [c0, c0 + n) of the tile, n >= 1
-        if (!one) {
-            const int local = u - a.unit0[i];
-            tile = local / p.kc;
-            c0 = local - tile * p.kc;
-            n = uend - u < p.kc - c0 ? uend - u : p.kc - c0;
+        int tile = w - a.tile0[i], c0 = 0;        // chunks [c0, c0 + n) of the tile
+        if (w >= a.whole) {
+            const int local = a.equal ? w - a.whole : w - a.item0[i], tiles = a.equal ? a.rest : p.tiles, sgm = local / tiles;
+            tile = local - sgm * tiles + (a.equal ? a.whole - a.tile0[i] : 0);
+            c0 = sgm * p.seg;
         }
+        const int left = p.kc - c0, n = w < a.whole || left < p.seg ? left : p.seg;
         int m0, n0;
         tile_at(p, tile, TM, TN, m0, n0);
 
@@ -459,7 +457,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
             buf = next;
         }
         // (nobody reads the buffers any more: the last meeting was behind the last fragment reads)
-        if constexpr (KW) __syncthreads();
+        if constexpr (KW) lds_barrier();
         float* const t = reinterpret_cast<float*>(lds);
         float* const mine = KW ? t + wave * (TM * (TN + TPAD)) : t;
 #pragma unroll
@@ -469,10 +467,10 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)      // register r of lane q: row (r & 3) + 8 (r >> 2) + 4 (q >> 5), column q & 31
                     mine[(wm + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * fh) * (TN + TPAD) + wn + 32 * y + fr] = acc[x][y][r];
-        __syncthreads();
+        lds_barrier();
         if (n == p.kc) epilogue<TN, KW ? 4 : 1>(a, p, t, TM, m0, n0);
-        else {        // a range's first piece and its last one may be parts of tiles: two slots a range
-            float4* o = reinterpret_cast<float4*>(a.part + (size_t)(2 * (w - a.whole) + (piece > 0)) * (TM * TN));
+        else {
+            float4* o = reinterpret_cast<float4*>(a.part + (size_t)(w - a.whole) * (TM * TN));
 #pragma unroll 4
             for (int q = threadIdx.x; q < TM * TN / 4; q += 256) {
                 const float* tt = t + q / (TN / 4) * (TN + TPAD) + q % (TN / 4) * 4;
@@ -489,30 +487,27 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
                 o[q] = x;
             }
         }
-        u += n;
-        if (one || u >= uend) break;
-        __syncthreads();
     }
 }
 
-// Tiles that the ranges cut: the parts' accumulators added in the order of the ranges, then the same epilogue.  A workgroup takes 32 rows.
+// Tiles cut along K: the segments' accumulators added in their order, then the same epilogue.  A workgroup takes 32 rows.
 template <int TM, int TN>
-__global__ __launch_bounds__(256) void ns_join_kernel(Probs a, int tile_first)
+__global__ __launch_bounds__(256) void ns_join_kernel(Probs a)
 {
     constexpr int STRIPS = TM / 32, PER = 32 * TN / 1024;
     __shared__ __align__(16) float t[32 * (TN + TPAD)];
-    const int strip = blockIdx.x % STRIPS, tile = tile_first + blockIdx.x / STRIPS;
+    const int strip = blockIdx.x % STRIPS, tile = a.whole + blockIdx.x / STRIPS;
     const int i = which(a.tile0, tile);
     const Prob p = a.p[i];
-    const int u0 = a.unit0[i] + (tile - a.tile0[i]) * p.kc;
-    const int w0 = (u0 - a.cut0) / a.cut, w1 = (u0 + p.kc - 1 - a.cut0) / a.cut;
-    if (w0 == w1) return;           // one range had it whole
+    const int segs = (p.kc + p.seg - 1) / p.seg;
+    if (segs == 1) return;
+    const int first = a.equal ? tile - a.whole : a.item0[i] - a.whole + tile - a.tile0[i], step = a.equal ? a.rest : p.tiles;
     float4 acc[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int w = w0; w <= w1; ++w) {
-        const int slot = 2 * w + (a.cut0 + w * a.cut < u0);
-        const float4* o = reinterpret_cast<const float4*>(a.part + (size_t)slot * (TM * TN) + strip * 32 * TN) + threadIdx.x;
+#pragma unroll 2
+    for (int sgm = 0; sgm < segs; ++sgm) {
+        const float4* o = reinterpret_cast<const float4*>(a.part + ((size_t)first + (size_t)sgm * step) * (TM * TN) + strip * 32 * TN) + threadIdx.x;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const float4 v = o[k * 256];
@@ -527,7 +522,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(Probs a, int tile_first)
         const int at = (k * 256 + threadIdx.x) * 4;
         *reinterpret_cast<float4*>(t + at / TN * (TN + TPAD) + at % TN) = acc[k];
     }
-    __syncthreads();
+    lds_barrier();
     int m0, n0;
     tile_at(p, tile - a.tile0[i], TM, TN, m0, n0);
     epilogue<TN, 1>(a, p, t, 32, m0 + strip * 32, n0);
@@ -768,20 +763,20 @@ size_t layout(const Shape& s, int steps, int dtype, int planes, char* base, Buff
 
 constexpr int CUS = 256;
 
-// What a launch does: tile size, tiles taken whole (one a workgroup) and the rest cut into equal ranges of (tile, chunk) units.
-struct Plan { int shape, whole, cuts, cut; };
-// Tile shapes.  cyc: cycles of a chunk on one CU (three plane products), from the MFMA time of 256 x 128, LDS traffic of the others
-// (reads and arrivals: 256 x 128 3/4 of its MFMA time, 128 x 128 1.0, 64 x 64 1.3).
-struct TileShape { int tm, tn; double cyc; };
-constexpr TileShape SHAPES[3] = {{256, 128, 1900.0}, {128, 128, 1100.0}, {64, 64, 330.0}};
-constexpr int MAX_CUTS = CUS;
-// accumulators of the cut tiles: two slots a range
-constexpr size_t PART_BYTES = (size_t)MAX_CUTS * 2 * 256 * 128 * sizeof(float);
+// What a launch does: tile shape, leading tiles taken whole, and the length of K's segments for the others (kmax: not cut).
+struct Plan { int shape, whole, seg; };
+// Tile shapes.  cyc: cycles of a chunk on one CU (three plane products) with all CUs at work, as measured; epi: of the epilogue.
+struct TileShape { int tm, tn; double cyc, epi; };
+constexpr TileShape SHAPES[3] = {{256, 128, 1900.0, 12000.0}, {128, 128, 1150.0, 6500.0}, {64, 64, 450.0, 3500.0}};
+// accumulators of the cut tiles
+constexpr size_t PART_BYTES = (size_t)96 << 20;
+constexpr int MAX_CUT = 32;
 
-// Estimated cycles of the launch in every shape, tiles whole or cut; the cheapest is taken.
+// Estimated cycles of the launch for every shape and cut; the cheapest is taken.  A cut sends the accumulators through memory (there and back
+// at ~2000 bytes a cycle of the chip) and takes another launch (~10 000 cycles).
 Plan plan_of(const Prob* p, int count, int products)
 {
-    Plan best{0, 0, 0, 0};
+    Plan best{-1, 0, 0};
     double best_cost = 1e300;
     for (int s = 0; s < 3; ++s) {
         int64_t tiles = 0, units = 0;
@@ -793,24 +788,34 @@ Plan plan_of(const Prob* p, int count, int products)
             kmin = p[i].kc < kmin ? p[i].kc : kmin;
             kmax = p[i].kc > kmax ? p[i].kc : kmax;
         }
-        if (tiles > (1 << 28) || units > (1 << 30)) continue;
-        const double cyc = SHAPES[s].cyc * products / 3.0, epi = SHAPES[s].tm * SHAPES[s].tn / 8.0;
-        // whole tiles only: as many rounds as it takes (unequal lengths: at least the longest one)
-        const double rounds = (double)((tiles + CUS - 1) / CUS);
-        double c = kmin == kmax ? rounds * (kmax * cyc + epi) : (double)units / CUS * cyc + kmax * cyc + rounds * epi;
-        if (tiles <= CUS) c = kmax * cyc + epi;
-        if (c < best_cost) { best_cost = c; best = Plan{s, (int)tiles, 0, 0}; }
-        // full rounds whole (equal lengths), the rest cut over all CUs, at least 4 chunks a range; partial accumulators there and back
-        // at ~2000 bytes a cycle of the chip, and one more launch
-        const int64_t whole = kmin == kmax ? tiles / CUS * CUS : 0, rest = tiles - whole;
-        const int64_t ru = kmin == kmax ? rest * kmax : units;
-        if (rest > 0) {
-            int64_t cut = (ru + CUS - 1) / CUS;
-            if (cut < 4) cut = 4;
-            const int64_t cuts = (ru + cut - 1) / cut;
-            const double bytes = 2.0 * (double)(cuts + rest < 2 * cuts ? cuts + rest : 2 * cuts) * SHAPES[s].tm * SHAPES[s].tn * 4.0;
-            c = (double)whole / CUS * (kmax * cyc + epi) + cut * cyc + epi + bytes / 2000.0 + 12000.0;
-            if (c < best_cost) { best_cost = c; best = Plan{s, (int)whole, (int)cuts, (int)cut}; }
+        if (tiles > (1 << 28)) continue;
+        const double cyc = SHAPES[s].cyc * products / 3.0, epi = SHAPES[s].epi, slot = (double)SHAPES[s].tm * SHAPES[s].tn * 4.0;
+        const bool equal = kmin == kmax;
+        for (int cut = 1; cut <= MAX_CUT && (cut == 1 || kmax / cut >= 4); ++cut) {
+            const int seg = (kmax + cut - 1) / cut;
+            for (int keep = 0; keep < 2; ++keep) {       // equal lengths: whole rounds uncut, only what is left cut
+                if (keep && (!equal || cut == 1 || tiles < CUS)) continue;
+                const int64_t whole = cut == 1 ? tiles : keep ? tiles / CUS * CUS : 0, rest = tiles - whole;
+                double c;
+                int64_t items = 0;
+                if (equal) {
+                    items = rest * ((kmax + seg - 1) / seg);
+                    c = (double)((whole + CUS - 1) / CUS) * (kmax * cyc + epi) + (double)((items + CUS - 1) / CUS) * (seg * cyc + epi);
+                } else {        // rounds of mixed lengths: the mean load and a part of the longest item
+                    for (int i = 0; i < count; ++i)
+                        items += (int64_t)tiles_of(p[i].M, p[i].N, p[i].sym, SHAPES[s].tm, SHAPES[s].tn) * ((p[i].kc + seg - 1) / seg);
+                    const double mean = ((double)units * cyc + (double)items * epi) / CUS, one = seg * cyc + epi;
+                    c = items <= CUS ? one : mean + 0.6 * one;
+                }
+                if (cut > 1) {
+                    if (rest == 0 || (double)items * slot > (double)PART_BYTES) continue;
+                    c += 2.0 * (double)items * slot / 2000.0 + 10000.0;
+                }
+                if (c < best_cost) {
+                    best_cost = c;
+                    best = Plan{s, (int)whole, seg};
+                }
+            }
         }
     }
     return best;
@@ -824,11 +829,10 @@ int launch_ring(const Probs& a, const char* tag, double flops, hipStream_t strea
     constexpr size_t ring = (size_t)RINGS * NS * 64 * (TM * PL + TN * PR), tile = (size_t)RINGS * TM * (TN + TPAD) * sizeof(float);
     constexpr size_t smem = ring > tile ? ring : tile;
     if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), smem)) return MP_ELAUNCH;
-    MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), dim3((unsigned)(a.whole + a.cuts)), dim3(256), smem, stream, a);
+    MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
     MP_CHECK_LAUNCH();
-    if (a.cuts) {
-        const int first = a.whole;        // (whole > 0 only with equal lengths: tile and unit order agree)
-        MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<TM, TN>), dim3((unsigned)(a.tiles - first) * (TM / 32)), dim3(256), 0, stream, a, first);
+    if (a.whole < a.tiles) {
+        MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<TM, TN>), dim3((unsigned)(a.tiles - a.whole) * (TM / 32)), dim3(256), 0, stream, a);
         MP_CHECK_LAUNCH();
     }
     return MP_OK;
@@ -841,7 +845,7 @@ int launch_as(const Probs& a, const char* tag, double flops, hipStream_t stream)
 {
     constexpr int lds = 147456, stage = KW ? 4 * 64 * 32 * (WM * PL + WN * PR) : 64 * 64 * (WM * PL + WN * PR);
     constexpr int deep = lds / stage < 8 ? lds / stage : 8, half = KW || WM * WN >= 8 ? deep : (lds / 2 / stage < 8 ? lds / 2 / stage : 8);
-    if (a.whole + a.cuts <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW>(a, tag, flops, stream);
+    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW>(a, tag, flops, stream);
     return launch_ring<WM, WN, PL, PR, half, KW>(a, tag, flops, stream);
 }
 
@@ -852,26 +856,30 @@ int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
     const int products = left + right - 1;
     const Plan pl = plan_of(a.p, a.count, products);
     const TileShape ts = SHAPES[pl.shape];
-    if (pl.whole + pl.cuts == 0) return MP_EUNSUPPORTED;
-    int64_t tiles = 0, units = 0;
+    if (pl.shape < 0) return MP_EUNSUPPORTED;
+    int64_t tiles = 0, items = pl.whole;
     double flops = 0.0;
+    a.equal = 1;
     for (int i = 0; i < a.count; ++i) {
         Prob& p = a.p[i];
         p.tiles_n = (p.N + ts.tn - 1) / ts.tn;
+        p.tiles = tiles_of(p.M, p.N, p.sym, ts.tm, ts.tn);
+        const int segs = (p.kc + pl.seg - 1) / pl.seg;
+        p.seg = (p.kc + segs - 1) / segs;
         a.tile0[i] = (int)tiles;
-        a.unit0[i] = (int)units;
-        const int t = tiles_of(p.M, p.N, p.sym, ts.tm, ts.tn);
-        tiles += t;
-        units += (int64_t)t * p.kc;
+        a.item0[i] = (int)items;
+        tiles += p.tiles;
+        items += (int64_t)p.tiles * segs;
+        a.equal &= p.kc == a.p[0].kc;
         flops += 2.0 * products * p.M * p.N * 32.0 * p.kc * (p.sym ? 0.5 : 1.0);
     }
-    for (int i = a.count; i < MAX_PROB; ++i) a.tile0[i] = a.unit0[i] = 0x7fffffff;
+    for (int i = a.count; i < MAX_PROB; ++i) a.tile0[i] = a.item0[i] = 0x7fffffff;
     a.tiles = (int)tiles;
-    a.units = (int)units;
     a.whole = pl.whole;
-    a.cuts = pl.cuts;
-    a.cut = pl.cut;
-    a.cut0 = pl.whole == 0 ? 0 : pl.whole * a.p[0].kc;
+    a.rest = a.tiles - a.whole;
+    if (a.whole == a.tiles) items = tiles;
+    else if (a.equal) items = a.whole + (int64_t)a.rest * ((a.p[0].kc + a.p[0].seg - 1) / a.p[0].seg);
+    a.items = (int)items;
 #define NS_SHAPES(PL, PR)                                                                  \
     return pl.shape == 0   ? launch_as<4, 2, PL, PR, false>(a, tag, flops, stream)         \
            : pl.shape == 1 ? launch_as<2, 2, PL, PR, false>(a, tag, flops, stream)         \
@@ -895,14 +903,16 @@ int next_chunk(int64_t count, const int64_t* rows, const int64_t* cols, int64_t&
 
 size_t chunk_bytes(const int64_t* rows, const int64_t* cols, const int64_t* idx, int k, int steps, int dtype)
 {
-    size_t bytes = 0;
+    size_t bytes = 0, part = 0;
     for (int q = 0; q < k; ++q) {
         const Shape s = shape_of(rows[idx[q]], cols[idx[q]]);
         // (one size for both uses of 16-bit matrices: as they are, or with a momentum)
         const size_t one = layout(s, steps, dtype, 1, nullptr, nullptr), two = layout(s, steps, dtype, 2, nullptr, nullptr);
         bytes += one > two ? one : two;
+        // cut tiles of any of its products (two m x m ones may share a launch): at most MAX_CUT segments of every tile
+        part += (size_t)MAX_CUT * 2 * ((s.m + 255) / 256 * 256) * ((s.n + 255) / 256 * 256) * sizeof(float);
     }
-    return bytes + PART_BYTES;
+    return bytes + up(part < PART_BYTES ? part : PART_BYTES);
 }
 
 int check_args(int64_t count, const int64_t* rows, const int64_t* cols, int dtype, int steps)
