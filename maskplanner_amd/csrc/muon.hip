@@ -217,12 +217,6 @@ __device__ __forceinline__ void put_packed(_Float16* o, const unsigned (&w)[8])
     *reinterpret_cast<uint4v*>(o) = h;
     *reinterpret_cast<uint4v*>(o + 32) = l;
 }
-__device__ __forceinline__ void put_one(_Float16* o, unsigned w)
-{
-    reinterpret_cast<unsigned short*>(o)[0] = (unsigned short)w;
-    reinterpret_cast<unsigned short*>(o)[32] = (unsigned short)(w >> 16);
-}
-
 constexpr int TPAD = 4;      // a tile's rows in LDS are TN + 4 floats apart: 16-byte pieces, columns spread over the banks
 
 // `rows` (a multiple of 32) x TN accumulators at (r0, c0) of the product, in LDS (COPIES of them, to be added in order), to wherever the
@@ -278,15 +272,8 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
         uint4v* wt = reinterpret_cast<uint4v*>(tt);
         wt[0] = uint4v{w[0], w[1], w[2], w[3]};
         wt[1] = uint4v{w[4], w[5], w[6], w[7]};
-        // a symmetric result takes its lower half: row >= column here, mirrored below
-        if (row < p.M && col < padN && (!p.sym || row >= col)) {
-            _Float16* o = p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31);
-            if (!p.sym || row >= col + 7) put_packed(o, w);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (row >= col + e) put_one(o + e, w[e]);
-        }
+        // a symmetric result takes its lower half in pieces of 8 x 8: those below the diagonal here and, mirrored, in the second pass
+        if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) put_packed(p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31), w);
     }
     if (p.fin && !p.fin_t) return;
     lds_barrier();          // (not __syncthreads: it would wait for the stores above)
@@ -302,16 +289,16 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
             if (row < p.M) put_fin(a, p, (size_t)col * p.M + row, p.M - row, v);
             continue;
         }
-        if (row >= padM) continue;
+        if (row >= padM || (p.sym && row >> 3 < col >> 3)) continue;
         unsigned w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = reinterpret_cast<const unsigned*>(tt)[e * S];
-        _Float16* o = p.outT + ((size_t)col * p.otc + (row >> 5)) * 64 + (row & 31);
-        if (!p.sym || row > col) put_packed(o, w);
-        else
+        if (p.sym && row >> 3 == col >> 3) {        // on the diagonal: row `col` of the piece, left of the diagonal from itself
+            const unsigned* d = reinterpret_cast<const unsigned*>(t) + (col - r0) * S + (row - c0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (row + e > col) put_one(o + e, w[e]);        // (row + e == col was written above)
+            for (int e = 0; e < 8; ++e) w[e] = row + e < col ? d[e] : w[e];
+        }
+        put_packed(p.outT + ((size_t)col * p.otc + (row >> 5)) * 64 + (row & 31), w);
     }
 }
 
