@@ -9,7 +9,7 @@
 // columns of every row its workgroup walks, its sums stay in registers, and one row of partial sums per workgroup goes through memory to
 // a second small kernel that adds them in a fixed order (no atomics: two calls give the same bits).  All sums in fp32 (partial rows: fp64).
 //
-// Rows wider than the register form (NV = 8) loop over the row in memory: the second and third reading come from the caches, and dw / db
+// Rows wider than the register form (2048 vectors) loop over the row in memory: the second and third reading come from the caches, and dw / db
 // take a kernel of their own over column strips.
 #include "common.h"
 
@@ -20,19 +20,18 @@ template <typename T> struct LnVec {     // 16 bytes that may lie at any element
     T v[N];
 };
 
+// `left` > 0 elements from p on (16 bytes where that many are left), zeros behind
 template <typename T>
-__device__ __forceinline__ void ln_load(const T* __restrict__ p, int left, float (&out)[LnVec<T>::N])
+__device__ __forceinline__ LnVec<T> ln_raw(const T* __restrict__ p, int left)
 {
     constexpr int V = LnVec<T>::N;
-    if (left >= V) {
-        LnVec<T> t;
-        __builtin_memcpy(&t, p, 16);
+    LnVec<T> t;
+    if (left >= V) __builtin_memcpy(&t, p, 16);
+    else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = (float)t.v[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = e < left ? (float)p[e] : 0.0f;
+        for (int e = 0; e < V; ++e) t.v[e] = e < left ? p[e] : (T)0.0f;
     }
+    return t;
 }
 
 template <typename T>
@@ -51,34 +50,42 @@ __device__ __forceinline__ void ln_store(T* __restrict__ p, int left, const floa
     }
 }
 
-// V parameters of columns c .. c + V - 1 (W may be wider than T: then two 16-byte loads)
+// V parameters (16 or, fp32 parameters of 16-bit rows, 32 bytes), kept as they are for all rows of a workgroup
+template <typename W, int V> struct LnParam { W v[V]; };
 template <typename W, int V>
-__device__ __forceinline__ void ln_param(const W* __restrict__ p, int c, int D, float def, float (&out)[V])
+__device__ __forceinline__ LnParam<W, V> ln_param(const W* __restrict__ p, int c, int D, float def)
 {
-    if (!p) {
+    LnParam<W, V> t;
+    if (p && c + V <= D) __builtin_memcpy(&t, p + c, sizeof(t));
+    else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = def;
-    } else if (c + V <= D) {
-        W t[V];
-        __builtin_memcpy(t, p + c, sizeof(t));
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = (float)t[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = c + e < D ? (float)p[c + e] : 0.0f;
+        for (int e = 0; e < V; ++e) t.v[e] = p && c + e < D ? p[c + e] : (W)def;
     }
+    return t;
 }
 
-// Sums of A values over the TPR threads of a row, left in all of them.  TPR <= 64: lanes of one wave (xor butterfly, the same order in
-// every lane); TPR = 256: four waves through LDS (buf: 4 x A floats; the two barriers make it reusable).
+// Sums of A values over the TPR threads of a row, left in all of them.  TPR <= 64: lanes of one wave, in registers (DPP inside rows of 16
+// lanes, row and half swaps above), every lane adding the same pairs; wider: the waves' sums through LDS (buf: TPR / 64 x A floats that the
+// previous call did not use: one barrier).
+template <int CTRL> __device__ __forceinline__ float dpp_f32(float v) { return __uint_as_float(mp::dpp_u32<CTRL>(__float_as_uint(v))); }
 template <int TPR, int A>
 __device__ __forceinline__ void row_sum(float (&v)[A], float* buf)
 {
-    constexpr int L = TPR < 64 ? TPR : 64;
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int a = 0; a < A; ++a) v[a] += __shfl_xor(v[a], o, 64);
+    for (int a = 0; a < A; ++a) {
+        v[a] += dpp_f32<mp::DPP_QUAD_XOR1>(v[a]);
+        v[a] += dpp_f32<mp::DPP_QUAD_XOR2>(v[a]);
+        v[a] += dpp_f32<mp::DPP_ROW_HALF_MIRROR>(v[a]);
+        if constexpr (TPR >= 16) v[a] += dpp_f32<mp::DPP_ROW_MIRROR>(v[a]);
+        if constexpr (TPR >= 32) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[a]), __float_as_uint(v[a]), false, false);
+            v[a] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+        if constexpr (TPR >= 64) {
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[a]), __float_as_uint(v[a]), false, false);
+            v[a] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+    }
     if constexpr (TPR > 64) {
         const int w = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0)
@@ -86,111 +93,156 @@ __device__ __forceinline__ void row_sum(float (&v)[A], float* buf)
             for (int a = 0; a < A; ++a) buf[w * A + a] = v[a];
         __syncthreads();
 #pragma unroll
-        for (int a = 0; a < A; ++a) v[a] = (buf[a] + buf[A + a]) + (buf[2 * A + a] + buf[3 * A + a]);
-        __syncthreads();
+        for (int a = 0; a < A; ++a) {
+            float p[TPR / 64];
+#pragma unroll
+            for (int k = 0; k < TPR / 64; ++k) p[k] = buf[k * A + a];
+#pragma unroll
+            for (int o = TPR / 128; o > 0; o >>= 1)
+#pragma unroll
+                for (int k = 0; k < o; ++k) p[k] += p[k + o];
+            v[a] = p[0];
+        }
     }
 }
 
+// A workgroup walks rows gridDim.x apart; the next row's values are on their way while one is reduced.
+constexpr int ln_block(int tpr) { return tpr > 256 ? tpr : 256; }
+
 template <typename T, typename W, int TPR, int NV>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, int64_t rows, int D, int64_t xs, const W* __restrict__ w,
+__global__ __launch_bounds__(ln_block(TPR)) void ln_fwd_kernel(const T* __restrict__ x, int64_t rows, int D, int64_t xs, const W* __restrict__ w,
                                                      const W* __restrict__ b, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                                                      float* __restrict__ rstd_out)
 {
-    constexpr int V = LnVec<T>::N;
-    __shared__ float buf[4];
-    const int t = threadIdx.x % TPR;
-    const int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-    const bool live = r < rows;
-    const T* xr = x + (live ? r : 0) * xs;
-    float v[NV][V];
-    float s[1] = {0.0f};
+    constexpr int V = LnVec<T>::N, RPB = ln_block(TPR) / TPR;
+    __shared__ float buf[2][16];
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const int64_t stride = (int64_t)gridDim.x * RPB;
+    LnParam<W, V> ww[NV], bb[NV];
+    LnVec<T> next[NV];
+    auto fetch = [&](int64_t r) {
+        const T* xr = x + (r < rows ? r : 0) * xs;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + t) * V;
-        ln_load(xr + c, D - c, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[0] += v[i][e];
-    row_sum<TPR>(s, buf);
-    const float mean = s[0] / (float)D;
-    s[0] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float d = v[i][e] - mean;
-            s[0] += (i * TPR + t) * V + e < D ? d * d : 0.0f;
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * V;
+            next[i] = c < D ? ln_raw(xr + c, D - c) : LnVec<T>{};
         }
-    row_sum<TPR>(s, buf);
-    const float rstd = 1.0f / sqrtf(s[0] / (float)D + eps);
-    if (!live) return;
-    if (t == 0 && mean_out) {
-        mean_out[r] = mean;
-        rstd_out[r] = rstd;
-    }
-    T* yr = y + r * D;
+    };
+    const bool full = D == NV * TPR * V;        // no columns behind D in any thread
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    fetch(r0 + slot);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + t) * V;
-        if (c < D) {
-            float ww[V], bb[V];
-            ln_param<W, V>(w, c, D, 1.0f, ww);
-            ln_param<W, V>(b, c, D, 0.0f, bb);
+        ww[i] = ln_param<W, V>(w, (i * TPR + t) * V, D, 1.0f);
+        bb[i] = ln_param<W, V>(b, (i * TPR + t) * V, D, 0.0f);
+    }
+    for (; r0 < rows; r0 += stride) {       // (uniform: row_sum has barriers)
+        const int64_t r = r0 + slot;
+        float v[NV][V];
+        float s[1] = {0.0f};
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[i][e] = fmaf((v[i][e] - mean) * rstd, ww[e], bb[e]);
-            ln_store(yr + c, D - c, v[i]);
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[i][e] = (float)next[i].v[e];       // (0 behind D)
+                s[0] += v[i][e];
+            }
+        if (r0 + stride < rows) fetch(r + stride);
+        row_sum<TPR>(s, buf[0]);
+        const float mean = s[0] / (float)D;
+        s[0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[i][e] -= mean;
+                s[0] += full || (i * TPR + t) * V + e < D ? v[i][e] * v[i][e] : 0.0f;
+            }
+        row_sum<TPR>(s, buf[1]);
+        const float rstd = 1.0f / sqrtf(s[0] / (float)D + eps);
+        if (r < rows) {
+            if (t == 0 && mean_out) {
+                mean_out[r] = mean;
+                rstd_out[r] = rstd;
+            }
+            T* yr = y + r * D;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * TPR + t) * V;
+                if (c < D) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, (float)ww[i].v[e], (float)bb[i].v[e]);
+                    ln_store(yr + c, D - c, v[i]);
+                }
+            }
         }
     }
 }
 
 // part: [gridDim.x][2][D] fp32 (dw row, db row), or NULL when neither is wanted
 template <typename T, typename W, int TPR, int NV>
-__global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs, int64_t rows,
+__global__ __launch_bounds__(ln_block(TPR)) void ln_bwd_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs, int64_t rows,
                                                      int D, const W* __restrict__ w, const float* __restrict__ mean_in,
                                                      const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part)
 {
-    constexpr int V = LnVec<T>::N, RPB = 256 / TPR;
-    __shared__ float buf[8];
+    constexpr int V = LnVec<T>::N, RPB = ln_block(TPR) / TPR;
+    __shared__ float buf[2][32];
     __shared__ float fold[TPR < 256 ? 256 * V : 1];
     const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-    float ww[NV][V], aw[NV][V], ab[NV][V];
+    const int64_t stride = (int64_t)gridDim.x * RPB;
+    LnParam<W, V> ww[NV];
+    float aw[NV][V], ab[NV][V];
+    LnVec<T> nx[NV], ng[NV];
+    float nmean = 0.0f, nrstd = 0.0f;
+    auto fetch = [&](int64_t r) {
+        // zeros behind D and behind the last row (mean and rstd too): they add exact zeros to every sum
+        const T* xr = x + r * xs;
+        const T* gr = dy + r * dys;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * V;
+            nx[i] = ng[i] = LnVec<T>{};
+            if (c < D && r < rows) {
+                nx[i] = ln_raw(xr + c, D - c);
+                ng[i] = ln_raw(gr + c, D - c);
+            }
+        }
+        nmean = r < rows ? mean_in[r] : 0.0f;
+        nrstd = r < rows ? rstd_in[r] : 0.0f;
+    };
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    fetch(r0 + slot);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        ln_param<W, V>(w, (i * TPR + t) * V, D, 1.0f, ww[i]);
+        ww[i] = ln_param<W, V>(w, (i * TPR + t) * V, D, 1.0f);
 #pragma unroll
         for (int e = 0; e < V; ++e) aw[i][e] = ab[i][e] = 0.0f;
     }
     const float inv = 1.0f / (float)D;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {     // (uniform: row_sum has barriers)
+    int flip = 0;
+    for (; r0 < rows; r0 += stride) {     // (uniform: row_sum has barriers)
         const int64_t r = r0 + slot;
         const bool live = r < rows;
-        const int64_t rr = live ? r : 0;
+        const float mean = nmean, rstd = nrstd;
         float z[NV][V], g[NV][V];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + t) * V;
-            ln_load(x + rr * xs + c, D - c, z[i]);
-            ln_load(dy + rr * dys + c, live ? D - c : 0, g[i]);
-        }
-        const float mean = mean_in[rr], rstd = rstd_in[rr];
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                // columns behind D and rows behind the last stay out of the sums by selection: 0 * inf would not
-                const bool in = live && (i * TPR + t) * V + e < D;
-                z[i][e] = in ? (z[i][e] - mean) * rstd : 0.0f;
+                z[i][e] = ((float)nx[i].v[e] - mean) * rstd;
+                g[i][e] = (float)ng[i].v[e];
                 aw[i][e] += g[i][e] * z[i][e];
                 ab[i][e] += g[i][e];
-                g[i][e] *= ww[i][e];
+                g[i][e] *= (float)ww[i].v[e];
                 s[0] += g[i][e];
                 s[1] += g[i][e] * z[i][e];
             }
-        row_sum<TPR>(s, buf);
-        if (live && dx) {
+        if (r0 + stride < rows) fetch(r + stride);
+        if (!dx) continue;
+        row_sum<TPR>(s, buf[flip]);
+        flip ^= 1;
+        if (live) {
             const float c1 = s[0] * inv, c2 = s[1] * inv;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -205,18 +257,16 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ dy, i
     }
     if (!part) return;
     float* pw = part + (size_t)blockIdx.x * 2 * D;
-    if constexpr (TPR == 256) {
+    if constexpr (TPR >= 256) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * TPR + t) * V;
-            if (c < D) {
-                ln_store(pw + c, D - c, *reinterpret_cast<float(*)[4]>(&aw[i][0]));
-                ln_store(pw + D + c, D - c, *reinterpret_cast<float(*)[4]>(&ab[i][0]));
-                if constexpr (V == 8) {
-                    ln_store(pw + c + 4, D - c - 4, *reinterpret_cast<float(*)[4]>(&aw[i][4]));
-                    ln_store(pw + D + c + 4, D - c - 4, *reinterpret_cast<float(*)[4]>(&ab[i][4]));
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (c + e < D) {
+                    pw[c + e] = aw[i][e];
+                    pw[D + c + e] = ab[i][e];
                 }
-            }
         }
     } else {      // the RPB row slots of the workgroup meet in LDS, one vector of columns at a time, in the order of the slots
 #pragma unroll
@@ -227,8 +277,8 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ dy, i
 #pragma unroll
                 for (int e = 0; e < V; ++e) fold[e * 256 + threadIdx.x] = k ? ab[i][e] : aw[i][e];
                 __syncthreads();
-                for (int q = threadIdx.x; q < TPR * V; q += 256) {     // q = e * TPR + thread of the row
-                    const int e = q / TPR, tt = q % TPR, c = (i * TPR + tt) * V + e;
+                for (int q = threadIdx.x; q < TPR * V; q += 256) {     // q = thread of the row * V + e
+                    const int e = q % V, tt = q / V, c = (i * TPR + tt) * V + e;
                     float sum = 0.0f;
 #pragma unroll
                     for (int sl = 0; sl < RPB; ++sl) sum += fold[e * 256 + sl * TPR + tt];
@@ -238,13 +288,73 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ dy, i
     }
 }
 
+// Few rows (a head's batch): one launch and no workspace.  Workgroups 0 .. rows - 1 take dx of a row, the others 256 columns of dw / db each
+// over all rows, in their order.
+template <typename T, typename W, int NV>
+__global__ __launch_bounds__(256) void ln_bwd_few_kernel(const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs, int rows, int D,
+                                                         const W* __restrict__ w, const float* __restrict__ mean_in,
+                                                         const float* __restrict__ rstd_in, T* __restrict__ dx, W* __restrict__ dw, W* __restrict__ db)
+{
+    constexpr int V = LnVec<T>::N;
+    __shared__ float buf[8];
+    const int r = blockIdx.x;
+    if (r >= rows) {
+        const int c = (r - rows) * 256 + threadIdx.x;
+        if (c >= D) return;
+        float aw = 0.0f, ab = 0.0f;
+#pragma unroll 8
+        for (int k = 0; k < rows; ++k) {
+            const float g = (float)dy[k * dys + c];
+            aw += g * (((float)x[k * xs + c] - mean_in[k]) * rstd_in[k]);
+            ab += g;
+        }
+        if (dw) dw[c] = (W)aw;
+        if (db) db[c] = (W)ab;
+        return;
+    }
+    if (!dx) return;
+    const float mean = mean_in[r], rstd = rstd_in[r], inv = 1.0f / (float)D;
+    float z[NV][V], g[NV][V];
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 256 + (int)threadIdx.x) * V;
+        if (c >= D) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[i][e] = g[i][e] = 0.0f;
+            continue;
+        }
+        const LnVec<T> nx = ln_raw(x + r * xs + c, D - c), ng = ln_raw(dy + r * dys + c, D - c);
+        const LnParam<W, V> ww = ln_param<W, V>(w, c, D, 1.0f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const bool in = c + e < D;
+            z[i][e] = in ? ((float)nx.v[e] - mean) * rstd : 0.0f;
+            g[i][e] = in ? (float)ng.v[e] * (float)ww.v[e] : 0.0f;
+            s[0] += g[i][e];
+            s[1] += g[i][e] * z[i][e];
+        }
+    }
+    row_sum<256>(s, buf);
+    const float c1 = s[0] * inv, c2 = s[1] * inv;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 256 + (int)threadIdx.x) * V;
+        if (c < D) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[i][e] = rstd * (g[i][e] - c1 - z[i][e] * c2);
+            ln_store(dx + (int64_t)r * D + c, D - c, g[i]);
+        }
+    }
+}
+
 // ---- rows wider than the register form: one workgroup walks a row three times (twice from the caches) -------------------------------
 template <typename T, typename W>
 __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(const T* __restrict__ x, int64_t rows, int64_t D, int64_t xs, const W* __restrict__ w,
                                                           const W* __restrict__ b, float eps, T* __restrict__ y,
                                                           float* __restrict__ mean_out, float* __restrict__ rstd_out)
 {
-    __shared__ float buf[4];
+    __shared__ float buf[8];
     const int64_t r = blockIdx.x;
     const T* xr = x + r * xs;
     float s[1] = {0.0f};
@@ -256,7 +366,7 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(const T* __restrict__ 
         const float d = (float)xr[c] - mean;
         s[0] += d * d;
     }
-    row_sum<256>(s, buf);
+    row_sum<256>(s, buf + 4);
     const float rstd = 1.0f / sqrtf(s[0] / (float)D + eps);
     if (threadIdx.x == 0 && mean_out) {
         mean_out[r] = mean;
@@ -309,11 +419,11 @@ __global__ __launch_bounds__(256) void ln_param_grad_wide_kernel(const T* __rest
     part[(size_t)blockIdx.y * 2 * D + D + c] = ab;
 }
 
-// dw, db = sums of the n partial rows, fp64, in a fixed order: 16 columns x 16 row groups a workgroup, y: dw or db
+// dw, db = sums of the n partial rows, fp64, in a fixed order: 16 columns x 64 row groups a workgroup, y: dw or db
 template <typename W>
-__global__ __launch_bounds__(256) void ln_param_reduce_kernel(const float* __restrict__ part, int n, int64_t D, W* __restrict__ dw, W* __restrict__ db)
+__global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* __restrict__ part, int n, int64_t D, W* __restrict__ dw, W* __restrict__ db)
 {
-    __shared__ double acc[16][17];
+    __shared__ double acc[64][17];
     const int cl = threadIdx.x & 15, rg = threadIdx.x >> 4;
     const int64_t c = (int64_t)blockIdx.x * 16 + cl;
     W* out = blockIdx.y ? db : dw;
@@ -321,28 +431,30 @@ __global__ __launch_bounds__(256) void ln_param_reduce_kernel(const float* __res
     if (c < D && out) {
         const float* p = part + blockIdx.y * D + c;
 #pragma unroll 8
-        for (int k = rg; k < n; k += 16) s += (double)p[(size_t)k * 2 * D];
+        for (int k = rg; k < n; k += 64) s += (double)p[(size_t)k * 2 * D];
     }
     acc[rg][cl] = s;
     __syncthreads();
-    if (rg == 0 && c < D && out) {
-        double v = 0.0;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v += acc[k][cl];
-        out[c] = (W)(float)v;
+    for (int o = 32; o > 0; o >>= 1) {
+        if (rg < o) acc[rg][cl] += acc[rg + o][cl];
+        __syncthreads();
     }
+    if (rg == 0 && c < D && out) out[c] = (W)(float)acc[0][cl];
 }
 
-constexpr int LN_MAX_PARTS = 1024;       // partial rows of dw / db (4 workgroups a CU)
+constexpr int LN_FWD_BLOCKS = 2048;      // workgroups of the forward kernel (8 a CU)
+constexpr int LN_MAX_PARTS = 1280;       // partial rows of dw / db, workgroups of the backward kernel (5 a CU)
 constexpr int LN_WIDE_PARTS = 64;
+// up to here dw / db are summed row by row by one thread a column: no partial sums, no second launch (32 x 1024 fp32: 4 us against 4 + 3)
+constexpr int LN_FEW_ROWS = 64;
 
 int esize(int dtype) { return dtype == MP_DTYPE_F32 ? 4 : 2; }
 int64_t reg_limit(int dtype) { return 256 * 8 * (16 / esize(dtype)); }
 
-// Threads a row: the smallest power of two (from 8) whose one vector each covers it, 64 with up to four; from there on, and for calls of
-// few rows (latency: more waves share a row), 256.  [TPR, NV]
+// Threads a row: the smallest power of two (from 8) whose one vector each covers it, 64 with up to four; calls of few rows (latency: more
+// waves share a row) 256; wider rows 256 to 1024 with two, so that the registers leave room for several rows a CU.  [TPR, NV]
 struct LnShape { int tpr, nv; };
-LnShape ln_shape(int64_t rows, int64_t D, int V)
+LnShape ln_shape(int64_t rows, int64_t D, int V, bool backward)
 {
     const int64_t vecs = (D + V - 1) / V;
     if (vecs <= 8) return {8, 1};
@@ -354,15 +466,17 @@ LnShape ln_shape(int64_t rows, int64_t D, int V)
     if (!few && vecs <= 256) return {64, 4};
     if (vecs <= 256) return {256, 1};
     if (vecs <= 512) return {256, 2};
-    if (vecs <= 1024) return {256, 4};
-    return {256, 8};
+    if (vecs <= 1024) return {512, 2};
+    if (backward) return {512, 4};       // (1024 threads leave 128 registers each: too few for the sums)
+    return {1024, 2};
 }
 
 int ln_parts(int64_t rows, int64_t D, int dtype)
 {
     if (D > reg_limit(dtype)) return (int)(rows < LN_WIDE_PARTS ? rows : LN_WIDE_PARTS);
-    const LnShape s = ln_shape(rows, D, 16 / esize(dtype));
-    const int64_t blocks = (rows + 256 / s.tpr - 1) / (256 / s.tpr);
+    if (rows <= LN_FEW_ROWS) return 0;
+    const LnShape s = ln_shape(rows, D, 16 / esize(dtype), true);
+    const int64_t blocks = (rows + ln_block(s.tpr) / s.tpr - 1) / (ln_block(s.tpr) / s.tpr);
     return (int)(blocks < LN_MAX_PARTS ? blocks : LN_MAX_PARTS);
 }
 
@@ -373,10 +487,10 @@ int ln_parts(int64_t rows, int64_t D, int dtype)
     else if (s.tpr == 64 && s.nv == 1) { GO(64, 1); }                              \
     else if (s.tpr == 64 && s.nv == 2) { GO(64, 2); }                              \
     else if (s.tpr == 64) { GO(64, 4); }                                           \
-    else if (s.nv == 1) { GO(256, 1); }                                            \
-    else if (s.nv == 2) { GO(256, 2); }                                            \
-    else if (s.nv == 4) { GO(256, 4); }                                            \
-    else { GO(256, 8); }
+    else if (s.tpr == 256 && s.nv == 1) { GO(256, 1); }                            \
+    else if (s.tpr == 256) { GO(256, 2); }                                         \
+    else if (s.tpr == 512 && s.nv == 2) { GO(512, 2); }                            \
+    else { GO_LAST; }
 
 template <typename T, typename W>
 int ln_fwd(const void* x, int dtype, int64_t rows, int64_t D, int64_t xs, const void* w, const void* b, double eps, void* y, float* mean, float* rstd,
@@ -387,12 +501,15 @@ int ln_fwd(const void* x, int dtype, int64_t rows, int64_t D, int64_t xs, const 
         MP_LAUNCH("ln_fwd_wide_kernel", 8.0 * n, bytes, (ln_fwd_wide_kernel<T, W>), dim3((unsigned)rows), dim3(256), 0, stream, (const T*)x, rows, D,
                   xs, (const W*)w, (const W*)b, (float)eps, (T*)y, mean, rstd);
     } else {
-        const LnShape s = ln_shape(rows, D, LnVec<T>::N);
-        const unsigned grid = (unsigned)((rows + 256 / s.tpr - 1) / (256 / s.tpr));
+        const LnShape s = ln_shape(rows, D, LnVec<T>::N, false);
+        const int64_t blocks = (rows + ln_block(s.tpr) / s.tpr - 1) / (ln_block(s.tpr) / s.tpr);
+        const unsigned grid = (unsigned)(blocks < LN_FWD_BLOCKS ? blocks : LN_FWD_BLOCKS);
 #define LN_GO(TPR, NV)                                                                                                                   \
-    MP_LAUNCH("ln_fwd_kernel", 8.0 * n, bytes, (ln_fwd_kernel<T, W, TPR, NV>), dim3(grid), dim3(256), 0, stream, (const T*)x, rows, (int)D, \
+    MP_LAUNCH("ln_fwd_kernel", 8.0 * n, bytes, (ln_fwd_kernel<T, W, TPR, NV>), dim3(grid), dim3(ln_block(TPR)), 0, stream, (const T*)x, rows, (int)D, \
               xs, (const W*)w, (const W*)b, (float)eps, (T*)y, mean, rstd)
+#define GO_LAST LN_GO(1024, 2)
         LN_EACH_SHAPE(LN_GO)
+#undef GO_LAST
 #undef LN_GO
     }
     MP_CHECK_LAUNCH();
@@ -414,17 +531,31 @@ int ln_bwd(const void* dy, int64_t dys, const void* x, int64_t xs, int dtype, in
             MP_LAUNCH("ln_param_grad_wide_kernel", 4.0 * n, 2.0 * n * sizeof(T), (ln_param_grad_wide_kernel<T>),
                       dim3((unsigned)((D + 255) / 256), (unsigned)parts), dim3(256), 0, stream, (const T*)dy, dys, (const T*)x, xs, rows, D, mean, rstd, part);
         MP_CHECK_LAUNCH();
+    } else if (rows > 0 && rows <= LN_FEW_ROWS) {
+        const unsigned grid = (unsigned)(rows + (pg ? (D + 255) / 256 : 0));
+#define LN_GO(NV)                                                                                                                            \
+    MP_LAUNCH("ln_bwd_few_kernel", 16.0 * n, bytes, (ln_bwd_few_kernel<T, W, NV>), dim3(grid), dim3(256), 0, stream, (const T*)dy, dys, (const T*)x, \
+              xs, (int)rows, (int)D, (const W*)w, mean, rstd, (T*)dx, (W*)dw, (W*)db)
+        const int64_t vecs = (D + LnVec<T>::N - 1) / LnVec<T>::N;
+        if (vecs <= 256) LN_GO(1);
+        else if (vecs <= 1024) LN_GO(4);
+        else LN_GO(8);
+#undef LN_GO
+        MP_CHECK_LAUNCH();
+        return MP_OK;
     } else if (rows > 0) {
-        const LnShape s = ln_shape(rows, D, LnVec<T>::N);
+        const LnShape s = ln_shape(rows, D, LnVec<T>::N, true);
 #define LN_GO(TPR, NV)                                                                                                                     \
-    MP_LAUNCH("ln_bwd_kernel", 16.0 * n, bytes, (ln_bwd_kernel<T, W, TPR, NV>), dim3((unsigned)parts), dim3(256), 0, stream, (const T*)dy, dys, \
+    MP_LAUNCH("ln_bwd_kernel", 16.0 * n, bytes, (ln_bwd_kernel<T, W, TPR, NV>), dim3((unsigned)parts), dim3(ln_block(TPR)), 0, stream, (const T*)dy, dys, \
               (const T*)x, xs, rows, (int)D, (const W*)w, mean, rstd, (T*)dx, pg ? part : nullptr)
+#define GO_LAST LN_GO(512, 4)
         LN_EACH_SHAPE(LN_GO)
+#undef GO_LAST
 #undef LN_GO
         MP_CHECK_LAUNCH();
     }
     if (pg) {      // (no rows: the sums are zero)
-        hipLaunchKernelGGL((ln_param_reduce_kernel<W>), dim3((unsigned)((D + 15) / 16), 2), dim3(256), 0, stream, part, parts, D, (W*)dw, (W*)db);
+        hipLaunchKernelGGL((ln_param_reduce_kernel<W>), dim3((unsigned)((D + 15) / 16), 2), dim3(1024), 0, stream, part, parts, D, (W*)dw, (W*)db);
         MP_CHECK_LAUNCH();
     }
     return MP_OK;
@@ -472,7 +603,8 @@ extern "C" int mp_layer_norm_bwd(const void* dy, int64_t dy_row_stride, const vo
     if (!dx && !dweight && !dbias) return MP_OK;
     if (rows > 0 && (!dy || !x || !mean || !rstd || dy_row_stride < 0 || x_row_stride < 0)) return MP_EINVAL;
     if ((dweight || dbias) && rows > 0) {
-        if (!workspace || workspace_bytes < mp_layer_norm_bwd_workspace_bytes(rows, cols, dtype)) return MP_EWORKSPACE;
+        const size_t need = mp_layer_norm_bwd_workspace_bytes(rows, cols, dtype);
+        if (need && (!workspace || workspace_bytes < need)) return MP_EWORKSPACE;
         if (reinterpret_cast<uintptr_t>(workspace) & 3) return MP_EINVAL;
     }
     hipStream_t s = mp_stream(stream_);

@@ -966,6 +966,8 @@ _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # include/
 def _rows_of(x):
     """x [..., D] as rows of contiguous elements at one stride: (tensor, row stride).  A view where the layout allows it, else a copy."""
     D = x.shape[-1]
+    if x.is_contiguous():
+        return x, D
     if x.ndim != 2:
         x = x.reshape(-1, D)
     if D > 1 and x.stride(1) != 1:
@@ -978,18 +980,18 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         D = x.shape[-1]
         x2, xs = _rows_of(x)
-        rows = x2.shape[0]
+        rows = x.numel() // D
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        wanted = any(ctx.needs_input_grad)
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if wanted else None
         like = weight if weight is not None else bias
         wt = _DTYPE[like.dtype if like is not None else x.dtype]
-        mean = stats.data_ptr() if wanted and rows else None
+        mean = None
+        if True in ctx.needs_input_grad:
+            stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+            mean = stats.data_ptr() if rows else None
+            ctx.save_for_backward(x, weight, stats)
+            ctx.args = rows, D, wt, None if like is None else like.dtype
         _run("layer_norm", x, _lib.load().mp_layer_norm_fwd, x2.data_ptr(), _DTYPE[x.dtype], rows, D, xs, _p(weight), _p(bias), wt, eps,
              y.data_ptr(), mean, mean + 4 * rows if mean else None)
-        if wanted:
-            ctx.save_for_backward(x, weight, stats)
-            ctx.wt = wt
         return y
 
     @staticmethod
@@ -1000,21 +1002,20 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def _backward(ctx, grad_y):
         x, weight, stats = ctx.saved_tensors
-        D = x.shape[-1]
-        x2, xs = _rows_of(x)
-        dy, dys = _rows_of(grad_y if grad_y.dtype == x.dtype else grad_y.to(x.dtype))
-        rows = x2.shape[0]
+        rows, D, wt, wdtype = ctx.args
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        wdtype = (torch.float32, torch.float16, torch.bfloat16)[ctx.wt]
-        gw = torch.empty((D,), dtype=wdtype, device=x.device) if need_w else None
-        gb = torch.empty((D,), dtype=wdtype, device=x.device) if need_b else None
-        lib, dt = _lib.load(), _DTYPE[x.dtype]
+        dtype, device = x.dtype, x.device
+        x2, xs = _rows_of(x)
+        dy, dys = _rows_of(grad_y if grad_y.dtype == dtype else grad_y.to(dtype))
+        gx = torch.empty(x.shape, dtype=dtype, device=device) if need_x else None
+        gw = torch.empty((D,), dtype=wdtype, device=device) if need_w else None
+        gb = torch.empty((D,), dtype=wdtype, device=device) if need_b else None
+        lib, dt = _lib.load(), _DTYPE[dtype]
         nbytes = lib.mp_layer_norm_bwd_workspace_bytes(rows, D, dt) if (need_w or need_b) else 0
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device) if nbytes else None
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
         mean = stats.data_ptr()
-        _run("layer_norm_bwd", x, lib.mp_layer_norm_bwd, dy.data_ptr(), dys, x2.data_ptr(), xs, dt, rows, D, _p(weight), ctx.wt, mean,
-             mean + 4 * rows, _p(gx), _p(gw), _p(gb), _p(ws), nbytes)
+        _run("layer_norm_bwd", x, lib.mp_layer_norm_bwd, dy.data_ptr(), dys, x2.data_ptr(), xs, dt, rows, D, _p(weight), wt, mean, mean + 4 * rows,
+             _p(gx), _p(gw), _p(gb), _p(ws), nbytes)
         return gx, gw, gb, None
 
     _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
