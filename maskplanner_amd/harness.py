@@ -71,7 +71,10 @@ def _even(n):
 class TrainStep:
     def __init__(self, category="cuboids", B=32, N=5120, device="cuda", seed=1235, hidden_size=(1024, 1024), lr=1e-3,
                  dist_points="cuboid", rank=0, loss_overrides=None, prefetch_sampling=False, factor_heads=True, graph=None,
-                 overlap_sampling=None, encoder="ssg", mlp_dtype="f32", sync_bn=False, stream_batches=0):
+                 overlap_sampling=None, encoder="ssg", mlp_dtype="f32", sync_bn=False, stream_batches=0, optimizer="adam", muon=None):
+        """optimizer "muon": the set-abstraction weight matrices by Muon (`muon`: its arguments, muon.MuonAdam), everything else by Adam as before."""
+        if optimizer not in ("adam", "muon"):
+            raise ValueError(f"TrainStep: optimizer is 'adam' or 'muon', not {optimizer!r}")
         self.cat = synthetic.CATEGORIES[category] if isinstance(category, str) else category
         self.device = torch.device(device)
         torch.manual_seed(seed)  # identical initial weights on every rank
@@ -158,7 +161,15 @@ class TrainStep:
         self._dp_recorded = False      # the data-parallel exchange is part of the recorded graphs (_record_split)
         # train_maskplanner.py:159.  On the GPU the dense parameters go through csrc/adam_multi.hip (same update, ~150 tensors in four
         # launches).
-        if fused:
+        if optimizer == "muon":
+            if not fused:
+                raise RuntimeError("TrainStep(optimizer='muon') runs on the MI355X only")
+            from .muon import MuonAdam
+            names = {p: n for n, p in self.model.named_parameters()}
+            mats = [p for p in dense if p.ndim >= 2 and names[p].startswith("sa")]
+            ids = {id(p) for p in mats}
+            self.opt = MuonAdam(mats, [p for p in dense if id(p) not in ids], lr=lr, capturable=self.use_graph, **(muon or {}))
+        elif fused:
             self.opt = DenseAdam(dense, lr=lr, capturable=self.use_graph)
         else:
             self.opt = torch.optim.Adam(dense, lr=lr, fused=fused, capturable=self.use_graph)
@@ -243,7 +254,7 @@ class TrainStep:
             sa_mlp.flush_ticks()
 
     def _opt_step(self):
-        if isinstance(self.opt, DenseAdam):
+        if hasattr(self.opt, "step_dev"):       # DenseAdam, MuonAdam
             self.opt.step(ticked=self._dense_ticked)
         else:
             self.opt.step()

@@ -14,6 +14,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .layer_norm import LayerNorm
 from .pointnet2_utils import PointNetSetAbstraction
 
 
@@ -24,7 +25,12 @@ class _SegBase(nn.Module):
         from . import graphed
         graphed.fast_zero_grad(self, set_to_none)
 
-    def _build(self, in_channel):
+    def _build(self, in_channel, point_norm="batch"):
+        """point_norm: what follows conv1..conv3.  "batch" (the reference's BatchNorm1d) or "layer": a layer norm over each point's features
+        (bn1..bn3 are layer_norm.LayerNorm): the same result for a cloud whatever else is in the batch, in training as in evaluation."""
+        if point_norm not in ("batch", "layer"):
+            raise ValueError(f"point_norm is 'batch' or 'layer', not {point_norm!r}")
+        self.point_norm = point_norm
         self.sa1 = PointNetSetAbstraction(npoint=512, radius=0.2, nsample=32, in_channel=in_channel, mlp=[64, 64, 128],
                                           group_all=False)
         self.sa2 = PointNetSetAbstraction(npoint=128, radius=0.4, nsample=64, in_channel=128 + 3, mlp=[128, 128, 256],
@@ -34,6 +40,10 @@ class _SegBase(nn.Module):
         self.conv1 = nn.Conv1d(1024 + in_channel, 512, 1)
         self.conv2 = nn.Conv1d(512, 256, 1)
         self.conv3 = nn.Conv1d(256, 128, 1)
+
+    def _build_norms(self):
+        norm = LayerNorm if self.point_norm == "layer" else nn.BatchNorm1d
+        self.bn1, self.bn2, self.bn3 = norm(512), norm(256), norm(128)
 
     def _trunk(self, xyz, full_points, input_set):
         """encoder + the three shared head layers -> [B,128,N]."""
@@ -45,6 +55,11 @@ class _SegBase(nn.Module):
         _, l3_points = self.sa3(l2_xyz, l2_points)
         g = l3_points.reshape(B, 1024)
         w = self.conv1.weight[:, :, 0]                                  # [512, 1024 + D]
+        if self.point_norm == "layer":                                  # points-major: a point's features are a row
+            x = F.linear(g, w[:, :1024], self.conv1.bias)[:, None] + F.linear(input_set.transpose(1, 2), w[:, 1024:])
+            x = F.relu(self.bn1(x))
+            x = F.relu(self.bn2(F.linear(x, self.conv2.weight[:, :, 0], self.conv2.bias)))
+            return F.relu(self.bn3(F.linear(x, self.conv3.weight[:, :, 0], self.conv3.bias))).transpose(1, 2)
         x = F.linear(g, w[:, :1024], self.conv1.bias)[:, :, None] + F.conv1d(input_set, w[:, 1024:, None])
         x = F.relu(self.bn1(x))
         x = F.relu(self.bn2(self.conv2(x)))
@@ -54,18 +69,16 @@ class _SegBase(nn.Module):
 class PointNet2Segmenter_v1(_SegBase):
     """models/pointnet2_seg.py:14-96.  forward(input_set [B,D,N]) -> [B,N,outdim]."""
 
-    def __init__(self, outdim=2, input_orient_dim=0, lambda_points=1, ball_in_xyz_space=False):
+    def __init__(self, outdim=2, input_orient_dim=0, lambda_points=1, ball_in_xyz_space=False, point_norm="batch"):
         super().__init__()
         self.ball_in_xyz_space = ball_in_xyz_space
         self.lambda_points = lambda_points
         self.input_orient_dim = input_orient_dim
         self.outdim = outdim
         self.in_channel = (3 + input_orient_dim) * lambda_points
-        self._build(self.in_channel)
+        self._build(self.in_channel, point_norm)
         self.conv4 = nn.Conv1d(128, outdim, 1)
-        self.bn1 = nn.BatchNorm1d(512)
-        self.bn2 = nn.BatchNorm1d(256)
-        self.bn3 = nn.BatchNorm1d(128)
+        self._build_norms()
 
     def forward(self, input_set, **kwargs):
         B, D, N = input_set.shape
@@ -83,21 +96,19 @@ class PointNet2Segmenter_v1(_SegBase):
 class PointNet2Segmenter_PaintNet_v1(_SegBase):
     """models/pointnet2_seg.py:258-339.  forward(input_set [B,3,N]) -> [B,N,lambda*(outdim_trasl+outdim_orient)]."""
 
-    def __init__(self, inputdim=3, outdim_trasl=3, outdim_orient=3, weight_orient=1., lambda_points=1):
+    def __init__(self, inputdim=3, outdim_trasl=3, outdim_orient=3, weight_orient=1., lambda_points=1, point_norm="batch"):
         super().__init__()
         self.lambda_points = lambda_points
         self.outdim_trasl = outdim_trasl
         self.outdim_orient = outdim_orient
         self.weight_orient = weight_orient
         self.in_channel = inputdim
-        self._build(inputdim)
+        self._build(inputdim, point_norm)
         self.conv4_trasl = nn.Conv1d(128, outdim_trasl * lambda_points, 1)
         if outdim_orient > 0:
             self.conv4_orient = nn.Conv1d(128, outdim_orient * lambda_points, 1)
             self.tanh = nn.Tanh()
-        self.bn1 = nn.BatchNorm1d(512)
-        self.bn2 = nn.BatchNorm1d(256)
-        self.bn3 = nn.BatchNorm1d(128)
+        self._build_norms()
 
     def forward(self, input_set, **kwargs):
         B, D, N = input_set.shape
