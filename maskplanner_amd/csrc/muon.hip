@@ -8,8 +8,8 @@
 // at 3 m^2 n + (4 h - 3) m^3 multiply-adds (symmetric products: the lower half only, mirrored) instead of h (3 m^2 n + m^3).  An extra step in
 // a hop multiplies the relative error of the smallest eigenvalues by a^2 ~ 12 (they grow by that, the rounding error of A does not shrink):
 // fp32 results take hops of at most two steps (error within 2x of the step-by-step form in fp32), 16-bit results of up to all five
-// (measured worst case 6e-4 relative for a matrix dominated by one direction, half a step of bf16 is 4e-3); hop_plan() takes the
-// cheapest schedule.
+// (measured worst case 6e-4 relative for a matrix dominated by one direction, half a step of bf16 is 4e-3); plan_hops()
+// takes the cheapest schedule.
 //
 // ARITHMETIC.  fp32 accuracy from the fp16 matrix cores: an operand is kept as two fp16 planes, x 2^k = h + l (h = fp16(x 2^k), l the rest:
 // 22 to 24 bits), a product is h h + h l + l h accumulated in fp32 -- three products at the fp16 rate (2.5 PFLOP/s) against one at the
@@ -688,29 +688,47 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
     return ldexpf(1.0f, 15 - e);
 }
 
-int hop_plan(const Shape& s, int steps, int dtype, int planes)
+// Steps a hop of every matrix of a chunk.  Allowed: fp32 two from n = 2 m on (it saves a fifth there; nearer to square less than 15 %, and
+// the error doubles: 128 x 131: 2.6e-6 of the exact result against 1.4e-6 step by step), 16-bit types all steps.  Of one limit for the whole
+// chunk the cheapest is taken: work at 0.8 PFLOP/s of plane products, and 6.5 us a launch -- hops of different lengths take turns, which costs
+// a list of small matrices more than it saves (the encoder's nine in fp32: 17 launches of one step each, 23 of mixed lengths).
+int hop_cap(const Shape& s, int steps, int dtype) { return dtype == MP_DTYPE_F32 ? (s.n >= 2 * s.m && steps > 1 ? 2 : 1) : steps; }
+
+void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, int* hop)
 {
-    // steps of a hop: cheapest of the allowed lengths (a hop of h: 3 m^2 n + (4 h - 3) m^3 against h (3 m^2 n + m^3)); ties to the short one
-    // (fp32: two steps a hop only from n = 2 m on, where it saves a fifth; nearer to square it saves less than 15 % and the error
-    // doubles: 128 x 131: 2.6e-6 of the exact result against 1.4e-6 step by step)
-    const int most = dtype == MP_DTYPE_F32 ? (s.n >= 2 * s.m ? 2 : 1) : steps;
-    int best = 1;
-    double cost = 1e300;
-    for (int h = 1; h <= most; ++h) {
-        double c = 0.0;
-        for (int left = steps; left > 0;) {
-            const int k = left < h ? left : h;
-            // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
-            c += left == steps && planes == 1 ? (1.0 + 2.0 * 2.0) * (double)s.n : 3.0 * 3.0 * (double)s.n;
-            c += 3.0 * (4.0 * k - 3.0) * (double)s.m;
-            left -= k;
+    double best = 1e300;
+    for (int h = 1; h <= steps; ++h) {
+        int use[MAX_MAT];
+        bool more = h == 1;
+        double work = 0.0;
+        int launches = 2;
+        for (int q = 0; q < k; ++q) {
+            const int cap = hop_cap(s[q], steps, dtype);
+            use[q] = h < cap ? h : cap;
+            more = more || use[q] == h;
+            const double m = (double)s[q].m, n = (double)s[q].n;
+            for (int left = steps; left > 0; left -= use[q]) {
+                const int len = left < use[q] ? left : use[q];
+                // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
+                work += 2.0 * m * m * ((left == steps && planes == 1 ? 1.0 + 2.0 * 2.0 : 3.0 * 3.0) * n + 3.0 * (4.0 * len - 3.0) * m);
+            }
         }
-        if (c < cost * 0.999) {
-            cost = c;
-            best = h;
+        if (!more) break;        // (no matrix may take that many)
+        for (int round = 0;; ++round) {
+            int len = 0;
+            for (int q = 0; q < k; ++q) {
+                const int left = steps - round * use[q], l = left < use[q] ? left : use[q];
+                len = l > len ? l : len;
+            }
+            if (len <= 0) break;
+            launches += len == 1 ? 3 : 3 * len + 1;       // Gram, apply; Q a step; T (and R), A between steps; R behind the last
+        }
+        const double cost = work / 0.8e15 + launches * 6.5e-6;
+        if (cost < best * 0.999) {
+            best = cost;
+            for (int q = 0; q < k; ++q) hop[q] = use[q];
         }
     }
-    return best;
 }
 
 size_t up(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -724,9 +742,8 @@ int norm_blocks(const Shape& s)
     return (int)(b < MAX_NORM_BLOCKS ? (b > 0 ? b : 1) : MAX_NORM_BLOCKS);
 }
 
-size_t layout(const Shape& s, int steps, int dtype, int planes, char* base, Buffers* b)
+size_t layout(const Shape& s, int steps, int hop, char* base, Buffers* b)
 {
-    const int hop = hop_plan(s, steps, dtype, planes);
     size_t at = 0;
     auto take = [&](size_t n) {
         char* p = base ? base + at : nullptr;
@@ -890,16 +907,21 @@ int next_chunk(int64_t count, const int64_t* rows, const int64_t* cols, int64_t&
 
 size_t chunk_bytes(const int64_t* rows, const int64_t* cols, const int64_t* idx, int k, int steps, int dtype)
 {
-    size_t bytes = 0, part = 0;
+    Shape sh[MAX_MAT];
+    size_t part = 0, most = 0;
     for (int q = 0; q < k; ++q) {
-        const Shape s = shape_of(rows[idx[q]], cols[idx[q]]);
-        // (one size for both uses of 16-bit matrices: as they are, or with a momentum)
-        const size_t one = layout(s, steps, dtype, 1, nullptr, nullptr), two = layout(s, steps, dtype, 2, nullptr, nullptr);
-        bytes += one > two ? one : two;
+        const Shape s = sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
         // cut tiles of any of its products (two m x m ones may share a launch): at most MAX_CUT segments of every tile
         part += (size_t)MAX_CUT * 2 * ((s.m + 255) / 256 * 256) * ((s.n + 255) / 256 * 256) * sizeof(float);
     }
-    return bytes + up(part < PART_BYTES ? part : PART_BYTES);
+    for (int planes = 1; planes <= 2; ++planes) {        // (one size for both uses of 16-bit matrices: as they are, or with a momentum)
+        int hop[MAX_MAT];
+        plan_hops(sh, k, steps, dtype, planes, hop);
+        size_t bytes = 0;
+        for (int q = 0; q < k; ++q) bytes += layout(sh[q], steps, hop[q], nullptr, nullptr);
+        most = bytes > most ? bytes : most;
+    }
+    return most + up(part < PART_BYTES ? part : PART_BYTES);
 }
 
 int check_args(int64_t count, const int64_t* rows, const int64_t* cols, int dtype, int steps)
@@ -927,10 +949,10 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     a.planes = dtype != MP_DTYPE_F32 && !mom ? 1 : 2;
     int64_t blocks = 0, tiles = 0;
     double elems = 0.0;
+    for (int q = 0; q < k; ++q) sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
+    plan_hops(sh, k, steps, dtype, a.planes, hop);
     for (int q = 0; q < k; ++q) {
-        sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
-        hop[q] = hop_plan(sh[q], steps, dtype, a.planes);
-        ws += layout(sh[q], steps, dtype, a.planes, ws, &bf[q]);
+        ws += layout(sh[q], steps, hop[q], ws, &bf[q]);
         Mat& m = a.m[q];
         const bool tall = sh[q].rows > sh[q].cols;
         m.g = in[idx[q]];
