@@ -536,6 +536,7 @@ static_assert(sizeof(Mats) <= 3584, "travels in the kernel arguments");
 
 // momentum (if any) updated and the sums of squares of the update's direction, one partial sum per workgroup (fp64: the squares of fp32
 // numbers neither overflow nor vanish there)
+template <int DT, bool MOM>
 __global__ __launch_bounds__(256) void ns_norm_kernel(Mats a)
 {
     __shared__ double s_acc[4];
@@ -544,25 +545,33 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Mats a)
     const size_t n = (size_t)m.rows * m.cols;
     const int b = blockIdx.x - a.blk0[i];
     double s = 0.0;
-#pragma unroll 4
-    for (size_t e = ((size_t)b * 256 + threadIdx.x) * 4; e < n; e += (size_t)m.blocks * 1024) {
-        const int64_t left = (int64_t)(n - e);
-        float u[4];
-        load4(m.g, a.dtype, e, left, u);
-        if (m.mom) {
-            float v[4];
-            load4(m.mom, MP_DTYPE_F32, e, left, v);
+    for (size_t e0 = (size_t)b * 4096 + threadIdx.x * 4; e0 < n; e0 += (size_t)m.blocks * 4096) {
+        float u[4][4], v[4][4];        // four loads on their way before the first is used
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[k] = v[k] + (1.0f - a.mu) * (u[k] - v[k]);
-                u[k] = a.nesterov ? u[k] + a.mu * (v[k] - u[k]) : v[k];
-            }
-            if (left >= 4) __builtin_memcpy(m.mom + e, v, 16);
-            else
-                for (int k = 0; k < (int)left; ++k) m.mom[e + k] = v[k];
+        for (int q = 0; q < 4; ++q) {
+            const int64_t left = (int64_t)n - (int64_t)(e0 + q * 1024);
+            load4(m.g, DT, e0 + q * 1024, left, u[q]);
+            if constexpr (MOM) load4(m.mom, MP_DTYPE_F32, e0 + q * 1024, left, v[q]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s += (double)u[k] * (double)u[k];
+        for (int q = 0; q < 4; ++q) {
+            const size_t e = e0 + q * 1024;
+            if (e >= n) break;
+            if constexpr (MOM) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[q][k] = v[q][k] + (1.0f - a.mu) * (u[q][k] - v[q][k]);
+                    u[q][k] = a.nesterov ? u[q][k] + a.mu * (v[q][k] - u[q][k]) : v[q][k];
+                }
+                if (n - e >= 4) __builtin_memcpy(m.mom + e, v[q], 16);
+                else
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+                        if (e + k < n) m.mom[e + k] = v[q][k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += (double)u[q][k] * (double)u[q][k];
+        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -971,7 +980,19 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     }
     for (int q = k; q < MAX_MAT; ++q) a.blk0[q] = a.tile0[q] = 0x7fffffff;
     const double esz = dtype == MP_DTYPE_F32 ? 4.0 : 2.0;
-    MP_LAUNCH("ns_norm_kernel", 2.0 * elems, elems * (esz + (mom ? 8.0 : 0.0)), ns_norm_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+#define NS_NORM(DT, MOM) \
+    MP_LAUNCH("ns_norm_kernel", 2.0 * elems, elems * (esz + (mom ? 8.0 : 0.0)), (ns_norm_kernel<DT, MOM>), dim3((unsigned)blocks), dim3(256), 0, stream, a)
+    if (dtype == MP_DTYPE_F32) {
+        if (mom) NS_NORM(MP_DTYPE_F32, true);
+        else NS_NORM(MP_DTYPE_F32, false);
+    } else if (dtype == MP_DTYPE_F16) {
+        if (mom) NS_NORM(MP_DTYPE_F16, true);
+        else NS_NORM(MP_DTYPE_F16, false);
+    } else {
+        if (mom) NS_NORM(MP_DTYPE_BF16, true);
+        else NS_NORM(MP_DTYPE_BF16, false);
+    }
+#undef NS_NORM
     MP_CHECK_LAUNCH();
     MP_LAUNCH("ns_planes_kernel", 2.0 * elems, elems * (esz + (mom ? 4.0 : 0.0) + 8.0), ns_planes_kernel, dim3((unsigned)tiles), dim3(256), 0, stream, a);
     MP_CHECK_LAUNCH();
