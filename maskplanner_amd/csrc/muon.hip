@@ -650,6 +650,250 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
     }
 }
 
+// ---- small matrices: everything in one launch ------------------------------------------------------------------------------------
+// m <= 64 and planes that fit a CU's LDS: a workgroup of eight waves has a matrix from gradient to result.  17 launches of a few
+// microseconds would be all there is to it (64 x 64 fp32: 100 us, <SMALL> here; from m = 96 on the launches win: 128 x 131 took 118 us this
+// way).  Wave v holds the columns of blocks v, v + 8, .. of 32 of X in registers (packed planes, in the accumulator layout of the product
+// that made them: that layout is the right operand's of the next product Q X if Q's columns are read in the same order, two runs of four).
+// LDS holds X's planes for the Gram product and one m x m matrix, A and then Q.
+struct Small {
+    const void* g;
+    float* mom;
+    void* out;
+    int rows, cols;
+    float fmul, fdecay;
+};
+constexpr int MAX_SMALL = 64;
+struct Smalls {
+    int count, nesterov, update, steps;
+    float mu, a, b, c, sX, sA, sQ;
+    double eps;
+    Small m[MAX_SMALL];
+};
+static_assert(sizeof(Smalls) <= 3584, "travels in the kernel arguments");
+
+constexpr int SMALL_LDS = 147456 + 256;        // (256: the padding of the fp32 tile that lies over X's planes on the way in and out)
+constexpr int small_nb(int mb) { return mb == 1 ? 4 : 2; }      // column blocks a wave
+
+template <int MB, int DT>
+__global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
+{
+    constexpr int NB = small_nb(MB);
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double s_sum[8];
+    const Small m = a.m[blockIdx.x];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 31, fh = lane >> 5, odd = lane & 1;
+    const bool tall = m.rows > m.cols;
+    const int M = tall ? m.cols : m.rows, N = tall ? m.rows : m.cols, npc = chunks(N);
+    char* S = lds;
+    char* X = lds + 32 * MB * MB * 128;
+    auto unit = [&](char* img, int row, int nch, int chunk, int u) { return img + ((size_t)row * nch + chunk) * 128 + ((u ^ (row & 7)) * 16); };
+
+    // In and out by way of LDS (over X's planes): a wave reads rows of the matrix as it lies in memory.
+    float* const t = reinterpret_cast<float*>(X);
+    const int stride = npc * 32 + 1, sr = tall ? 1 : stride, sc = tall ? stride : 1;       // element (r, c) of the matrix at t[r sr + c sc]
+    double sum = 0.0;
+    if (M < 32 * MB || N < npc * 32) {         // rows and columns that fill up the blocks: zeros
+        for (int q = threadIdx.x; q < 32 * MB * stride; q += 512) t[q] = 0.0f;
+        __syncthreads();
+    }
+    for (int r0 = wave; r0 < m.rows; r0 += 32)
+        for (int c = lane; c < m.cols; c += 64) {
+            float x[4], v[4];           // four rows on their way at once
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const size_t at = (size_t)(r0 + 8 * q) * m.cols + c;
+                if (r0 + 8 * q < m.rows) {
+                    x[q] = load_any(m.g, DT, at);
+                    v[q] = m.mom ? m.mom[at] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int rr = r0 + 8 * q;
+                if (rr >= m.rows) continue;
+                if (m.mom) {
+                    v[q] = v[q] + (1.0f - a.mu) * (x[q] - v[q]);
+                    m.mom[(size_t)rr * m.cols + c] = v[q];
+                    x[q] = a.nesterov ? x[q] + a.mu * (v[q] - x[q]) : v[q];
+                }
+                sum += (double)x[q] * (double)x[q];
+                t[rr * sr + c * sc] = x[q];
+            }
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += s_sum[k];
+    const double norm = sqrt(sum);
+    int e2 = 0;
+    if (norm > 0.0 && norm < 1e300) {       // the norm to [2^13, 2^14), as in ns_planes_kernel
+        (void)frexp(norm, &e2);
+        e2 = 14 - e2;
+    }
+    const float r = (float)(1.0 / ldexp(norm > a.eps || norm != norm ? norm : a.eps, e2));
+    unsigned xp[NB][MB][16];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int row = 32 * i + (k & 3) + 8 * (k >> 2) + 4 * fh, col = (wave + 8 * b) * 32 + fr;
+                xp[b][i][k] = wave + 8 * b < npc ? planes_of(ldexpf(t[row * stride + col], e2)) : 0u;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    __syncthreads();
+
+    float sx = r;           // X = planes * sx
+    for (int step = 0; step < a.steps; ++step) {
+        // (a zero the compiler does not know: it would keep the addresses of every access below in registers across the steps, and spill)
+        int zero = 0;
+        asm volatile("" : "+v"(zero));
+        S = lds + zero;
+        X = lds + 32 * MB * MB * 128 + zero;
+        // X's planes to LDS.  A lane has a column: neighbours swap so that each writes two columns of one row.
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int nb = wave + 8 * b;
+            if (nb < npc)
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    const unsigned p0 = xp[b][i][k], p1 = xp[b][i][k + 1];
+                    const unsigned mine = odd ? p1 : p0, got = mp::dpp_u32<mp::DPP_QUAD_XOR1>(odd ? p0 : p1);
+                    const unsigned lo = odd ? got : mine, hi = odd ? mine : got;
+                    const int row = 32 * i + (k & 3) + 8 * (k >> 2) + 4 * fh + odd;
+                    *reinterpret_cast<unsigned*>(unit(X, row, npc, nb, fr >> 3) + (fr & 6) * 2) = __builtin_amdgcn_perm(hi, lo, 0x05040100);
+                    *reinterpret_cast<unsigned*>(unit(X, row, npc, nb, 4 + (fr >> 3)) + (fr & 6) * 2) = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+                    __builtin_amdgcn_sched_barrier(0);       // (here and below: addresses and fragments of all of it at once do not fit the registers)
+                }
+        }
+        __syncthreads();
+        auto product = [&](char* img, int nch, int i, int j) {        // rows 32 i .. of the image times rows 32 j ..
+            float16v acc;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
+            const int ri = 32 * i + fr, rj = 32 * j + fr;
+            for (int c = 0; c < nch; ++c)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    const half8 lh = *reinterpret_cast<const half8*>(unit(img, ri, nch, c, ks * 2 + fh)), ll = *reinterpret_cast<const half8*>(unit(img, ri, nch, c, 4 + ks * 2 + fh));
+                    const half8 rh = *reinterpret_cast<const half8*>(unit(img, rj, nch, c, ks * 2 + fh)), rl = *reinterpret_cast<const half8*>(unit(img, rj, nch, c, 4 + ks * 2 + fh));
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, acc, 0, 0, 0);
+                }
+            return acc;
+        };
+        auto keep = [&](const float16v& v, float scale, int i, int j) {      // block (i, j) of a symmetric matrix as block (j, i): runs of four
+#pragma unroll
+            for (int rg = 0; rg < 4; ++rg) {
+                half4 h, l;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = v[rg * 4 + e] * scale;
+                    h[e] = (_Float16)x;
+                    l[e] = (_Float16)(x - (float)h[e]);
+                }
+                *reinterpret_cast<half4*>(unit(S, 32 * j + fr, MB, i, rg) + fh * 8) = h;
+                *reinterpret_cast<half4*>(unit(S, 32 * j + fr, MB, i, 4 + rg) + fh * 8) = l;
+            }
+        };
+        // A, then Q, block (i, j) by wave i MB + j
+        float16v A;
+        const int i0 = wave / MB, j0 = wave % MB;
+        const bool mine = wave < MB * MB;
+        if (mine) {
+            A = product(X, npc, i0, j0);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) A[k] *= sx * sx;
+            keep(A, a.sA, i0, j0);
+        }
+        __syncthreads();
+        if (mine) {
+            const float16v sq = product(S, MB, i0, j0);
+            const float cc = a.c / (a.sA * a.sA);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int row = 32 * i0 + (k & 3) + 8 * (k >> 2) + 4 * fh;
+                A[k] = cc * sq[k] + a.b * A[k] + (row == 32 * j0 + fr && row < M ? a.a : 0.0f);
+            }
+        }
+        __syncthreads();
+        if (mine) keep(A, a.sQ, i0, j0);
+        __syncthreads();
+        const bool last = step + 1 == a.steps;
+        const float alpha = sx / a.sQ;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int nb = wave + 8 * b;
+            if (nb < npc) {
+            float16v acc[MB];
+#pragma unroll
+            for (int i = 0; i < MB; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[i][k] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < MB; ++c)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    // k slot j of half fh is row 16 ks + 8 (j >> 2) + 4 fh + (j & 3) of the chunk, on both sides
+                    uint4v wh, wl;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        wh[e] = __builtin_amdgcn_perm(xp[b][c][8 * ks + 2 * e + 1], xp[b][c][8 * ks + 2 * e], 0x05040100);
+                        wl[e] = __builtin_amdgcn_perm(xp[b][c][8 * ks + 2 * e + 1], xp[b][c][8 * ks + 2 * e], 0x07060302);
+                    }
+                    const half8 rh = __builtin_bit_cast(half8, wh), rl = __builtin_bit_cast(half8, wl);
+#pragma unroll
+                    for (int i = 0; i < MB; ++i) {
+                        const int row = 32 * i + fr;
+                        const half4 h0 = *reinterpret_cast<const half4*>(unit(S, row, MB, c, 2 * ks) + fh * 8);
+                        const half4 h1 = *reinterpret_cast<const half4*>(unit(S, row, MB, c, 2 * ks + 1) + fh * 8);
+                        const half4 l0 = *reinterpret_cast<const half4*>(unit(S, row, MB, c, 4 + 2 * ks) + fh * 8);
+                        const half4 l1 = *reinterpret_cast<const half4*>(unit(S, row, MB, c, 4 + 2 * ks + 1) + fh * 8);
+                        const half8 lh = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7), ll = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh, acc[i], 0, 0, 0);
+                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl, acc[i], 0, 0, 0);
+                        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, acc[i], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            if (!last) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) xp[b][i][k] = planes_of(acc[i][k] * alpha * a.sX);
+            } else {        // (the planes are not read any more)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const int row = 32 * i + (k & 3) + 8 * (k >> 2) + 4 * fh;
+                        t[row * stride + nb * 32 + fr] = acc[i][k] * alpha;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+            }
+        }
+        sx = 1.0f / a.sX;
+    }
+    __syncthreads();
+    for (int rr = wave; rr < m.rows; rr += 8)
+#pragma unroll 2
+        for (int c = lane; c < m.cols; c += 64) {
+            const size_t at = (size_t)rr * m.cols + c;
+            float x = t[rr * sr + c * sc];
+            if (a.update) x = m.fdecay * load_any(m.out, DT, at) - m.fmul * x;
+            store_fin(m.out, DT, at, x);
+        }
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 struct Shape { int64_t rows, cols, m, n; };
 
@@ -780,7 +1024,8 @@ constexpr int CUS = 256;
 struct Plan { int shape, whole, seg; };
 // Tile shapes.  cyc: cycles of a chunk on one CU (three plane products) with all CUs at work, as measured; epi: of the epilogue.
 struct TileShape { int tm, tn; double cyc, epi; };
-constexpr TileShape SHAPES[3] = {{256, 128, 1900.0, 12000.0}, {128, 128, 1150.0, 6500.0}, {64, 64, 450.0, 3500.0}};
+constexpr int NSHAPES = 4;
+constexpr TileShape SHAPES[NSHAPES] = {{256, 128, 1900.0, 12000.0}, {128, 128, 1150.0, 6500.0}, {64, 64, 450.0, 4500.0}, {32, 32, 210.0, 1500.0}};
 // accumulators of the cut tiles
 constexpr size_t PART_BYTES = (size_t)96 << 20;
 constexpr int MAX_CUT = 32;
@@ -791,7 +1036,7 @@ Plan plan_of(const Prob* p, int count, int products)
 {
     Plan best{-1, 0, 0};
     double best_cost = 1e300;
-    for (int s = 0; s < 3; ++s) {
+    for (int s = 0; s < NSHAPES; ++s) {
         int64_t tiles = 0, units = 0;
         int kmin = 1 << 30, kmax = 0;
         for (int i = 0; i < count; ++i) {
@@ -896,7 +1141,8 @@ int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
 #define NS_SHAPES(PL, PR)                                                                  \
     return pl.shape == 0   ? launch_as<4, 2, PL, PR, false>(a, tag, flops, stream)         \
            : pl.shape == 1 ? launch_as<2, 2, PL, PR, false>(a, tag, flops, stream)         \
-                           : launch_as<2, 2, PL, PR, true>(a, tag, flops, stream)
+           : pl.shape == 2 ? launch_as<2, 2, PL, PR, true>(a, tag, flops, stream)          \
+                           : launch_as<1, 1, PL, PR, true>(a, tag, flops, stream)
     if (left == 2 && right == 2) NS_SHAPES(2, 2);
     if (left == 2) NS_SHAPES(2, 1);
     NS_SHAPES(1, 1);
@@ -904,6 +1150,75 @@ int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
 }
 
 struct Update { int on; double lr, mu, decay; int nesterov, scale; };
+
+double update_scale(const Update& u, int64_t rows, int64_t cols)
+{
+    const double r = (double)rows, c = (double)cols;
+    return u.scale == MP_MUON_SCALE_MATCH_RMS ? 0.2 * sqrt(r > c ? r : c) : u.scale == MP_MUON_SCALE_ORIGINAL ? sqrt(r > c ? r / c : 1.0) : 1.0;
+}
+
+// LDS that ns_small_kernel needs for a matrix; 0: it is not for it
+size_t small_lds(int64_t rows, int64_t cols)
+{
+    const Shape s = shape_of(rows, cols);
+    if (s.m > 64 || s.n > 1024) return 0;
+    const int mb = chunks(s.m), npc = chunks(s.n);
+    const size_t lds = (size_t)32 * mb * 128 * (npc + mb) + 256;
+    return npc <= 8 * small_nb(mb) && lds <= SMALL_LDS ? lds : 0;
+}
+
+bool all_small(int64_t count, const int64_t* rows, const int64_t* cols)
+{
+    for (int64_t i = 0; i < count; ++i)
+        if (rows[i] > 0 && cols[i] > 0 && !small_lds(rows[i], cols[i])) return false;
+    return true;
+}
+
+template <int MB, int DT>
+int launch_small(const Smalls& a, double flops, double bytes, size_t lds, hipStream_t stream)
+{
+    static mp::DynLds dyn;
+    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_small_kernel<MB, DT>), SMALL_LDS)) return MP_ELAUNCH;
+    MP_LAUNCH("ns_small_kernel", flops, bytes, (ns_small_kernel<MB, DT>), dim3((unsigned)a.count), dim3(512), lds, stream, a);
+    MP_CHECK_LAUNCH();
+    return MP_OK;
+}
+template <int MB>
+int launch_small_of(const Smalls& a, int dtype, double flops, double bytes, size_t lds, hipStream_t stream)
+{
+    if (dtype == MP_DTYPE_F32) return launch_small<MB, MP_DTYPE_F32>(a, flops, bytes, lds, stream);
+    if (dtype == MP_DTYPE_F16) return launch_small<MB, MP_DTYPE_F16>(a, flops, bytes, lds, stream);
+    return launch_small<MB, MP_DTYPE_BF16>(a, flops, bytes, lds, stream);
+}
+
+// one launch for the matrices of each number of 32-row blocks
+int run_small(int64_t count, const void* const* in, void* const* out, float* const* mom, const int64_t* rows, const int64_t* cols, int dtype, int steps,
+              const double* coef, double eps, const Bounds& bd, const Update& u, hipStream_t stream)
+{
+    Smalls a;
+    a.nesterov = u.nesterov; a.update = u.on; a.steps = steps;
+    a.mu = (float)u.mu; a.a = (float)coef[0]; a.b = (float)coef[1]; a.c = (float)coef[2]; a.eps = eps;
+    a.sX = pow2_scale(bd.x); a.sA = pow2_scale(bd.x * bd.x); a.sQ = pow2_scale(bd.q);
+    for (int mb = 1; mb <= 2; ++mb)
+        for (int64_t i = 0; i < count;) {
+            size_t lds = 0;
+            double elems = 0.0, flops = 0.0;
+            for (a.count = 0; i < count && a.count < MAX_SMALL; ++i) {
+                const Shape s = shape_of(rows[i], cols[i]);
+                if (s.m <= 0 || chunks(s.m) != mb) continue;
+                const size_t need = small_lds(rows[i], cols[i]);
+                lds = need > lds ? need : lds;
+                a.m[a.count++] = Small{in[i], mom ? mom[i] : nullptr, out[i], (int)rows[i], (int)cols[i], (float)(u.lr * update_scale(u, rows[i], cols[i])),
+                                       (float)(1.0 - u.lr * u.decay)};
+                elems += (double)s.m * s.n;
+                flops += 6.0 * steps * s.m * s.m * (2.0 * s.n + s.m);
+            }
+            if (a.count == 0) break;
+            const int rc = mb == 1 ? launch_small_of<1>(a, dtype, flops, elems * 8.0, lds, stream) : launch_small_of<2>(a, dtype, flops, elems * 8.0, lds, stream);
+            if (rc) return rc;
+        }
+    return MP_OK;
+}
 
 // next chunk of matrices that have elements, from index i on: their indices (<= MAX_MAT)
 int next_chunk(int64_t count, const int64_t* rows, const int64_t* cols, int64_t& i, int64_t* idx)
@@ -1090,9 +1405,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                 p.fin = out[idx[q]];
                 p.fin_t = tall;
                 if (up_.on) {
-                    const double rr = (double)sh[q].rows, cc = (double)sh[q].cols;
-                    const double sc = up_.scale == MP_MUON_SCALE_MATCH_RMS ? 0.2 * sqrt(rr > cc ? rr : cc) : up_.scale == MP_MUON_SCALE_ORIGINAL ? sqrt(rr > cc ? rr / cc : 1.0) : 1.0;
-                    p.fmul = (float)(up_.lr * sc);
+                    p.fmul = (float)(up_.lr * update_scale(up_, sh[q].rows, sh[q].cols));
                     p.fdecay = (float)(1.0 - up_.lr * up_.decay);
                 }
                 --left;
@@ -1126,14 +1439,17 @@ int run_all(int64_t count, const void* const* in, void* const* out, float* const
     const Bounds bd = bounds_of(steps, coef);
     if (!bd.ok) return MP_EUNSUPPORTED;
     int64_t idx[MAX_MAT];
+    const bool small = all_small(count, rows, cols);
     for (int64_t i = 0; i < count;) {       // everything is checked before anything is launched
         const int k = next_chunk(count, rows, cols, i, idx);
         if (k == 0) continue;
         for (int q = 0; q < k; ++q)
             if (!in[idx[q]] || !out[idx[q]] || (u.on && !mom[idx[q]])) return MP_EINVAL;
+        if (small) continue;
         if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255)) return MP_EWORKSPACE;
         if (chunk_bytes(rows, cols, idx, k, steps, dtype) > workspace_bytes) return MP_EWORKSPACE;
     }
+    if (small) return run_small(count, in, out, mom, rows, cols, dtype, steps, coef, eps, bd, u, stream);
     for (int64_t i = 0; i < count;) {
         const int k = next_chunk(count, rows, cols, i, idx);
         if (k == 0) continue;
@@ -1150,6 +1466,7 @@ extern "C" size_t mp_orthogonalize_workspace_bytes(int64_t count, const int64_t*
     if (check_args(count, rows, cols, dtype, steps)) return 0;
     size_t most = 0;
     int64_t idx[MAX_MAT];
+    if (all_small(count, rows, cols)) return 0;
     for (int64_t i = 0; i < count;) {
         const int k = next_chunk(count, rows, cols, i, idx);
         const size_t b = k ? chunk_bytes(rows, cols, idx, k, steps, dtype) : 0;
