@@ -7,16 +7,14 @@
 //     A = X X^T;   Q_i = a I + b A_i + c A_i^2,   A_{i+1} = (A_i Q_i) Q_i,   R_i = Q_i R_{i-1};   X <- R_h X
 // at 3 m^2 n + (4 h - 3) m^3 multiply-adds (symmetric products: the lower half only, mirrored) instead of h (3 m^2 n + m^3).  An extra step in
 // a hop multiplies the relative error of the smallest eigenvalues by a^2 ~ 12 (they grow by that, the rounding error of A does not shrink):
-// fp32 results take hops of at most two steps (error within 2x of the step-by-step form in fp32), 16-bit results of up to all five
-// (measured worst case 6e-4 relative for a matrix dominated by one direction, half a step of bf16 is 4e-3); plan_hops()
-// takes the cheapest schedule.
+// hop_cap() says how many a type allows, plan_hops() takes the cheapest schedule.
 //
 // ARITHMETIC.  fp32 accuracy from the fp16 matrix cores: an operand is kept as two fp16 planes, x 2^k = h + l (h = fp16(x 2^k), l the rest:
 // 22 to 24 bits), a product is h h + h l + l h accumulated in fp32 -- three products at the fp16 rate (2.5 PFLOP/s) against one at the
 // fp32 rate (0.16).  The power of two puts the largest entry below 2^15, so l keeps its bits down to entries of 2^-24 of that.
 //
-// All matrices of a call go through each stage in ONE launch (problem list in the kernel arguments): a call is 2 + 3..17 launches
-// whatever the number of matrices.  Operand image: row r = chunks of 32 k, each [h: 32 fp16][l: 32 fp16] (128 bytes); columns up to the
+// All matrices of a call (up to 12 at a time) go through each stage in ONE launch (problem list in the kernel arguments): five steps are 17 to
+// 19 launches whatever their number.  Operand image: row r = chunks of 32 k, each [h: 32 fp16][l: 32 fp16] (128 bytes); columns up to the
 // chunk's end are zero, rows end where the matrix does (loads clamp the row).  X is kept in both orientations (X for the Gram product, X^T for
 // the product with R: both contract over the last axis).
 #include "common.h"
@@ -311,7 +309,7 @@ template <int PL> __device__ __forceinline__ int swz(int row) { return PL == 2 ?
 
 // KW: the four waves share a (32 WM) x (32 WN) tile by K instead, wave v taking chunks v, v + 4, ..: each with a ring of its own and no
 // meeting at all; their sums meet in LDS at the end, added in the order of the waves.  For 64 x 64 tiles, where a wave of the shared form has
-// three products between two meetings (136 tiles of K = 1024: 15 us against <KWTIME>).
+// three products between two meetings (136 tiles of K = 1024: 15.2 us shared, 12.7 this way).
 template <int WM, int WN, int PL, int PR, int NS, bool KW>
 __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 {
@@ -652,7 +650,7 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
 
 // ---- small matrices: everything in one launch ------------------------------------------------------------------------------------
 // m <= 64 and planes that fit a CU's LDS: a workgroup of eight waves has a matrix from gradient to result.  17 launches of a few
-// microseconds would be all there is to it (64 x 64 fp32: 100 us, <SMALL> here; from m = 96 on the launches win: 128 x 131 took 118 us this
+// microseconds would be all there is to it (64 x 64 fp32: 100 us, 31 here; from m = 96 on the launches win: 128 x 131 took 118 us this
 // way).  Wave v holds the columns of blocks v, v + 8, .. of 32 of X in registers (packed planes, in the accumulator layout of the product
 // that made them: that layout is the right operand's of the next product Q X if Q's columns are read in the same order, two runs of four).
 // LDS holds X's planes for the Gram product and one m x m matrix, A and then Q.
@@ -941,13 +939,24 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
     return ldexpf(1.0f, 15 - e);
 }
 
-// Steps a hop of every matrix of a chunk.  Allowed: fp32 two from n = 2 m on (it saves a fifth there; nearer to square less than 15 %, and
-// the error doubles: 128 x 131: 2.6e-6 of the exact result against 1.4e-6 step by step), 16-bit types all steps.  Of one limit for the whole
-// chunk the cheapest is taken: work at 0.8 PFLOP/s of plane products, and 6.5 us a launch -- hops of different lengths take turns, which costs
-// a list of small matrices more than it saves (the encoder's nine in fp32: 17 launches of one step each, 23 of mixed lengths).
-int hop_cap(const Shape& s, int steps, int dtype) { return dtype == MP_DTYPE_F32 ? (s.n >= 2 * s.m && steps > 1 ? 2 : 1) : steps; }
+// Steps a hop of every matrix of a chunk.  Allowed, with g = max |Q|^2 (a^2 = 11.9 for the usual coefficients) the growth of the smallest
+// eigenvalues' relative error a further step:
+//   fp32: two from n = 2 m on (it saves a fifth there; nearer to square less than 15 %, and the error doubles: 128 x 131: 2.6e-6 of the exact
+//         result against 1.4e-6 step by step);
+//   bf16: 2^-22 g^(h-1) <= 5e-3, five steps (worst case measured 6e-4, a matrix dominated by one direction; the result's rounding: 1.7e-3);
+//   fp16: 2^-22 g^(h-1) <= 5e-5, three steps (the rounding: 2e-4).
+// Of one limit for the whole chunk the cheapest is taken: work at 0.8 PFLOP/s of plane products, and 6.5 us a launch -- hops of different
+// lengths take turns, which costs a list of small matrices more than it saves (the encoder's nine in fp32: 17 launches of one step each, 23
+// of mixed lengths).
+int hop_cap(const Shape& s, int steps, int dtype, double g)
+{
+    const double most = dtype == MP_DTYPE_F32 ? (s.n >= 2 * s.m ? 16.0 : 1.0) : dtype == MP_DTYPE_F16 ? 200.0 : 20000.0;
+    int h = 1;
+    for (double e = g > 1.5 ? g : 1.5; h < steps && e <= most && (dtype != MP_DTYPE_F32 || h < 2); e *= g > 1.5 ? g : 1.5) ++h;
+    return h;
+}
 
-void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, int* hop)
+void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, double g, int* hop)
 {
     double best = 1e300;
     for (int h = 1; h <= steps; ++h) {
@@ -956,7 +965,7 @@ void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, int* hop
         double work = 0.0;
         int launches = 2;
         for (int q = 0; q < k; ++q) {
-            const int cap = hop_cap(s[q], steps, dtype);
+            const int cap = hop_cap(s[q], steps, dtype, g);
             use[q] = h < cap ? h : cap;
             more = more || use[q] == h;
             const double m = (double)s[q].m, n = (double)s[q].n;
@@ -995,8 +1004,10 @@ int norm_blocks(const Shape& s)
     return (int)(b < MAX_NORM_BLOCKS ? (b > 0 ? b : 1) : MAX_NORM_BLOCKS);
 }
 
-size_t layout(const Shape& s, int steps, int hop, char* base, Buffers* b)
+// (what any schedule may use: the size does not depend on the coefficients)
+size_t layout(const Shape& s, int steps, int dtype, char* base, Buffers* b)
 {
+    const bool chain = steps > 1 && (dtype != MP_DTYPE_F32 || s.n >= 2 * s.m);
     size_t at = 0;
     auto take = [&](size_t n) {
         char* p = base ? base + at : nullptr;
@@ -1008,12 +1019,12 @@ size_t layout(const Shape& s, int steps, int hop, char* base, Buffers* b)
     d.r = reinterpret_cast<float*>(take(256));
     d.X = take(image(s.m, s.n));
     d.XT = take(image(s.n, s.m));
-    d.XT2 = steps > hop ? take(image(s.n, s.m)) : nullptr;
+    d.XT2 = steps > 1 ? take(image(s.n, s.m)) : nullptr;
     d.A = take(image(s.m, s.m));
-    d.T = hop > 1 ? take(image(s.m, s.m)) : nullptr;
+    d.T = chain ? take(image(s.m, s.m)) : nullptr;
     d.P[0] = take(image(s.m, s.m));
-    d.P[1] = hop > 1 ? take(image(s.m, s.m)) : nullptr;
-    d.P[2] = hop > 1 ? take(image(s.m, s.m)) : nullptr;
+    d.P[1] = chain ? take(image(s.m, s.m)) : nullptr;
+    d.P[2] = chain ? take(image(s.m, s.m)) : nullptr;
     if (b) *b = d;
     return at;
 }
@@ -1231,21 +1242,14 @@ int next_chunk(int64_t count, const int64_t* rows, const int64_t* cols, int64_t&
 
 size_t chunk_bytes(const int64_t* rows, const int64_t* cols, const int64_t* idx, int k, int steps, int dtype)
 {
-    Shape sh[MAX_MAT];
-    size_t part = 0, most = 0;
+    size_t bytes = 0, part = 0;
     for (int q = 0; q < k; ++q) {
-        const Shape s = sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
+        const Shape s = shape_of(rows[idx[q]], cols[idx[q]]);
+        bytes += layout(s, steps, dtype, nullptr, nullptr);
         // cut tiles of any of its products (two m x m ones may share a launch): at most MAX_CUT segments of every tile
         part += (size_t)MAX_CUT * 2 * ((s.m + 255) / 256 * 256) * ((s.n + 255) / 256 * 256) * sizeof(float);
     }
-    for (int planes = 1; planes <= 2; ++planes) {        // (one size for both uses of 16-bit matrices: as they are, or with a momentum)
-        int hop[MAX_MAT];
-        plan_hops(sh, k, steps, dtype, planes, hop);
-        size_t bytes = 0;
-        for (int q = 0; q < k; ++q) bytes += layout(sh[q], steps, hop[q], nullptr, nullptr);
-        most = bytes > most ? bytes : most;
-    }
-    return most + up(part < PART_BYTES ? part : PART_BYTES);
+    return bytes + up(part < PART_BYTES ? part : PART_BYTES);
 }
 
 int check_args(int64_t count, const int64_t* rows, const int64_t* cols, int dtype, int steps)
@@ -1274,9 +1278,9 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     int64_t blocks = 0, tiles = 0;
     double elems = 0.0;
     for (int q = 0; q < k; ++q) sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
-    plan_hops(sh, k, steps, dtype, a.planes, hop);
+    plan_hops(sh, k, steps, dtype, a.planes, bd.q * bd.q, hop);
     for (int q = 0; q < k; ++q) {
-        ws += layout(sh[q], steps, hop[q], ws, &bf[q]);
+        ws += layout(sh[q], steps, dtype, ws, &bf[q]);
         Mat& m = a.m[q];
         const bool tall = sh[q].rows > sh[q].cols;
         m.g = in[idx[q]];

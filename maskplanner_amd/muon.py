@@ -11,7 +11,7 @@ class Muon(torch.optim.Optimizer):
     scale: "original" s = sqrt(max(1, rows / columns)), "match_rms" s = 0.2 sqrt(max(rows, columns)) (an update of Adam's usual size), None 1.
     Parameters: contiguous HIP tensors of at least two axes, float32, float16 or bfloat16, gradients of the same type.  The momentum
     (`momentum_buffer`) is float32 whatever the parameter's type.  All parameters of one group and type go through each stage in one launch.
-    The learning rate is fixed in a recorded graph."""
+    The learning rate is fixed in a recorded graph; one step has to come before the recording."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, scale="original", steps=5, coefficients=ops.NEWTON_SCHULZ,
                  eps=1e-7):
@@ -44,6 +44,8 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError("Muon does not take sparse gradients")
                 st = self.state[p]
                 if "momentum_buffer" not in st:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: take one step before recording a graph (a momentum made inside it would be zeroed by every replay)")
                     st["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 kinds.setdefault((p.device, p.dtype), []).append((p, p.grad, st["momentum_buffer"]))
             for rows in kinds.values():

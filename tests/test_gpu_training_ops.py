@@ -114,6 +114,32 @@ def test_muon_notices_a_stale_graph():
         loss.backward()
 
 
+def test_muon_recorded_after_one_step_and_refused_before():
+    from maskplanner_amd.muon import Muon
+
+    def make():
+        w = torch.randn(70, 90, device="cuda", generator=gen(1)).requires_grad_(True)
+        w.grad = torch.randn(70, 90, device="cuda", generator=gen(2))
+        return w, Muon([w], lr=0.1)
+    w, opt = make()
+    with pytest.raises(RuntimeError, match="before recording"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    (a, oa), (b, ob) = make(), make()
+    oa.step()
+    ob.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ob.step()
+    for k in range(3):
+        for t in (a, b):
+            t.grad.copy_(torch.randn(70, 90, device="cuda", generator=gen(20 + k)))
+        oa.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, b) and torch.equal(oa.state[a]["momentum_buffer"], ob.state[b]["momentum_buffer"])
+
+
 def test_train_step_with_muon_eager_and_replayed():
     """the replayed step makes the eager step's updates: Muon on the encoder's matrices, Adam on the rest"""
     from maskplanner_amd.harness import TrainStep

@@ -28,12 +28,14 @@ def test_c_entries_check_before_they_launch():
     assert lib.mp_layer_norm_bwd(64, 70, 64, 70, 0, 1000, 70, None, 0, 64, 64, None, 64, None, 64, need - 1, None) == _lib.MP_EWORKSPACE
     assert lib.mp_layer_norm_bwd(None, 70, 64, 70, 0, 1000, 70, None, 0, 64, 64, 64, None, None, None, 0, None) == _lib.MP_EINVAL
     # orthogonalisation
-    rows, cols = _arr(i64, [8]), _arr(i64, [9])
+    rows, cols = _arr(i64, [80]), _arr(i64, [90])
     coef = _arr(ctypes.c_double, [3.4445, -4.7750, 2.0315])
     ptr = _arr(ctypes.c_void_p, [1 << 20])
     need = lib.mp_orthogonalize_workspace_bytes(1, rows, cols, 0, 5)
     assert need > 0
     assert lib.mp_orthogonalize_workspace_bytes(1, _arr(i64, [0]), cols, 0, 5) == 0
+    assert lib.mp_orthogonalize_workspace_bytes(2, _arr(i64, [64, 3]), _arr(i64, [64, 64]), 0, 5) == 0        # small ones need none
+    assert lib.mp_orthogonalize_workspace_bytes(2, _arr(i64, [64, 80]), _arr(i64, [64, 90]), 0, 5) > need     # unless they go with others
     ok = (1, ptr, ptr, rows, cols, 0, 5, coef, 1e-7, 1 << 20, need, None)
 
     def call(**kw):
