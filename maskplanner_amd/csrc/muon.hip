@@ -300,6 +300,72 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
     }
 }
 
+// The same for a tile whose results go out as planes and whose accumulators are still in registers: formed and rounded there (a block of
+// 32 x 32: register r of lane q is row (r & 3) + 8 (r >> 2) + 4 (q >> 5), column q & 31), one packed word each through LDS, then both
+// orientations without another rounding (128 x 128: 5.9 us by way of epilogue(), <EPIREG> this way).
+template <int WM, int WN, int TM, int TN>
+__device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, const float16v (&acc)[WM][WN], int m0, int n0, int wm, int wn)
+{
+    constexpr int S = TN + TPAD;
+    const int fr = threadIdx.x & 31, fh = (threadIdx.x & 63) >> 5;
+    const float alpha = alpha_of(p) * p.so, cb = p.cb * p.so, ca = p.ca * p.so;
+    const int padN = p.oc * 32, padM = p.otc * 32;
+    const bool diagonal = p.ca != 0.0f && m0 < n0 + TN && n0 < m0 + TM, edge = m0 + TM > p.M || n0 + TN > p.N;
+#pragma unroll
+    for (int x = 0; x < WM; ++x)
+#pragma unroll
+        for (int y = 0; y < WN; ++y) {
+            const int cl = wn + 32 * y + fr, col = n0 + cl;
+            half4 ch[4], cl4[4];
+            if (p.C)            // symmetric: row `col` of it has this lane's rows side by side
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int row = m0 + wm + 32 * x + 8 * g + 4 * fh;
+                    ch[g] = cl4[g] = half4{0, 0, 0, 0};
+                    if (col < p.N && row < padM) {
+                        const _Float16* c = p.C + ((size_t)col * p.oc + (row >> 5)) * 64 + (row & 31);
+                        ch[g] = *reinterpret_cast<const half4*>(c);
+                        cl4[g] = *reinterpret_cast<const half4*>(c + 32);
+                    }
+                }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int rl = wm + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * fh, row = m0 + rl;
+                float v = alpha * acc[x][y][r];
+                if (p.C) v += cb * ((float)ch[r >> 2][r & 3] + (float)cl4[r >> 2][r & 3]);
+                if (diagonal) v += row == col ? ca : 0.0f;
+                if (edge) v = row < p.M && col < p.N ? v : 0.0f;
+                t[rl * S + cl] = planes_of(v);
+            }
+        }
+    lds_barrier();
+    // (tiles wholly inside, off the diagonal: no conditions)
+#pragma unroll 4
+    for (int q = threadIdx.x; q < TM * (TN / 8); q += 256) {
+        const int rl = q / (TN / 8), cl = q % (TN / 8) * 8, row = m0 + rl, col = n0 + cl;
+        if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) {
+            const uint4v lo = *reinterpret_cast<const uint4v*>(t + rl * S + cl), hi = *reinterpret_cast<const uint4v*>(t + rl * S + cl + 4);
+            const unsigned w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            put_packed(p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31), w);
+        }
+    }
+#pragma unroll 4
+    for (int q = threadIdx.x; q < TM / 8 * TN; q += 256) {
+        const int cl = (q >> 2) % TN, rl = (q / (4 * TN)) * 32 + (q & 3) * 8, row = m0 + rl, col = n0 + cl;
+        if (col < p.N && row < padM && !(p.sym && row >> 3 < col >> 3)) {
+            unsigned w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = t[(rl + e) * S + cl];
+            if (p.sym && row >> 3 == col >> 3) {        // on the diagonal: row `col` of the piece, left of the diagonal from itself
+                const unsigned* d = t + (col - m0) * S + (row - n0);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = row + e < col ? d[e] : w[e];
+            }
+            put_packed(p.outT + ((size_t)col * p.otc + (row >> 5)) * 64 + (row & 31), w);
+        }
+    }
+}
+
 // A tile of (64 WM) x (64 WN), four waves (2 x 2), NS LDS buffers of one 32-k chunk.  Halfway through chunk c (its second 16 k are in
 // registers by then) the workgroup meets: chunk c + 1 has arrived for everybody, buffer c is free and takes chunk c + NS; the first fragments
 // of c + 1 are read while the second half of c is multiplied.  One barrier a chunk, NS - 1 chunks of latency covered.
@@ -443,6 +509,11 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
         }
         // (nobody reads the buffers any more: the last meeting was behind the last fragment reads)
         if constexpr (KW) lds_barrier();
+        if constexpr (!KW)
+            if (n == p.kc && !p.fin) {
+                epilogue_planes<WM, WN, TM, TN>(p, reinterpret_cast<unsigned*>(lds), acc, m0, n0, wm, wn);
+                return;
+            }
         float* const t = reinterpret_cast<float*>(lds);
         float* const mine = KW ? t + wave * (TM * (TN + TPAD)) : t;
 #pragma unroll
