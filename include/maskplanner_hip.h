@@ -613,19 +613,19 @@ int mp_layer_norm_bwd(const void* dy, int64_t dy_row_stride, const void* x, int6
  * For every matrix U [rows[i], cols[i]] of the list (row-major, contiguous):
  *     X = U / max(|U|_F, eps);  `steps` times:  A = X X^T,  X <- (c0 I + c1 A + c2 A^2) X;  out = X
  * (a matrix with more rows than columns: of its transpose, transposed back).  in / out are HOST arrays of `count` device pointers of
- * `dtype` (they travel in the kernel arguments), rows / cols / coefficients [3] HOST arrays; out[i] may be in[i] (no other overlap).  Products and sums in
- * fp32 accuracy whatever the type, one rounding at the end (16-bit types: the singular values' polynomial is evaluated on the Gram
+ * `dtype` (they travel in the kernel arguments), rows / cols / coefficients [3] HOST arrays; out[i] may be in[i] (no other overlap).
+ * Products and sums in fp32 accuracy whatever the type, one rounding at the end (16-bit types: the singular values' polynomial is evaluated on the Gram
  * matrix).  The scalar recursion s <- |s (c0 + c1 s^2 + c2 s^4)| of the coefficients must keep s <= 16 from every start in [0, 1], steps <= 16,
  * min(rows, cols) <= 65536, max <= 2^21: else MP_EUNSUPPORTED.  Matrices without elements are skipped.  workspace: 256-byte aligned,
- * mp_orthogonalize_workspace_bytes bytes (of the same rows, cols, dtype and steps; 0 where all matrices are small: NULL will do), used by one
- *     call at a time. */
+ * mp_orthogonalize_workspace_bytes bytes (of the same rows, cols, dtype and steps; 0 where all matrices are small: NULL will do), used by
+ * one call at a time. */
 size_t mp_orthogonalize_workspace_bytes(int64_t count, const int64_t* rows, const int64_t* cols, int dtype, int steps);
 int mp_orthogonalize(int64_t count, const void* const* in, void* const* out, const int64_t* rows, const int64_t* cols, int dtype, int steps,
                      const double* coefficients, double eps, void* workspace, size_t workspace_bytes, mp_stream_t stream);
 /* The Muon update of a list of matrices in place: momentum m (f32) <- m + (1 - mu)(g - m);  u = nesterov ? g + mu (m - g) : m;
  *     p <- (1 - lr weight_decay) p - lr s O(u),  O the orthogonalisation above (not rounded in between),  s by `scale`:
  *     MP_MUON_SCALE_ORIGINAL sqrt(max(1, rows / cols)), MP_MUON_SCALE_MATCH_RMS 0.2 sqrt(max(rows, cols)), MP_MUON_SCALE_NONE 1.
- * params, grads of `dtype`; workspace as above. */
+ * params, grads of `dtype`; params and momentum share no memory with each other or with grads; workspace as above. */
 #define MP_MUON_SCALE_NONE 0
 #define MP_MUON_SCALE_ORIGINAL 1
 #define MP_MUON_SCALE_MATCH_RMS 2

@@ -302,7 +302,7 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
 
 // The same for a tile whose results go out as planes and whose accumulators are still in registers: formed and rounded there (a block of
 // 32 x 32: register r of lane q is row (r & 3) + 8 (r >> 2) + 4 (q >> 5), column q & 31), one packed word each through LDS, then both
-// orientations without another rounding (128 x 128: 5.9 us by way of epilogue(), <EPIREG> this way).
+// orientations without another rounding (128 x 128: 5.9 us by way of epilogue(), 5.5 this way).
 template <int WM, int WN, int TM, int TN>
 __device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, const float16v (&acc)[WM][WN], int m0, int n0, int wm, int wn)
 {
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
 
 // ---- small matrices: everything in one launch ------------------------------------------------------------------------------------
 // m <= 64 and planes that fit a CU's LDS: a workgroup of eight waves has a matrix from gradient to result.  17 launches of a few
-// microseconds would be all there is to it (64 x 64 fp32: 100 us, 31 here; from m = 96 on the launches win: 128 x 131 took 118 us this
+// microseconds would be all there is to it (64 x 64 fp32: 100 us, 26 here; from m = 96 on the launches win: 128 x 131 took 118 us this
 // way).  Wave v holds the columns of blocks v, v + 8, .. of 32 of X in registers (packed planes, in the accumulator layout of the product
 // that made them: that layout is the right operand's of the next product Q X if Q's columns are read in the same order, two runs of four).
 // LDS holds X's planes for the Gram product and one m x m matrix, A and then Q.
@@ -976,10 +976,17 @@ constexpr int MAX_STEPS = 16;
 
 struct Bounds { double x, q, r[MAX_STEPS + 1]; bool ok; };    // of |X|, |Q| and |Q^h| (products of up to h successive Q) in spectral norm
 
-// The scalar recursion of a singular value, on a grid of starting values in [0, 1]: what the matrices can grow to.
+// The scalar recursion of a singular value, on a grid of starting values in [0, 1]: what the matrices can grow to.  30 us of host time, the
+// same for all steps of a training run: a thread keeps the last one (a property of the coefficients alone; 64 x 64 fp32: 31 us a call with
+// it formed every time, 26 this way).
 Bounds bounds_of(int steps, const double* c)
 {
-    Bounds b;
+    thread_local Bounds b;
+    thread_local int of_steps = 0;
+    thread_local double of[3];
+    if (of_steps == steps && of[0] == c[0] && of[1] == c[1] && of[2] == c[2]) return b;
+    of_steps = steps;
+    for (int k = 0; k < 3; ++k) of[k] = c[k];
     b.x = 1.0; b.q = 0.0; b.ok = true;
     for (double& v : b.r) v = 0.0;
     for (int g = 0; g < 768; ++g) {
@@ -1404,9 +1411,9 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
         p.so = so;
         return p;
     };
-    int done[MAX_MAT], at[MAX_MAT], rbuf[MAX_MAT], qbuf[MAX_MAT];       // steps finished, step inside the hop, which P holds R / Q
+    int done[MAX_MAT], rbuf[MAX_MAT], qbuf[MAX_MAT];       // steps finished, which P holds R / Q
     bool first[MAX_MAT];
-    for (int q = 0; q < k; ++q) { done[q] = at[q] = 0; first[q] = true; rbuf[q] = qbuf[q] = 0; }
+    for (int q = 0; q < k; ++q) { done[q] = 0; first[q] = true; rbuf[q] = qbuf[q] = 0; }
     int left = k;
     while (left > 0) {        // every matrix is at the start of a hop (or finished); hops of one chunk may differ in length
         int len[MAX_MAT], longest = 0;

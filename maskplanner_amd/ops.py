@@ -1094,7 +1094,7 @@ def _ns_setup(op, mats, steps, coefficients, eps):
 def orthogonalize(matrices, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Newton-Schulz orthogonalisation of every matrix G: X = G / max(|G|_F, eps), `steps` times X <- (a I + b A + c A^2) X with A = X X^T
     (of the transpose where G has more rows than columns): singular values go to about 1, singular vectors stay.  `matrices`: a list of 2-D
-    tensors of one type (float32, float16, bfloat16; any sizes; strided ones are copied) -> a list of new tensors, or one tensor [..., m, n] ->
+    tensors of one type (float32, float16, bfloat16; any sizes up to 65536 by 2^21; strided ones are copied) -> a list of new tensors, or one tensor [..., m, n] ->
     one tensor.  All matrices go through each stage in one launch.  Products in fp32 accuracy, rounded once.  Not differentiable.  The
     coefficients must keep s <- |s (a + b s^2 + c s^4)| <= 16 for starts in [0, 1]."""
     if torch.is_tensor(matrices):
@@ -1126,6 +1126,18 @@ def _orthogonalize_into(mats, out, steps, coefficients, eps):
          _p(ws), nbytes)
 
 
+def _no_overlap(written, read):
+    """ValueError if a tensor of `written` shares memory with another one of either list (all contiguous)."""
+    spans = [(t.data_ptr(), t.numel() * t.element_size(), True) for t in written] + [(t.data_ptr(), t.numel() * t.element_size(), False) for t in read]
+    end = end_written = 0
+    for at, size, w in sorted(spans):
+        if size and at < (end if w else end_written):
+            raise ValueError("muon_step: a parameter or momentum buffer is given twice, or shares memory with another tensor of the call")
+        end = max(end, at + size)
+        if w:
+            end_written = max(end_written, at + size)
+
+
 @torch.no_grad()
 def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale="original", steps=5,
               coefficients=NEWTON_SCHULZ, eps=1e-7):
@@ -1142,7 +1154,6 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
     if not params:
         return
     _need_hip(*params, *grads, *bufs)
-    seen = set()
     for p, g, m in zip(params, grads, bufs):
         if p.ndim < 2:
             raise ValueError("muon_step updates matrices: a parameter has fewer than two axes")
@@ -1152,11 +1163,8 @@ def muon_step(params, grads, momentum_buffers, lr, momentum=0.95, nesterov=True,
             raise ValueError("muon_step: momentum buffers are float32")
         if not (p.is_contiguous() and m.is_contiguous()):
             raise ValueError("muon_step updates contiguous parameters and momentum buffers")
-        for t in (p, m):
-            if t.numel() and t.data_ptr() in seen:
-                raise ValueError("muon_step: a parameter or momentum buffer is given twice")
-            seen.add(t.data_ptr())
     grads = [g.contiguous() for g in grads]
+    _no_overlap(params + bufs, grads)
     dt, rows, cols, coef, ws, nbytes = _ns_setup("muon_step", params, steps, coefficients, eps)
     _run("muon_step", params[0], _lib.load().mp_muon_step, len(params), _ptrs(params), _ptrs(grads), _ptrs(bufs), rows, cols, dt, float(lr),
          float(momentum), int(bool(nesterov)), float(weight_decay), MUON_SCALES[scale], int(steps), coef, float(eps), _p(ws), nbytes)

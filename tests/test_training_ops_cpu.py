@@ -132,3 +132,15 @@ def test_train_step_refuses_unknown_optimizers():
         TrainStep("cuboids", B=2, N=256, device="cpu", optimizer="sgd")
     with pytest.raises(RuntimeError, match="MI355X"):
         TrainStep("cuboids", B=2, N=256, device="cpu", optimizer="muon", hidden_size=(64, 64))
+
+
+def test_muon_step_finds_shared_memory():
+    from maskplanner_amd.ops import _no_overlap
+    buf, g = torch.zeros(64, 8), torch.zeros(32, 8)
+    p, q, m, n = buf[:16], buf[16:32], buf[32:48], buf[48:]
+    _no_overlap([p, q, m, n], [g, g])                       # neighbours in one buffer, one gradient for two parameters
+    _no_overlap([p, q, m, n, buf[:0]], [buf[:0], buf[:0]])  # nothing to share
+    for written, read in (([p, p, m, n], [g]), ([p, m, m], [g]), ([p, buf[15:31], m, n], [g]), ([p, m], [p]), ([p, m], [buf[40:56]]),
+                          ([buf, m], [g]), ([buf[60:], p], [buf[:64]]), ([p, m, n], [g, buf[20:40], g])):
+        with pytest.raises(ValueError, match="shares memory"):
+            _no_overlap(written, read)
