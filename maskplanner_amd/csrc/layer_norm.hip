@@ -15,21 +15,44 @@
 
 namespace {
 
-template <typename T> struct LnVec {     // 16 bytes that may lie at any element address: rows of odd width are not aligned
-    static constexpr int N = 16 / (int)sizeof(T);
-    T v[N];
+// N values in whole registers, two of 16 bits to one (as an array of them the compiler gives each a register of its own)
+template <typename T, int N_> struct LnPack {
+    static constexpr int N = N_, WORDS = N * (int)sizeof(T) / 4;
+    unsigned w[WORDS];
+    __device__ __forceinline__ float at(int e) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else {
+            const unsigned short h = (unsigned short)(e & 1 ? w[e / 2] >> 16 : w[e / 2]);
+            T t;
+            __builtin_memcpy(&t, &h, 2);
+            return (float)t;
+        }
+    }
+    __device__ __forceinline__ void set(int e, T v)        // of a zero value, once
+    {
+        unsigned short h;
+        if constexpr (sizeof(T) == 4) __builtin_memcpy(&w[e], &v, 4);
+        else {
+            __builtin_memcpy(&h, &v, 2);
+            w[e / 2] |= (unsigned)h << (e & 1 ? 16 : 0);
+        }
+    }
 };
+// 16 bytes that may lie at any element address: rows of odd width are not aligned
+template <typename T> using LnVec = LnPack<T, 16 / (int)sizeof(T)>;
 
 // `left` > 0 elements from p on (16 bytes where that many are left), zeros behind
 template <typename T>
 __device__ __forceinline__ LnVec<T> ln_raw(const T* __restrict__ p, int left)
 {
     constexpr int V = LnVec<T>::N;
-    LnVec<T> t;
-    if (left >= V) __builtin_memcpy(&t, p, 16);
+    LnVec<T> t{};
+    if (left >= V) __builtin_memcpy(t.w, p, 16);
     else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) t.v[e] = e < left ? p[e] : (T)0.0f;
+        for (int e = 0; e < V; ++e)
+            if (e < left) t.set(e, p[e]);
     }
     return t;
 }
@@ -39,10 +62,10 @@ __device__ __forceinline__ void ln_store(T* __restrict__ p, int left, const floa
 {
     constexpr int V = LnVec<T>::N;
     if (left >= V) {
-        LnVec<T> t;
+        T t[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) t.v[e] = (T)in[e];       // the one rounding of the result: to nearest, ties to even
-        __builtin_memcpy(p, &t, 16);
+        for (int e = 0; e < V; ++e) t[e] = (T)in[e];       // the one rounding of the result: to nearest, ties to even
+        __builtin_memcpy(p, t, 16);
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -51,17 +74,25 @@ __device__ __forceinline__ void ln_store(T* __restrict__ p, int left, const floa
 }
 
 // V parameters (16 or, fp32 parameters of 16-bit rows, 32 bytes), kept as they are for all rows of a workgroup
-template <typename W, int V> struct LnParam { W v[V]; };
 template <typename W, int V>
-__device__ __forceinline__ LnParam<W, V> ln_param(const W* __restrict__ p, int c, int D, float def)
+__device__ __forceinline__ LnPack<W, V> ln_param(const W* __restrict__ p, int c, int D, float def)
 {
-    LnParam<W, V> t;
-    if (p && c + V <= D) __builtin_memcpy(&t, p + c, sizeof(t));
+    LnPack<W, V> t{};
+    if (p && c + V <= D) __builtin_memcpy(t.w, p + c, sizeof(t));
     else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) t.v[e] = p && c + e < D ? p[c + e] : (W)def;
+        for (int e = 0; e < V; ++e) t.set(e, p && c + e < D ? p[c + e] : (W)def);
     }
     return t;
+}
+
+// 16-bit values that are to stay as they came: the compiler would keep them converted from one use to the next, in twice the registers
+template <typename T, int N>
+__device__ __forceinline__ void ln_packed(LnPack<T, N>& t)
+{
+    if constexpr (sizeof(T) == 2)
+#pragma unroll
+        for (unsigned& x : t.w) asm volatile("" : "+v"(x));
 }
 
 // Sums of A values over the TPR threads of a row, left in all of them.  TPR <= 64: lanes of one wave, in registers (DPP inside rows of 16
@@ -109,16 +140,24 @@ __device__ __forceinline__ void row_sum(float (&v)[A], float* buf)
 // A workgroup walks rows gridDim.x apart; the next row's values are on their way while one is reduced.
 constexpr int ln_block(int tpr) { return tpr > 256 ? tpr : 256; }
 
+// row of the workgroup that this thread is on: the same for a wave from 64 threads a row on, and then its addresses are scalar
+template <int TPR> __device__ __forceinline__ int ln_slot()
+{
+    if constexpr (TPR >= 256) return 0;
+    else if constexpr (TPR == 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    else return threadIdx.x / TPR;
+}
+
 template <typename T, typename W, int TPR, int NV>
 __global__ __launch_bounds__(ln_block(TPR)) void ln_fwd_kernel(const T* __restrict__ x, int64_t rows, int D, int64_t xs, const W* __restrict__ w,
                                                      const W* __restrict__ b, float eps, T* __restrict__ y, float* __restrict__ mean_out,
                                                      float* __restrict__ rstd_out)
 {
     constexpr int V = LnVec<T>::N, RPB = ln_block(TPR) / TPR;
-    __shared__ float buf[2][16];
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    __shared__ float buf[2][8];
+    const int t = threadIdx.x % TPR, slot = ln_slot<TPR>();
     const int64_t stride = (int64_t)gridDim.x * RPB;
-    LnParam<W, V> ww[NV], bb[NV];
+    LnPack<W, V> ww[NV], bb[NV];
     LnVec<T> next[NV];
     auto fetch = [&](int64_t r) {
         const T* xr = x + (r < rows ? r : 0) * xs;
@@ -144,7 +183,7 @@ __global__ __launch_bounds__(ln_block(TPR)) void ln_fwd_kernel(const T* __restri
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                v[i][e] = (float)next[i].v[e];       // (0 behind D)
+                v[i][e] = next[i].at(e);       // (0 behind D)
                 s[0] += v[i][e];
             }
         if (r0 + stride < rows) fetch(r + stride);
@@ -171,7 +210,7 @@ __global__ __launch_bounds__(ln_block(TPR)) void ln_fwd_kernel(const T* __restri
                 const int c = (i * TPR + t) * V;
                 if (c < D) {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, (float)ww[i].v[e], (float)bb[i].v[e]);
+                    for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, ww[i].at(e), bb[i].at(e));
                     ln_store(yr + c, D - c, v[i]);
                 }
             }
@@ -186,11 +225,11 @@ __global__ __launch_bounds__(ln_block(TPR)) void ln_bwd_kernel(const T* __restri
                                                      const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part)
 {
     constexpr int V = LnVec<T>::N, RPB = ln_block(TPR) / TPR;
-    __shared__ float buf[2][32];
+    __shared__ float buf[2][16];
     __shared__ float fold[TPR < 256 ? 256 * V : 1];
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const int t = threadIdx.x % TPR, slot = ln_slot<TPR>();
     const int64_t stride = (int64_t)gridDim.x * RPB;
-    LnParam<W, V> ww[NV];
+    LnPack<W, V> ww[NV];
     float aw[NV][V], ab[NV][V];
     LnVec<T> nx[NV], ng[NV];
     float nmean = 0.0f, nrstd = 0.0f;
@@ -224,20 +263,24 @@ __global__ __launch_bounds__(ln_block(TPR)) void ln_bwd_kernel(const T* __restri
         const int64_t r = r0 + slot;
         const bool live = r < rows;
         const float mean = nmean, rstd = nrstd;
-        float z[NV][V], g[NV][V];
+        // the row stays as it came (half the registers of 16-bit values converted); z and g are formed again for dx
+        LnVec<T> cx[NV], cg[NV];
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            cx[i] = nx[i];
+            cg[i] = ng[i];
+            ln_packed(ww[i]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                z[i][e] = ((float)nx[i].v[e] - mean) * rstd;
-                g[i][e] = (float)ng[i].v[e];
-                aw[i][e] += g[i][e] * z[i][e];
-                ab[i][e] += g[i][e];
-                g[i][e] *= (float)ww[i].v[e];
-                s[0] += g[i][e];
-                s[1] += g[i][e] * z[i][e];
+                const float z = (cx[i].at(e) - mean) * rstd, g = cg[i].at(e), gw = g * ww[i].at(e);
+                aw[i][e] += g * z;
+                ab[i][e] += g;
+                s[0] += gw;
+                s[1] += gw * z;
             }
+            if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);        // (one vector converted at a time)
+        }
         if (r0 + stride < rows) fetch(r + stride);
         if (!dx) continue;
         row_sum<TPR>(s, buf[flip]);
@@ -247,11 +290,19 @@ __global__ __launch_bounds__(ln_block(TPR)) void ln_bwd_kernel(const T* __restri
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * TPR + t) * V;
+                ln_packed(cx[i]);
+                ln_packed(cg[i]);
+                ln_packed(ww[i]);
                 if (c < D) {
+                    float o[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) g[i][e] = rstd * (g[i][e] - c1 - z[i][e] * c2);
-                    ln_store(dx + r * D + c, D - c, g[i]);
+                    for (int e = 0; e < V; ++e) {
+                        const float z = (cx[i].at(e) - mean) * rstd;
+                        o[e] = rstd * (cg[i].at(e) * ww[i].at(e) - c1 - z * c2);
+                    }
+                    ln_store(dx + r * D + c, D - c, o);
                 }
+                if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -325,12 +376,12 @@ __global__ __launch_bounds__(256) void ln_bwd_few_kernel(const T* __restrict__ d
             continue;
         }
         const LnVec<T> nx = ln_raw(x + r * xs + c, D - c), ng = ln_raw(dy + r * dys + c, D - c);
-        const LnParam<W, V> ww = ln_param<W, V>(w, c, D, 1.0f);
+        const LnPack<W, V> ww = ln_param<W, V>(w, c, D, 1.0f);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const bool in = c + e < D;
-            z[i][e] = in ? ((float)nx.v[e] - mean) * rstd : 0.0f;
-            g[i][e] = in ? (float)ng.v[e] * (float)ww.v[e] : 0.0f;
+            z[i][e] = in ? (nx.at(e) - mean) * rstd : 0.0f;
+            g[i][e] = in ? ng.at(e) * ww.at(e) : 0.0f;
             s[0] += g[i][e];
             s[1] += g[i][e] * z[i][e];
         }
@@ -442,8 +493,6 @@ __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* __re
     if (rg == 0 && c < D && out) out[c] = (W)(float)acc[0][cl];
 }
 
-constexpr int LN_FWD_BLOCKS = 2048;      // workgroups of the forward kernel (8 a CU)
-constexpr int LN_MAX_PARTS = 1280;       // partial rows of dw / db, workgroups of the backward kernel (5 a CU)
 constexpr int LN_WIDE_PARTS = 64;
 // up to here dw / db are summed row by row by one thread a column: no partial sums, no second launch (32 x 1024 fp32: 4 us against 4 + 3)
 constexpr int LN_FEW_ROWS = 64;
@@ -451,8 +500,10 @@ constexpr int LN_FEW_ROWS = 64;
 int esize(int dtype) { return dtype == MP_DTYPE_F32 ? 4 : 2; }
 int64_t reg_limit(int dtype) { return 256 * 8 * (16 / esize(dtype)); }
 
-// Threads a row: the smallest power of two (from 8) whose one vector each covers it, 64 with up to four; calls of few rows (latency: more
-// waves share a row) 256; wider rows 256 to 1024 with two, so that the registers leave room for several rows a CU.  [TPR, NV]
+// Threads a row and vectors a thread.  Up to 64 vectors the smallest power of two (from 8) that covers the row with one each; then the least
+// waste of threads that leaves a CU several workgroups' registers (12 000 bf16 columns forward: 512 x 3 45 us, 1024 x 2 60).  The backward
+// kernel holds two sums a column, 16 registers a vector of 16-bit values: one vector a thread while 512 threads cover the row (3000 bf16
+// columns: 512 x 1 126 us, 256 x 2 141).  Calls of few rows (latency: more waves share a row): 256 threads.
 struct LnShape { int tpr, nv; };
 LnShape ln_shape(int64_t rows, int64_t D, int V, bool backward)
 {
@@ -463,34 +514,40 @@ LnShape ln_shape(int64_t rows, int64_t D, int V, bool backward)
     if (vecs <= 64) return {64, 1};
     const bool few = rows < 1024;
     if (!few && vecs <= 128) return {64, 2};
-    if (!few && vecs <= 256) return {64, 4};
+    if (!few && vecs <= 192) return {64, 3};
     if (vecs <= 256) return {256, 1};
-    if (vecs <= 512) return {256, 2};
+    if (vecs <= 512) return backward ? LnShape{512, 1} : LnShape{256, 2};
+    if (vecs <= 768 && !backward) return {256, 3};
     if (vecs <= 1024) return {512, 2};
-    if (backward) return {512, 4};       // (1024 threads leave 128 registers each: too few for the sums)
-    return {1024, 2};
+    if (vecs <= 1536) return {512, 3};
+    return {512, 4};
 }
+
+// Workgroups that walk the rows: about as many as the CUs hold at once.  Backward, every one writes a row of partial sums: 1280 of them cost
+// 12 000 bf16 columns 220 us, 256 121.
+int ln_fwd_blocks(LnShape s) { return s.tpr <= 256 ? 1024 : 512; }
+int ln_bwd_blocks(LnShape s) { return s.tpr <= 256 ? (s.nv <= 2 ? 768 : 512) : s.nv == 1 ? 512 : 256; }
 
 int ln_parts(int64_t rows, int64_t D, int dtype)
 {
     if (D > reg_limit(dtype)) return (int)(rows < LN_WIDE_PARTS ? rows : LN_WIDE_PARTS);
     if (rows <= LN_FEW_ROWS) return 0;
     const LnShape s = ln_shape(rows, D, 16 / esize(dtype), true);
-    const int64_t blocks = (rows + ln_block(s.tpr) / s.tpr - 1) / (ln_block(s.tpr) / s.tpr);
-    return (int)(blocks < LN_MAX_PARTS ? blocks : LN_MAX_PARTS);
+    const int64_t blocks = (rows + ln_block(s.tpr) / s.tpr - 1) / (ln_block(s.tpr) / s.tpr), most = ln_bwd_blocks(s);
+    return (int)(blocks < most ? blocks : most);
 }
 
-#define LN_EACH_SHAPE(GO)                                                          \
-    if (s.tpr == 8) { GO(8, 1); }                                                  \
-    else if (s.tpr == 16) { GO(16, 1); }                                           \
-    else if (s.tpr == 32) { GO(32, 1); }                                           \
-    else if (s.tpr == 64 && s.nv == 1) { GO(64, 1); }                              \
-    else if (s.tpr == 64 && s.nv == 2) { GO(64, 2); }                              \
-    else if (s.tpr == 64) { GO(64, 4); }                                           \
-    else if (s.tpr == 256 && s.nv == 1) { GO(256, 1); }                            \
-    else if (s.tpr == 256) { GO(256, 2); }                                         \
-    else if (s.tpr == 512 && s.nv == 2) { GO(512, 2); }                            \
-    else { GO_LAST; }
+#define LN_COMMON_SHAPES(GO)                          \
+    if (s.tpr == 8) { GO(8, 1); }                     \
+    else if (s.tpr == 16) { GO(16, 1); }              \
+    else if (s.tpr == 32) { GO(32, 1); }              \
+    else if (s.tpr == 64 && s.nv == 1) { GO(64, 1); } \
+    else if (s.tpr == 64 && s.nv == 2) { GO(64, 2); } \
+    else if (s.tpr == 64) { GO(64, 3); }              \
+    else if (s.tpr == 256 && s.nv == 1) { GO(256, 1); } \
+    else if (s.tpr == 512 && s.nv == 2) { GO(512, 2); } \
+    else if (s.tpr == 512 && s.nv == 3) { GO(512, 3); } \
+    else if (s.tpr == 512 && s.nv == 4) { GO(512, 4); }
 
 template <typename T, typename W>
 int ln_fwd(const void* x, int dtype, int64_t rows, int64_t D, int64_t xs, const void* w, const void* b, double eps, void* y, float* mean, float* rstd,
@@ -503,13 +560,13 @@ int ln_fwd(const void* x, int dtype, int64_t rows, int64_t D, int64_t xs, const 
     } else {
         const LnShape s = ln_shape(rows, D, LnVec<T>::N, false);
         const int64_t blocks = (rows + ln_block(s.tpr) / s.tpr - 1) / (ln_block(s.tpr) / s.tpr);
-        const unsigned grid = (unsigned)(blocks < LN_FWD_BLOCKS ? blocks : LN_FWD_BLOCKS);
+        const unsigned grid = (unsigned)(blocks < ln_fwd_blocks(s) ? blocks : ln_fwd_blocks(s));
 #define LN_GO(TPR, NV)                                                                                                                   \
     MP_LAUNCH("ln_fwd_kernel", 8.0 * n, bytes, (ln_fwd_kernel<T, W, TPR, NV>), dim3(grid), dim3(ln_block(TPR)), 0, stream, (const T*)x, rows, (int)D, \
               xs, (const W*)w, (const W*)b, (float)eps, (T*)y, mean, rstd)
-#define GO_LAST LN_GO(1024, 2)
-        LN_EACH_SHAPE(LN_GO)
-#undef GO_LAST
+        LN_COMMON_SHAPES(LN_GO)
+        else if (s.nv == 2) { LN_GO(256, 2); }
+        else { LN_GO(256, 3); }
 #undef LN_GO
     }
     MP_CHECK_LAUNCH();
@@ -548,9 +605,8 @@ int ln_bwd(const void* dy, int64_t dys, const void* x, int64_t xs, int dtype, in
 #define LN_GO(TPR, NV)                                                                                                                     \
     MP_LAUNCH("ln_bwd_kernel", 16.0 * n, bytes, (ln_bwd_kernel<T, W, TPR, NV>), dim3((unsigned)parts), dim3(ln_block(TPR)), 0, stream, (const T*)dy, dys, \
               (const T*)x, xs, rows, (int)D, (const W*)w, mean, rstd, (T*)dx, pg ? part : nullptr)
-#define GO_LAST LN_GO(512, 4)
-        LN_EACH_SHAPE(LN_GO)
-#undef GO_LAST
+        LN_COMMON_SHAPES(LN_GO)
+        else { LN_GO(512, 1); }
 #undef LN_GO
         MP_CHECK_LAUNCH();
     }
