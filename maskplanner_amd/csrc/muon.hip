@@ -1023,9 +1023,8 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
 //         result against 1.4e-6 step by step);
 //   bf16: 2^-22 g^(h-1) <= 5e-3, five steps (worst case measured 6e-4, a matrix dominated by one direction; the result's rounding: 1.7e-3);
 //   fp16: 2^-22 g^(h-1) <= 5e-5, three steps (the rounding: 2e-4).
-// Of one limit for the whole chunk the cheapest is taken: work at 0.8 PFLOP/s of plane products, and 6.5 us a launch -- hops of different
-// lengths take turns, which costs a list of small matrices more than it saves (the encoder's nine in fp32: 17 launches of one step each, 23
-// of mixed lengths).
+// Of one limit for the whole chunk the cheapest is taken: work at 0.8 PFLOP/s of plane products, and 6.5 us for each launch of the matrix that
+// has most of them.
 int hop_cap(const Shape& s, int steps, int dtype, double g)
 {
     const double most = dtype == MP_DTYPE_F32 ? (s.n >= 2 * s.m ? 16.0 : 1.0) : dtype == MP_DTYPE_F16 ? 200.0 : 20000.0;
@@ -1041,8 +1040,9 @@ void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, double g
         int use[MAX_MAT];
         bool more = h == 1;
         double work = 0.0;
-        int launches = 2;
+        int launches = 0;
         for (int q = 0; q < k; ++q) {
+            int mine = 2;
             const int cap = hop_cap(s[q], steps, dtype, g);
             use[q] = h < cap ? h : cap;
             more = more || use[q] == h;
@@ -1051,18 +1051,11 @@ void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, double g
                 const int len = left < use[q] ? left : use[q];
                 // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
                 work += 2.0 * m * m * ((left == steps && planes == 1 ? 1.0 + 2.0 * 2.0 : 3.0 * 3.0) * n + 3.0 * (4.0 * len - 3.0) * m);
+                mine += len == 1 ? 3 : 3 * len + 1;       // Gram, apply; Q a step; T (and R), A between steps; R behind the last
             }
+            launches = mine > launches ? mine : launches;
         }
         if (!more) break;        // (no matrix may take that many)
-        for (int round = 0;; ++round) {
-            int len = 0;
-            for (int q = 0; q < k; ++q) {
-                const int left = steps - round * use[q], l = left < use[q] ? left : use[q];
-                len = l > len ? l : len;
-            }
-            if (len <= 0) break;
-            launches += len == 1 ? 3 : 3 * len + 1;       // Gram, apply; Q a step; T (and R), A between steps; R behind the last
-        }
         const double cost = work / 0.8e15 + launches * 6.5e-6;
         if (cost < best * 0.999) {
             best = cost;
@@ -1169,14 +1162,14 @@ Plan plan_of(const Prob* p, int count, int products)
 }
 
 template <int WM, int WN, int PL, int PR, int NS, bool KW>
-int launch_ring(const Probs& a, const char* tag, double flops, hipStream_t stream)
+int launch_ring(const Probs& a, double flops, hipStream_t stream)
 {
     static mp::DynLds dyn;
     constexpr int TM = KW ? 32 * WM : 64 * WM, TN = KW ? 32 * WN : 64 * WN, RINGS = KW ? 4 : 1;
     constexpr size_t ring = (size_t)RINGS * NS * 64 * (TM * PL + TN * PR), tile = (size_t)RINGS * TM * (TN + TPAD) * sizeof(float);
     constexpr size_t smem = ring > tile ? ring : tile;
     if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), smem)) return MP_ELAUNCH;
-    MP_LAUNCH(tag, flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
+    MP_LAUNCH("ns_gemm_kernel", flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
     MP_CHECK_LAUNCH();
     if (a.whole < a.tiles) {
         MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<TM, TN>), dim3((unsigned)(a.tiles - a.whole) * (TM / 32)), dim3(256), 0, stream, a);
@@ -1188,16 +1181,16 @@ int launch_ring(const Probs& a, const char* tag, double flops, hipStream_t strea
 // Depth of the ring: what 144 KB hold (at most 8 chunks) where the launch has one workgroup a CU at most, else half of that so that two
 // share a CU (256 x 128 and the K-sharing 64 x 64: always one).
 template <int WM, int WN, int PL, int PR, bool KW>
-int launch_as(const Probs& a, const char* tag, double flops, hipStream_t stream)
+int launch_as(const Probs& a, double flops, hipStream_t stream)
 {
     constexpr int lds = 147456, stage = KW ? 4 * 64 * 32 * (WM * PL + WN * PR) : 64 * 64 * (WM * PL + WN * PR);
     constexpr int deep = lds / stage < 8 ? lds / stage : 8, half = KW || WM * WN >= 8 ? deep : (lds / 2 / stage < 8 ? lds / 2 / stage : 8);
-    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW>(a, tag, flops, stream);
-    return launch_ring<WM, WN, PL, PR, half, KW>(a, tag, flops, stream);
+    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW>(a, flops, stream);
+    return launch_ring<WM, WN, PL, PR, half, KW>(a, flops, stream);
 }
 
 // planes of the left and the right operands: (2, 2), (2, 1) or (1, 1)
-int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
+int launch(Probs& a, int left, int right, hipStream_t stream)
 {
     if (a.count == 0) return MP_OK;
     const int products = left + right - 1;
@@ -1228,10 +1221,10 @@ int launch(Probs& a, int left, int right, const char* tag, hipStream_t stream)
     else if (a.equal) items = a.whole + (int64_t)a.rest * ((a.p[0].kc + a.p[0].seg - 1) / a.p[0].seg);
     a.items = (int)items;
 #define NS_SHAPES(PL, PR)                                                                  \
-    return pl.shape == 0   ? launch_as<4, 2, PL, PR, false>(a, tag, flops, stream)         \
-           : pl.shape == 1 ? launch_as<2, 2, PL, PR, false>(a, tag, flops, stream)         \
-           : pl.shape == 2 ? launch_as<2, 2, PL, PR, true>(a, tag, flops, stream)          \
-                           : launch_as<1, 1, PL, PR, true>(a, tag, flops, stream)
+    return pl.shape == 0   ? launch_as<4, 2, PL, PR, false>(a, flops, stream)         \
+           : pl.shape == 1 ? launch_as<2, 2, PL, PR, false>(a, flops, stream)         \
+           : pl.shape == 2 ? launch_as<2, 2, PL, PR, true>(a, flops, stream)          \
+                           : launch_as<1, 1, PL, PR, true>(a, flops, stream)
     if (left == 2 && right == 2) NS_SHAPES(2, 2);
     if (left == 2) NS_SHAPES(2, 1);
     NS_SHAPES(1, 1);
@@ -1411,103 +1404,97 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
         p.so = so;
         return p;
     };
-    int done[MAX_MAT], rbuf[MAX_MAT], qbuf[MAX_MAT];       // steps finished, which P holds R / Q
-    bool first[MAX_MAT];
-    for (int q = 0; q < k; ++q) { done[q] = 0; first[q] = true; rbuf[q] = qbuf[q] = 0; }
-    int left = k;
-    while (left > 0) {        // every matrix is at the start of a hop (or finished); hops of one chunk may differ in length
-        int len[MAX_MAT], longest = 0;
-        float sR[MAX_MAT];
-        g.count = 0;
-        for (int q = 0; q < k; ++q) {       // A = X X^T
-            len[q] = done[q] < steps ? (steps - done[q] < hop[q] ? steps - done[q] : hop[q]) : 0;
-            longest = len[q] > longest ? len[q] : longest;
-            if (!len[q]) continue;
-            Prob p = sym_prob(q, bf[q].X, bf[q].X, first[q] ? 1.0f : sX, first[q] ? 1.0f : sX, bf[q].A, sA);
-            p.kc = chunks(sh[q].n);
-            if (first[q]) { p.rdev = bf[q].r; p.rpow = 2; }
-            g.p[g.count++] = p;
-        }
-        const int xp = left == k && done[0] == 0 ? a.planes : 2;       // planes of X in this round of hops
-        int rc = launch(g, xp, xp, "ns_gemm_kernel (gram)", stream);
-        if (rc) return rc;
-        for (int s = 0; s < longest; ++s) {
+    // Every matrix walks through its hops by itself; a launch takes the present stage of each, whatever it is, so that hops of different lengths
+    // fill each other's launches (seven matrices up to 11988 x 1024, hops of two steps and of one: 23 products' launches in turns, 17 this way).
+    enum Stage { GRAM, SQUARE, STEP, NEXT, APPLY, END };
+    struct Walk {
+        Stage at;
+        int done, len, s, r, q;      // steps behind it, steps of this hop, step inside it, which P holds R / Q
+        float sR;
+        bool first;                  // X is still the input's planes (to be multiplied by r)
+    } w[MAX_MAT];
+    for (int q = 0; q < k; ++q) w[q] = Walk{GRAM, 0, steps < hop[q] ? steps : hop[q], 0, 0, 0, sQ, true};
+    for (;;) {
+        bool more = false;
+        for (int kind = 0; kind < 3; ++kind) {        // operands of two planes, Gram products and X <- R X of one-plane matrices
             g.count = 0;
-            for (int q = 0; q < k; ++q) {      // Q = a I + b A + c A^2
-                if (s >= len[q]) continue;
-                qbuf[q] = s == 0 ? 0 : (rbuf[q] + 1) % 3;
-                Prob p = sym_prob(q, bf[q].A, bf[q].A, sA, sA, bf[q].P[qbuf[q]], sQ);
-                p.alpha *= (float)coef[2];
-                p.C = reinterpret_cast<const _Float16*>(bf[q].A);
-                p.cb = (float)(coef[1] / sA);
-                p.ca = (float)coef[0];
-                g.p[g.count++] = p;
-            }
-            rc = launch(g, 2, 2, "ns_gemm_kernel (square)", stream);
-            if (rc) return rc;
-            g.count = 0;
-            for (int q = 0; q < k; ++q) {      // T = A Q (another step follows), R = Q R: independent, one launch
-                if (s >= len[q]) continue;
-                if (s + 1 < len[q]) g.p[g.count++] = sym_prob(q, bf[q].A, bf[q].P[qbuf[q]], sA, sQ, bf[q].T, sT);
-                if (s == 0) {
-                    rbuf[q] = qbuf[q];
-                    sR[q] = sQ;
-                } else {
-                    const int to = 3 - rbuf[q] - qbuf[q];
-                    const float so = pow2_scale(bd.r[s + 1]);
-                    g.p[g.count++] = sym_prob(q, bf[q].P[qbuf[q]], bf[q].P[rbuf[q]], sQ, sR[q], bf[q].P[to], so);
-                    rbuf[q] = to;
-                    sR[q] = so;
+            for (int q = 0; q < k; ++q) {
+                Walk& v = w[q];
+                const bool one = v.first && a.planes == 1;
+                if (v.at == END || kind != (one && v.at == GRAM ? 1 : one && v.at == APPLY ? 2 : 0)) continue;
+                more = true;
+                if (v.at == GRAM) {                   // A = X X^T
+                    Prob p = sym_prob(q, bf[q].X, bf[q].X, v.first ? 1.0f : sX, v.first ? 1.0f : sX, bf[q].A, sA);
+                    p.kc = chunks(sh[q].n);
+                    if (v.first) { p.rdev = bf[q].r; p.rpow = 2; }
+                    g.p[g.count++] = p;
+                } else if (v.at == SQUARE) {          // Q = a I + b A + c A^2
+                    v.q = v.s == 0 ? 0 : (v.r + 1) % 3;
+                    Prob p = sym_prob(q, bf[q].A, bf[q].A, sA, sA, bf[q].P[v.q], sQ);
+                    p.alpha *= (float)coef[2];
+                    p.C = reinterpret_cast<const _Float16*>(bf[q].A);
+                    p.cb = (float)(coef[1] / sA);
+                    p.ca = (float)coef[0];
+                    g.p[g.count++] = p;
+                    if (v.s == 0) { v.r = v.q; v.sR = sQ; }
+                } else if (v.at == STEP) {            // T = A Q (another step follows), R = Q R: independent
+                    if (v.s + 1 < v.len) g.p[g.count++] = sym_prob(q, bf[q].A, bf[q].P[v.q], sA, sQ, bf[q].T, sT);
+                    if (v.s > 0) {
+                        const int to = 3 - v.r - v.q;
+                        const float so = pow2_scale(bd.r[v.s + 1]);
+                        g.p[g.count++] = sym_prob(q, bf[q].P[v.q], bf[q].P[v.r], sQ, v.sR, bf[q].P[to], so);
+                        v.r = to;
+                        v.sR = so;
+                    }
+                } else if (v.at == NEXT) {            // A = T Q
+                    g.p[g.count++] = sym_prob(q, bf[q].T, bf[q].P[v.q], sT, sQ, bf[q].A, sA);
+                } else {                              // X <- R X
+                    Prob p{};
+                    p.L = reinterpret_cast<const _Float16*>(bf[q].P[v.r]);
+                    p.R = reinterpret_cast<const _Float16*>(bf[q].XT);
+                    p.M = (int)sh[q].m;
+                    p.N = (int)sh[q].n;
+                    p.kc = chunks(sh[q].m);
+                    p.alpha = 1.0f / (v.sR * (v.first ? 1.0f : sX));
+                    if (v.first) { p.rdev = bf[q].r; p.rpow = 1; }
+                    if (v.done + v.len == steps) {
+                        p.fin = out[idx[q]];
+                        p.fin_t = sh[q].rows > sh[q].cols;
+                        if (up_.on) {
+                            p.fmul = (float)(up_.lr * update_scale(up_, sh[q].rows, sh[q].cols));
+                            p.fdecay = (float)(1.0 - up_.lr * up_.decay);
+                        }
+                    } else {
+                        p.out = reinterpret_cast<_Float16*>(bf[q].X);
+                        p.outT = reinterpret_cast<_Float16*>(bf[q].XT2);
+                        p.oc = chunks(sh[q].n);
+                        p.otc = chunks(sh[q].m);
+                        p.so = sX;
+                        char* t = bf[q].XT;
+                        bf[q].XT = bf[q].XT2;
+                        bf[q].XT2 = t;
+                    }
+                    g.p[g.count++] = p;
                 }
             }
-            rc = launch(g, 2, 2, "ns_gemm_kernel (step)", stream);
-            if (rc) return rc;
-            g.count = 0;
-            for (int q = 0; q < k; ++q)        // A = T Q
-                if (s + 1 < len[q]) g.p[g.count++] = sym_prob(q, bf[q].T, bf[q].P[qbuf[q]], sT, sQ, bf[q].A, sA);
-            rc = launch(g, 2, 2, "ns_gemm_kernel (step)", stream);
+            const int rc = kind == 0 ? launch(g, 2, 2, stream) : kind == 1 ? launch(g, 1, 1, stream) : launch(g, 2, 1, stream);
             if (rc) return rc;
         }
-        g.count = 0;
-        for (int q = 0; q < k; ++q) {          // X <- R X
-            if (!len[q]) continue;
-            done[q] += len[q];
-            const bool last = done[q] == steps, tall = sh[q].rows > sh[q].cols;
-            Prob p{};
-            const _Float16* R = reinterpret_cast<const _Float16*>(bf[q].P[rbuf[q]]);
-            const _Float16* XT = reinterpret_cast<const _Float16*>(bf[q].XT);
-            p.L = R;
-            p.R = XT;
-            p.M = (int)sh[q].m;
-            p.N = (int)sh[q].n;
-            p.kc = chunks(sh[q].m);
-            p.alpha = 1.0f / (sR[q] * (first[q] ? 1.0f : sX));
-            if (first[q]) { p.rdev = bf[q].r; p.rpow = 1; }
-            if (last) {
-                p.fin = out[idx[q]];
-                p.fin_t = tall;
-                if (up_.on) {
-                    p.fmul = (float)(up_.lr * update_scale(up_, sh[q].rows, sh[q].cols));
-                    p.fdecay = (float)(1.0 - up_.lr * up_.decay);
-                }
-                --left;
-            } else {
-                p.out = reinterpret_cast<_Float16*>(bf[q].X);
-                p.outT = reinterpret_cast<_Float16*>(bf[q].XT2);
-                p.oc = chunks(sh[q].n);
-                p.otc = chunks(sh[q].m);
-                p.so = sX;
-                char* t = bf[q].XT;
-                bf[q].XT = bf[q].XT2;
-                bf[q].XT2 = t;
+        if (!more) return MP_OK;
+        for (int q = 0; q < k; ++q) {
+            Walk& v = w[q];
+            if (v.at == GRAM || v.at == STEP) v.at = v.at == GRAM ? SQUARE : v.s + 1 < v.len ? NEXT : APPLY;
+            else if (v.at == SQUARE) v.at = v.len == 1 ? APPLY : STEP;
+            else if (v.at == NEXT) { ++v.s; v.at = SQUARE; }
+            else if (v.at == APPLY) {
+                v.done += v.len;
+                v.len = steps - v.done < hop[q] ? steps - v.done : hop[q];
+                v.s = 0;
+                v.first = false;
+                v.at = v.len ? GRAM : END;
             }
-            first[q] = false;
-            g.p[g.count++] = p;
         }
-        rc = launch(g, 2, xp, "ns_gemm_kernel (apply)", stream);
-        if (rc) return rc;
     }
-    return MP_OK;
 }
 
 int run_all(int64_t count, const void* const* in, void* const* out, float* const* mom, const int64_t* rows, const int64_t* cols, int dtype, int steps,
