@@ -403,7 +403,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
         w = base + x * per + (x < rest ? x : rest) + y;
     }
     {
-        const int i = w < a.whole ? which(a.tile0, w) : a.equal ? which(a.tile0, a.whole + (w - a.whole) % a.rest) : which(a.item0, w);
+        const int i = a.count == 1 ? 0 : w < a.whole ? which(a.tile0, w) : a.equal ? which(a.tile0, a.whole + (w - a.whole) % a.rest) : which(a.item0, w);
         const Prob p = a.p[i];
         int tile = w - a.tile0[i], c0 = 0;        // chunks [c0, c0 + n) of the tile
         if (w >= a.whole) {
