@@ -12,6 +12,9 @@
 // ARITHMETIC.  fp32 accuracy from the fp16 matrix cores: an operand is kept as two fp16 planes, x 2^k = h + l (h = fp16(x 2^k), l the rest:
 // 22 to 24 bits), a product is h h + h l + l h accumulated in fp32 -- three products at the fp16 rate (2.5 PFLOP/s) against one at the
 // fp32 rate (0.16).  The power of two puts the largest entry below 2^15, so l keeps its bits down to entries of 2^-24 of that.
+// What the small singular values suffer from is an error of Q that is not one of A (they grow by up to a^5 = 485 meanwhile): b A and c A^2 are
+// formed of the same planes, and in fp32 up to m = 128, where sums of so few terms hide nothing, A^2 takes l l too (400 shapes up to 300 x 1000
+// in emulation, largest error: 2.8e-6 of the exact result with b A from the accumulators, 2.1e-6 from the planes, 1.3e-6 with l l).
 //
 // All matrices of a call (up to 12 at a time) go through each stage in ONE launch (problem list in the kernel arguments): five steps are 17 to
 // 19 launches whatever their number.  Operand image: row r = chunks of 32 k, each [h: 32 fp16][l: 32 fp16] (128 bytes); columns up to the
@@ -42,6 +45,7 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     int M, N, kc, oc, otc, rpow, sym, tiles_n, fin_t;
     float alpha, cb, ca, so, fmul, fdecay;
     int tiles, seg;          // tiles of the result; chunks of a segment of K (kc: not cut)
+    int ll;                  // the product of the l planes too (LL)
 };
 // A launch's work items, one a workgroup: the first `whole` tiles uncut, then the rest in segments of K.  Items are ordered by segment, then by
 // tile: neighbours share operand rows, not just the tile.  equal: all problems have one K, the rest is `rest` tiles x segments; else every
@@ -376,7 +380,7 @@ template <int PL> __device__ __forceinline__ int swz(int row) { return PL == 2 ?
 // KW: the four waves share a (32 WM) x (32 WN) tile by K instead, wave v taking chunks v, v + 4, ..: each with a ring of its own and no
 // meeting at all; their sums meet in LDS at the end, added in the order of the waves.  For 64 x 64 tiles, where a wave of the shared form has
 // three products between two meetings (136 tiles of K = 1024: 15.2 us shared, 12.7 this way).
-template <int WM, int WN, int PL, int PR, int NS, bool KW>
+template <int WM, int WN, int PL, int PR, int NS, bool KW, bool LL>
 __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 {
     constexpr int WAVES = KW ? 1 : 4;                              // waves that load a stage together
@@ -465,6 +469,11 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
         // The PRODS matrix instructions of 16 k, the small products first, a block's WM * WN apart; in the shadow of each (32 cycles) go its
         // share of the reads of the other half's fragments and of the loads of a chunk to come: with one wave a SIMD nothing else fills it.
         auto multiply = [&](int ks, bool reads, int rbuf, bool fetches, int fbuf) {
+            if constexpr (LL)        // (a question of its own kernel: asked in all of them it costs 1 % of a small launch)
+                if (p.ll)
+#pragma unroll
+                    for (int g = 0; g < WM * WN; ++g)
+                        acc[g / WN][g % WN] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][g / WN][1], fq[ks][g % WN][1], acc[g / WN][g % WN], 0, 0, 0);
 #pragma unroll
             for (int g = 0; g < PRODS; ++g) {
                 const int k = g / (WM * WN), x = g / WN % WM, y = g % WN;
@@ -843,7 +852,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
                 }
         }
         __syncthreads();
-        auto product = [&](char* img, int nch, int i, int j) {        // rows 32 i .. of the image times rows 32 j ..
+        auto product = [&](char* img, int nch, int i, int j, bool full) {        // rows 32 i .. of the image times rows 32 j ..
             float16v acc;
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
@@ -853,13 +862,14 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
                 for (int ks = 0; ks < 2; ++ks) {
                     const half8 lh = *reinterpret_cast<const half8*>(unit(img, ri, nch, c, ks * 2 + fh)), ll = *reinterpret_cast<const half8*>(unit(img, ri, nch, c, 4 + ks * 2 + fh));
                     const half8 rh = *reinterpret_cast<const half8*>(unit(img, rj, nch, c, ks * 2 + fh)), rl = *reinterpret_cast<const half8*>(unit(img, rj, nch, c, 4 + ks * 2 + fh));
+                    if (full) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rl, acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh, acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl, acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, acc, 0, 0, 0);
                 }
             return acc;
         };
-        auto keep = [&](const float16v& v, float scale, int i, int j) {      // block (i, j) of a symmetric matrix as block (j, i): runs of four
+        auto keep = [&](float16v& v, float scale, int i, int j) {      // block (i, j) of a symmetric matrix as block (j, i), runs of four; v: what the planes hold
 #pragma unroll
             for (int rg = 0; rg < 4; ++rg) {
                 half4 h, l;
@@ -868,6 +878,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
                     const float x = v[rg * 4 + e] * scale;
                     h[e] = (_Float16)x;
                     l[e] = (_Float16)(x - (float)h[e]);
+                    v[rg * 4 + e] = (float)h[e] + (float)l[e];
                 }
                 *reinterpret_cast<half4*>(unit(S, 32 * j + fr, MB, i, rg) + fh * 8) = h;
                 *reinterpret_cast<half4*>(unit(S, 32 * j + fr, MB, i, 4 + rg) + fh * 8) = l;
@@ -878,19 +889,19 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
         const int i0 = wave / MB, j0 = wave % MB;
         const bool mine = wave < MB * MB;
         if (mine) {
-            A = product(X, npc, i0, j0);
+            A = product(X, npc, i0, j0, false);
 #pragma unroll
             for (int k = 0; k < 16; ++k) A[k] *= sx * sx;
             keep(A, a.sA, i0, j0);
         }
         __syncthreads();
         if (mine) {
-            const float16v sq = product(S, MB, i0, j0);
-            const float cc = a.c / (a.sA * a.sA);
+            const float16v sq = product(S, MB, i0, j0, DT == MP_DTYPE_F32);
+            const float cc = a.c / (a.sA * a.sA), bb = a.b / a.sA;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
                 const int row = 32 * i0 + (k & 3) + 8 * (k >> 2) + 4 * fh;
-                A[k] = cc * sq[k] + a.b * A[k] + (row == 32 * j0 + fr && row < M ? a.a : 0.0f);
+                A[k] = cc * sq[k] + bb * A[k] + (row == 32 * j0 + fr && row < M ? a.a : 0.0f);
             }
         }
         __syncthreads();
@@ -1019,15 +1030,17 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
 
 // Steps a hop of every matrix of a chunk.  Allowed, with g = max |Q|^2 (a^2 = 11.9 for the usual coefficients) the growth of the smallest
 // eigenvalues' relative error a further step:
-//   fp32: two from n = 2 m on (it saves a fifth there; nearer to square less than 15 %, and the error doubles: 128 x 131: 2.6e-6 of the exact
-//         result against 1.4e-6 step by step);
+//   fp32: two from n = 2 m and m = 256 on (it saves a fifth there; nearer to square less than 15 %, in small matrices nothing, and the error
+//         grows: 128 x 131: 2.6e-6 of the exact result against 1.4e-6 step by step, 70 x 600: 2.5e-6 against 1.6e-6);
 //   bf16: 2^-22 g^(h-1) <= 5e-3, five steps (worst case measured 6e-4, a matrix dominated by one direction; the result's rounding: 1.7e-3);
 //   fp16: 2^-22 g^(h-1) <= 5e-5, three steps (the rounding: 2e-4).
 // Of one limit for the whole chunk the cheapest is taken: work at 0.8 PFLOP/s of plane products, and 6.5 us for each launch of the matrix that
 // has most of them.
+bool hops_in_f32(const Shape& s) { return s.m >= 256 && s.n >= 2 * s.m; }
+
 int hop_cap(const Shape& s, int steps, int dtype, double g)
 {
-    const double most = dtype == MP_DTYPE_F32 ? (s.n >= 2 * s.m ? 16.0 : 1.0) : dtype == MP_DTYPE_F16 ? 200.0 : 20000.0;
+    const double most = dtype == MP_DTYPE_F32 ? (hops_in_f32(s) ? 16.0 : 1.0) : dtype == MP_DTYPE_F16 ? 200.0 : 20000.0;
     int h = 1;
     for (double e = g > 1.5 ? g : 1.5; h < steps && e <= most && (dtype != MP_DTYPE_F32 || h < 2); e *= g > 1.5 ? g : 1.5) ++h;
     return h;
@@ -1078,7 +1091,7 @@ int norm_blocks(const Shape& s)
 // (what any schedule may use: the size does not depend on the coefficients)
 size_t layout(const Shape& s, int steps, int dtype, char* base, Buffers* b)
 {
-    const bool chain = steps > 1 && (dtype != MP_DTYPE_F32 || s.n >= 2 * s.m);
+    const bool chain = steps > 1 && (dtype != MP_DTYPE_F32 || hops_in_f32(s));
     size_t at = 0;
     auto take = [&](size_t n) {
         char* p = base ? base + at : nullptr;
@@ -1161,15 +1174,15 @@ Plan plan_of(const Prob* p, int count, int products)
     return best;
 }
 
-template <int WM, int WN, int PL, int PR, int NS, bool KW>
+template <int WM, int WN, int PL, int PR, int NS, bool KW, bool LL>
 int launch_ring(const Probs& a, double flops, hipStream_t stream)
 {
     static mp::DynLds dyn;
     constexpr int TM = KW ? 32 * WM : 64 * WM, TN = KW ? 32 * WN : 64 * WN, RINGS = KW ? 4 : 1;
     constexpr size_t ring = (size_t)RINGS * NS * 64 * (TM * PL + TN * PR), tile = (size_t)RINGS * TM * (TN + TPAD) * sizeof(float);
     constexpr size_t smem = ring > tile ? ring : tile;
-    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), smem)) return MP_ELAUNCH;
-    MP_LAUNCH("ns_gemm_kernel", flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
+    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW, LL>), smem)) return MP_ELAUNCH;
+    MP_LAUNCH("ns_gemm_kernel", flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW, LL>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
     MP_CHECK_LAUNCH();
     if (a.whole < a.tiles) {
         MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<TM, TN>), dim3((unsigned)(a.tiles - a.whole) * (TM / 32)), dim3(256), 0, stream, a);
@@ -1185,8 +1198,13 @@ int launch_as(const Probs& a, double flops, hipStream_t stream)
 {
     constexpr int lds = 147456, stage = KW ? 4 * 64 * 32 * (WM * PL + WN * PR) : 64 * 64 * (WM * PL + WN * PR);
     constexpr int deep = lds / stage < 8 ? lds / stage : 8, half = KW || WM * WN >= 8 ? deep : (lds / 2 / stage < 8 ? lds / 2 / stage : 8);
-    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW>(a, flops, stream);
-    return launch_ring<WM, WN, PL, PR, half, KW>(a, flops, stream);
+    if constexpr (KW && PL == 2 && PR == 2) {
+        bool ll = false;
+        for (int i = 0; i < a.count; ++i) ll = ll || a.p[i].ll;
+        if (ll) return launch_ring<WM, WN, PL, PR, deep, KW, true>(a, flops, stream);
+    }
+    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW, false>(a, flops, stream);
+    return launch_ring<WM, WN, PL, PR, half, KW, false>(a, flops, stream);
 }
 
 // planes of the left and the right operands: (2, 2), (2, 1) or (1, 1)
@@ -1435,6 +1453,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                     p.C = reinterpret_cast<const _Float16*>(bf[q].A);
                     p.cb = (float)(coef[1] / sA);
                     p.ca = (float)coef[0];
+                    p.ll = dtype == MP_DTYPE_F32 && sh[q].m < 128;
                     g.p[g.count++] = p;
                     if (v.s == 0) { v.r = v.q; v.sR = sQ; }
                 } else if (v.at == STEP) {            // T = A Q (another step follows), R = Q R: independent
