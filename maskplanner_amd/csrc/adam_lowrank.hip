@@ -179,8 +179,8 @@ __global__ __launch_bounds__(256) void linear_dx_skinny_kernel(const float* __re
     }
     __syncthreads();
     if (i >= I) return;
-    // two-wide accumulators: the inner product is VALU-bound with scalar FMAs (128 per weight row per thread), and
-    // v_pk_fma_f32 retires two per lane per pass
+    // two accumulators side by side (the inner product is VALU-bound: 128 FMAs per weight row per thread; the library is compiled
+    // without packed fp32 instructions)
     typedef float f2 __attribute__((ext_vector_type(2)));
     f2 acc[SK_B][2];
 #pragma unroll

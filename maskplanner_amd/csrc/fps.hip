@@ -71,9 +71,8 @@ __global__ __launch_bounds__(T) void fps_kernel(const float* __restrict__ xyz, i
     if (tid < 4) slots[tid] = 0ull;
     __syncthreads();
 
-    // Points are held two to a register pair so that the distance runs on packed fp32 (v_pk_add_f32 / v_pk_mul_f32: two
-    // IEEE operations per lane and issue slot -- the step is VALU-bound, ~10 instructions per point before packing);
-    // every operation is still separately rounded, so the result is bit-identical to the scalar form.
+    // Points are held two to a register pair; the library is compiled without packed fp32 instructions, so a pair's operations are two
+    // scalar ones (the step is VALU-bound, ~10 instructions per point).  Every operation is rounded by itself.
     typedef float f2 __attribute__((ext_vector_type(2)));
     constexpr int PP2 = (PPT + 1) / 2;
     f2 px[PP2], py[PP2], pz[PP2], dist[PP2];

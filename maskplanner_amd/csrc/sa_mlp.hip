@@ -213,7 +213,7 @@ __global__ __launch_bounds__(CO > 128 ? 512 : 256) void fwd_chunk_kernel(PosOper
     //  * raw Z goes out through buffer stores: the row part that is uniform over the wave sits in the scalar offset, the lane
     //    part in one VGPR advanced once per chunk, and rows past the workgroup's last position are dropped by the hardware's
     //    range check -- no 64-bit address arithmetic, no EXEC masking per row;
-    //  * the BatchNorm sums run on register pairs (v_pk_add_f32 / v_pk_mul_f32); rows past P are exact zeros and need no mask;
+    //  * the BatchNorm sums are held as register pairs; rows past P are exact zeros and need no mask;
     //  * the pool tracks one extremum per column (sign of gamma), as a maximum of the sign-flipped value.
     typedef float f2 __attribute__((ext_vector_type(2)));
     // ONE: Z is STORED as bf16 (2 bytes per element): adjacent lanes hold adjacent columns, so a lane pair exchanges one value per row
