@@ -5,7 +5,7 @@
 // MATHEMATICS.  With Q = a I + b A + c A^2 (symmetric, a polynomial of A) the next step's Gram matrix is A' = Q A Q: it need not be formed
 // from X again.  So a HOP of h steps runs on the small side only (m <= n):
 //     A = X X^T;   Q_i = a I + b A_i + c A_i^2,   A_{i+1} = (A_i Q_i) Q_i,   R_i = Q_i R_{i-1};   X <- R_h X
-// at 3 m^2 n + (4 h - 3) m^3 multiply-adds (symmetric products: the lower half only, mirrored) instead of h (3 m^2 n + m^3).  An extra step in
+// at 3 m^2 n + (4 h - 3) m^3 operations (symmetric products: the lower half only, mirrored) instead of h (3 m^2 n + m^3).  An extra step in
 // a hop multiplies the relative error of the smallest eigenvalues by a^2 ~ 12 (they grow by that, the rounding error of A does not shrink):
 // hop_cap() says how many a type allows, plan_hops() takes the cheapest schedule.
 //
@@ -37,7 +37,7 @@ constexpr int MAX_NORM_BLOCKS = 2048;   // partial sums of squares per matrix
 struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T over kc chunks of 32
     const _Float16* L;
     const _Float16* R;
-    const _Float16* C;       // planes [M][oc] or NULL
+    const _Float16* C;       // planes [M][oc] or NULL (symmetric)
     _Float16* out;           // planes [M][oc] or NULL
     _Float16* outT;          // planes [N][otc] or NULL
     void* fin;               // [M, N] of the result type, or [N, M] (fin_t), or NULL
@@ -45,7 +45,8 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     int M, N, kc, oc, otc, rpow, sym, tiles_n, fin_t;
     float alpha, cb, ca, so, fmul, fdecay;
     int tiles, seg;          // tiles of the result; chunks of a segment of K (kc: not cut)
-    int ll;                  // the product of the l planes too (LL)
+    int ll : 8;              // the product of the l planes too (LL)  (bits: of bytes the scalar loads of the arguments know nothing)
+    int opl : 8, cpl : 8;    // planes of out / outT, of C
 };
 // A launch's work items, one a workgroup: the first `whole` tiles uncut, then the rest in segments of K.  Items are ordered by segment, then by
 // tile: neighbours share operand rows, not just the tile.  equal: all problems have one K, the rest is `rest` tiles x segments; else every
@@ -207,9 +208,10 @@ __device__ __forceinline__ unsigned planes_of(float x)
     __builtin_memcpy(&lb, &l, 2);
     return (unsigned)hb | ((unsigned)lb << 16);
 }
-// eight packed elements to the h and l runs of an image (16 bytes each)
-__device__ __forceinline__ void put_packed(_Float16* o, const unsigned (&w)[8])
+// eight packed elements to the h and l runs of an image (16 bytes each), or to the h run alone
+__device__ __forceinline__ void put_packed(_Float16* img, int row, int nchunk, int col, int planes, const unsigned (&w)[8])
 {
+    _Float16* o = img + ((size_t)row * nchunk + (col >> 5)) * (32 * planes) + (col & 31);
     uint4v h, l;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -217,7 +219,7 @@ __device__ __forceinline__ void put_packed(_Float16* o, const unsigned (&w)[8])
         l[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302);
     }
     *reinterpret_cast<uint4v*>(o) = h;
-    *reinterpret_cast<uint4v*>(o + 32) = l;
+    if (planes == 2) *reinterpret_cast<uint4v*>(o + 32) = l;
 }
 constexpr int TPAD = 4;      // a tile's rows in LDS are TN + 4 floats apart: 16-byte pieces, columns spread over the banks
 
@@ -247,8 +249,8 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= alpha;
         if (p.C && row < p.M && col < padN) {
-            const half8* c = reinterpret_cast<const half8*>(p.C + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31));
-            const half8 h = c[0], l = c[4];
+            const half8* c = reinterpret_cast<const half8*>(p.C + ((size_t)row * p.oc + (col >> 5)) * (32 * p.cpl) + (col & 31));
+            const half8 h = c[0], l = p.cpl == 2 ? c[4] : half8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += cb * ((float)h[e] + (float)l[e]);
         }
@@ -275,7 +277,7 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
         wt[0] = uint4v{w[0], w[1], w[2], w[3]};
         wt[1] = uint4v{w[4], w[5], w[6], w[7]};
         // a symmetric result takes its lower half in pieces of 8 x 8: those below the diagonal here and, mirrored, in the second pass
-        if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) put_packed(p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31), w);
+        if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) put_packed(p.out, row, p.oc, col, p.opl, w);
     }
     if (p.fin && !p.fin_t) return;
     lds_barrier();          // (not __syncthreads: it would wait for the stores above)
@@ -300,7 +302,7 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = row + e < col ? d[e] : w[e];
         }
-        put_packed(p.outT + ((size_t)col * p.otc + (row >> 5)) * 64 + (row & 31), w);
+        put_packed(p.outT, col, p.otc, row, p.opl, w);
     }
 }
 
@@ -327,9 +329,9 @@ __device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, cons
                     const int row = m0 + wm + 32 * x + 8 * g + 4 * fh;
                     ch[g] = cl4[g] = half4{0, 0, 0, 0};
                     if (col < p.N && row < padM) {
-                        const _Float16* c = p.C + ((size_t)col * p.oc + (row >> 5)) * 64 + (row & 31);
+                        const _Float16* c = p.C + ((size_t)col * p.oc + (row >> 5)) * (32 * p.cpl) + (row & 31);
                         ch[g] = *reinterpret_cast<const half4*>(c);
-                        cl4[g] = *reinterpret_cast<const half4*>(c + 32);
+                        if (p.cpl == 2) cl4[g] = *reinterpret_cast<const half4*>(c + 32);
                     }
                 }
 #pragma unroll
@@ -350,7 +352,7 @@ __device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, cons
         if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) {
             const uint4v lo = *reinterpret_cast<const uint4v*>(t + rl * S + cl), hi = *reinterpret_cast<const uint4v*>(t + rl * S + cl + 4);
             const unsigned w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            put_packed(p.out + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31), w);
+            put_packed(p.out, row, p.oc, col, p.opl, w);
         }
     }
 #pragma unroll 4
@@ -365,7 +367,7 @@ __device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, cons
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = row + e < col ? d[e] : w[e];
             }
-            put_packed(p.outT + ((size_t)col * p.otc + (row >> 5)) * 64 + (row & 31), w);
+            put_packed(p.outT, col, p.otc, row, p.opl, w);
         }
     }
 }
@@ -1034,8 +1036,7 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
 //         grows: 128 x 131: 2.6e-6 of the exact result against 1.4e-6 step by step, 70 x 600: 2.5e-6 against 1.6e-6);
 //   bf16: 2^-22 g^(h-1) <= 5e-3, five steps (worst case measured 6e-4, a matrix dominated by one direction; the result's rounding: 1.7e-3);
 //   fp16: 2^-22 g^(h-1) <= 5e-5, three steps (the rounding: 2e-4).
-// Of one limit for the whole chunk the cheapest is taken: work at 0.8 PFLOP/s of plane products, and 6.5 us for each launch of the matrix that
-// has most of them.
+// Of one limit for the whole chunk the cheapest is taken: the work, and 6.5 us for each launch of the matrix that has most of them.
 bool hops_in_f32(const Shape& s) { return s.m >= 256 && s.n >= 2 * s.m; }
 
 int hop_cap(const Shape& s, int steps, int dtype, double g)
@@ -1046,35 +1047,48 @@ int hop_cap(const Shape& s, int steps, int dtype, double g)
     return h;
 }
 
-void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, double g, int* hop)
+// Steps at the end that run one by one on one plane, h alone, where that is cheaper: bf16 only, two.  The singular values are within a factor
+// of a few of 1 by then, nothing grows any more: whatever the spectrum it adds 4e-4 (one step) to 8e-4 (two; three: up to 2e-3) to the
+// result's own rounding of 1.7e-3 (8 of 2048 x 2048: 4180 us without, 3560 with two).  Other coefficients: while |Q| and |X| stay as small.
+constexpr int MAX_TAIL = 2;
+int tail_cap(int steps, int dtype, const Bounds& b) { return dtype == MP_DTYPE_BF16 && steps > MAX_TAIL && b.q <= 4.0 && b.x <= 2.0 ? MAX_TAIL : 0; }
+
+// -> tail.  work: operations of plane products, at 0.4 PFLOP/s (1024 x 1024 x 1024 reach 0.25, large ones 1.0)
+int plan_hops(const Shape* s, int k, int steps, int dtype, int planes, const Bounds& bd, int* hop)
 {
+    const double g = bd.q * bd.q;
     double best = 1e300;
-    for (int h = 1; h <= steps; ++h) {
-        int use[MAX_MAT];
-        bool more = h == 1;
-        double work = 0.0;
-        int launches = 0;
-        for (int q = 0; q < k; ++q) {
-            int mine = 2;
-            const int cap = hop_cap(s[q], steps, dtype, g);
-            use[q] = h < cap ? h : cap;
-            more = more || use[q] == h;
-            const double m = (double)s[q].m, n = (double)s[q].n;
-            for (int left = steps; left > 0; left -= use[q]) {
-                const int len = left < use[q] ? left : use[q];
-                // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
-                work += 2.0 * m * m * ((left == steps && planes == 1 ? 1.0 + 2.0 * 2.0 : 3.0 * 3.0) * n + 3.0 * (4.0 * len - 3.0) * m);
-                mine += len == 1 ? 3 : 3 * len + 1;       // Gram, apply; Q a step; T (and R), A between steps; R behind the last
+    int best_tail = 0;
+    for (int tail = 0; tail <= tail_cap(steps, dtype, bd); tail += MAX_TAIL)
+        for (int h = 1; h <= steps - tail; ++h) {
+            int use[MAX_MAT];
+            bool more = h == 1;
+            double work = 0.0;
+            int launches = 0;
+            for (int q = 0; q < k; ++q) {
+                int mine = 2 + 3 * tail;
+                const int cap = hop_cap(s[q], steps - tail, dtype, g);
+                use[q] = h < cap ? h : cap;
+                more = more || use[q] == h;
+                const double m = (double)s[q].m, n = (double)s[q].n;
+                for (int left = steps - tail; left > 0; left -= use[q]) {
+                    const int len = left < use[q] ? left : use[q];
+                    // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
+                    work += m * m * ((left == steps - tail && planes == 1 ? 1.0 + 2.0 * 2.0 : 3.0 * 3.0) * n + 3.0 * (4.0 * len - 3.0) * m);
+                    mine += len == 1 ? 3 : 3 * len + 1;       // Gram, apply; Q a step; T (and R), A between steps; R behind the last
+                }
+                work += tail * m * m * (3.0 * n + m);
+                launches = mine > launches ? mine : launches;
             }
-            launches = mine > launches ? mine : launches;
+            if (!more) break;        // (no matrix may take that many)
+            const double cost = work / 0.4e15 + launches * 6.5e-6;
+            if (cost < best * 0.999) {
+                best = cost;
+                best_tail = tail;
+                for (int q = 0; q < k; ++q) hop[q] = use[q];
+            }
         }
-        if (!more) break;        // (no matrix may take that many)
-        const double cost = work / 0.8e15 + launches * 6.5e-6;
-        if (cost < best * 0.999) {
-            best = cost;
-            for (int q = 0; q < k; ++q) hop[q] = use[q];
-        }
-    }
+    return best_tail;
 }
 
 size_t up(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -1367,7 +1381,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     int64_t blocks = 0, tiles = 0;
     double elems = 0.0;
     for (int q = 0; q < k; ++q) sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
-    plan_hops(sh, k, steps, dtype, a.planes, bd.q * bd.q, hop);
+    const int body = steps - plan_hops(sh, k, steps, dtype, a.planes, bd, hop);
     for (int q = 0; q < k; ++q) {
         ws += layout(sh[q], steps, dtype, ws, &bf[q]);
         Mat& m = a.m[q];
@@ -1406,6 +1420,16 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     MP_CHECK_LAUNCH();
 
     const float sX = pow2_scale(bd.x), sA = pow2_scale(bd.x * bd.x), sT = pow2_scale(bd.x * bd.x * bd.q), sQ = pow2_scale(bd.q);
+    // Every matrix walks through its hops by itself; a launch takes the present stage of each, whatever it is, so that hops of different lengths
+    // fill each other's launches (seven matrices up to 11988 x 1024, hops of two steps and of one: 23 products' launches in turns, 17 this way).
+    enum Stage { GRAM, SQUARE, STEP, NEXT, APPLY, END };
+    struct Walk {
+        Stage at;
+        int done, len, s, r, q;      // steps behind it, steps of this hop, step inside it, which P holds R / Q
+        float sR;
+        bool first;                  // X is still the input's planes (to be multiplied by r)
+        int xpl;                     // planes of X
+    } w[MAX_MAT];
     Probs g;
     g.fin_dtype = dtype;
     g.fin_update = up_.on;
@@ -1420,26 +1444,22 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
         p.sym = 1;
         p.alpha = 1.0f / (sl * sr);
         p.so = so;
+        p.opl = p.cpl = w[q].done < body ? 2 : 1;
         return p;
     };
-    // Every matrix walks through its hops by itself; a launch takes the present stage of each, whatever it is, so that hops of different lengths
-    // fill each other's launches (seven matrices up to 11988 x 1024, hops of two steps and of one: 23 products' launches in turns, 17 this way).
-    enum Stage { GRAM, SQUARE, STEP, NEXT, APPLY, END };
-    struct Walk {
-        Stage at;
-        int done, len, s, r, q;      // steps behind it, steps of this hop, step inside it, which P holds R / Q
-        float sR;
-        bool first;                  // X is still the input's planes (to be multiplied by r)
-    } w[MAX_MAT];
-    for (int q = 0; q < k; ++q) w[q] = Walk{GRAM, 0, steps < hop[q] ? steps : hop[q], 0, 0, 0, sQ, true};
+    for (int q = 0; q < k; ++q) w[q] = Walk{GRAM, 0, body < hop[q] ? body : hop[q], 0, 0, 0, sQ, true, a.planes};
     for (;;) {
         bool more = false;
-        for (int kind = 0; kind < 3; ++kind) {        // operands of two planes, Gram products and X <- R X of one-plane matrices
+        int planes[MAX_MAT];        // of the operands: 0 (2, 2), 1 (1, 1), 2 (2, 1)
+        for (int q = 0; q < k; ++q) {
+            const int apl = w[q].done < body ? 2 : 1, left = w[q].at == GRAM ? w[q].xpl : apl, right = w[q].at == GRAM || w[q].at == APPLY ? w[q].xpl : apl;
+            planes[q] = left + right == 4 ? 0 : left == 1 ? 1 : 2;
+        }
+        for (int kind = 0; kind < 3; ++kind) {
             g.count = 0;
             for (int q = 0; q < k; ++q) {
                 Walk& v = w[q];
-                const bool one = v.first && a.planes == 1;
-                if (v.at == END || kind != (one && v.at == GRAM ? 1 : one && v.at == APPLY ? 2 : 0)) continue;
+                if (v.at == END || kind != planes[q]) continue;
                 more = true;
                 if (v.at == GRAM) {                   // A = X X^T
                     Prob p = sym_prob(q, bf[q].X, bf[q].X, v.first ? 1.0f : sX, v.first ? 1.0f : sX, bf[q].A, sA);
@@ -1489,6 +1509,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                         p.oc = chunks(sh[q].n);
                         p.otc = chunks(sh[q].m);
                         p.so = sX;
+                        p.opl = v.xpl = v.done + v.len < body ? 2 : 1;
                         char* t = bf[q].XT;
                         bf[q].XT = bf[q].XT2;
                         bf[q].XT2 = t;
@@ -1507,7 +1528,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
             else if (v.at == NEXT) { ++v.s; v.at = SQUARE; }
             else if (v.at == APPLY) {
                 v.done += v.len;
-                v.len = steps - v.done < hop[q] ? steps - v.done : hop[q];
+                v.len = v.done >= body ? (v.done < steps ? 1 : 0) : body - v.done < hop[q] ? body - v.done : hop[q];
                 v.s = 0;
                 v.first = false;
                 v.at = v.len ? GRAM : END;

@@ -272,3 +272,19 @@ def test_refusals(ops):
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.orthogonalize([g.cpu()])
     ops.muon_step([], [], [], **ok)
+
+
+@pytest.mark.parametrize("kind", ["plain", "gradient", "lowrank"])
+@pytest.mark.parametrize("rows,cols", [(256, 256), (700, 700), (1000, 1300), (1300, 1000)])
+def test_bfloat16_steps_on_one_plane(ops, rows, cols, kind):
+    """The last two bf16 steps round X, A and Q to fp16: each is off by an rms of 2^-12 / sqrt(3) of its entries, six such roundings, the first
+    three carried through a step of slope <= a = 3.45 whose rms over singular values near 1 is about 1: they add at most 0.5 of the result's own
+    rounding (rms 2^-9 / sqrt(3), 8 times as large), the Gram-side hop before them 0.4.  In 2-norm together with it: sqrt(1 + 0.25 + 0.16) = 1.19."""
+    g = make(rows, cols, torch.bfloat16, 11, kind)
+    want, _ = reference(g)
+    rounding = float((want.to(torch.bfloat16).double() - want).norm())
+    p, m = torch.zeros_like(g), g.float()
+    outs = [ops.orthogonalize([g])[0], ops.orthogonalize([g, make(90, 120, torch.bfloat16), g])[2]]
+    ops.muon_step([p], [g], [m], lr=1.0, scale=None)         # the momentum is the gradient: p = -orthogonalize(g)
+    for out in outs + [-p]:
+        assert float((out.double().cpu() - want).norm()) <= 1.19 * rounding
