@@ -240,3 +240,16 @@ def test_refusals(ops):
     (gx,) = torch.autograd.grad(ops.layer_norm(xg, w).square().sum(), xg, create_graph=True)
     with pytest.raises(RuntimeError):
         gx.sum().backward()
+
+
+# vectors of a row (16 bytes each) on both sides of every form's limits; rows enough for the register form of the backward pass, and for some
+# workgroups to walk several of them
+@pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.float16, torch.float32), (torch.float16, torch.float16),
+                                          (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("vecs,rows", [(65, 1100), (128, 6200), (129, 1100), (192, 3300), (193, 1100), (256, 1700), (257, 700), (512, 600), (513, 300),
+                                       (768, 300), (769, 300), (1024, 300), (1025, 300), (1536, 300), (1537, 300), (2047, 270), (2048, 65)])
+@pytest.mark.parametrize("off", [0, 1])
+def test_every_form_backward(ops, vecs, rows, off, dtype, wdtype):
+    V = 16 // dtype.itemsize
+    x, w, b, dy = make((rows, vecs * V - off), dtype, wdtype, vecs + off)
+    check(x, w, b, dy, 1e-5, run(ops, x, w, b, dy))
