@@ -643,18 +643,27 @@ def knn(p1, p2, lengths1=None, lengths2=None, K=1):
 
 
 _REDUCE_COUNTERS = {}
+_RECORDED_COUNTERS = {}      # device -> [pool of zeros, next free index, earlier pools (recordings point into them)]
+_COUNTER_POOL = 4096
 
 
 def _reduce_counter(device):
     """The zero-on-entry / zero-on-exit device counter of the one-launch reductions.  Launches on one stream run one after the other
     and may share a counter; launches on two streams (evaluation metrics next to the training stream) must not, so eager launches
-    get one counter per (device, stream).  Launches recorded into a hipGraph get the device's "graph" counter: replays of the
-    training step's graphs are ordered among themselves, and the counter is created by the first EAGER call (the harness runs
-    eager steps before it records), so no allocation or fill lands inside a capture."""
-    graph_key = (device, "graph")
-    if graph_key not in _REDUCE_COUNTERS and not torch.cuda.is_current_stream_capturing():
-        _REDUCE_COUNTERS[graph_key] = torch.zeros((1,), dtype=torch.int32, device=device)
-    key = graph_key if torch.cuda.is_current_stream_capturing() else (device, torch.cuda.current_stream(device).cuda_stream)
+    get one counter per (device, stream).  Every launch recorded into a hipGraph gets a counter of its own: two graphs may replay at the same
+    time on two streams.  They come from a pool of zeros that eager calls make and refill (the harness runs eager steps before it records), so
+    no allocation or fill lands inside a capture; a recording beyond the pool makes its counter inside the graph, cleared by every replay."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    pool = _RECORDED_COUNTERS.get(device)
+    if not capturing and (pool is None or pool[1] > _COUNTER_POOL // 2):
+        pool = _RECORDED_COUNTERS[device] = [torch.zeros((_COUNTER_POOL,), dtype=torch.int32, device=device), 0,
+                                             [] if pool is None else pool[2] + [pool[0]]]
+    if capturing:
+        if pool is None or pool[1] >= _COUNTER_POOL:
+            return torch.zeros((1,), dtype=torch.int32, device=device)
+        pool[1] += 1
+        return pool[0][pool[1] - 1:pool[1]]
+    key = (device, torch.cuda.current_stream(device).cuda_stream)
     t = _REDUCE_COUNTERS.get(key)
     if t is None:
         t = torch.zeros((1,), dtype=torch.int32, device=device)

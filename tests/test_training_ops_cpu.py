@@ -144,3 +144,24 @@ def test_muon_step_finds_shared_memory():
                           ([buf, m], [g]), ([buf[60:], p], [buf[:64]]), ([p, m, n], [g, buf[20:40], g])):
         with pytest.raises(ValueError, match="shares memory"):
             _no_overlap(written, read)
+
+
+def test_recorded_reductions_have_counters_of_their_own(monkeypatch):
+    """Two recordings replayed on two streams at once must not count each other's workgroups (a loss term came out partial)."""
+    from maskplanner_amd import ops
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": 7})())
+    monkeypatch.setattr(ops, "_REDUCE_COUNTERS", {})
+    monkeypatch.setattr(ops, "_RECORDED_COUNTERS", {})
+    monkeypatch.setattr(ops, "_COUNTER_POOL", 8)
+    d = torch.device("cpu")
+    eager = ops._reduce_counter(d)
+    assert ops._reduce_counter(d) is eager
+    capturing[0] = True
+    taken = [ops._reduce_counter(d) for _ in range(10)]           # the last two beyond the pool
+    assert len({t.data_ptr() for t in taken + [eager]}) == 11 and all(int(t) == 0 and t.numel() == 1 for t in taken)
+    capturing[0] = False
+    assert ops._reduce_counter(d) is eager
+    capturing[0] = True
+    assert ops._reduce_counter(d).data_ptr() not in {t.data_ptr() for t in taken}
