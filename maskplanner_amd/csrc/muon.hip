@@ -45,7 +45,7 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     int M, N, kc, oc, otc, rpow, sym, tiles_n, fin_t;
     float alpha, cb, ca, so, fmul, fdecay;
     int tiles, seg;          // tiles of the result; chunks of a segment of K (kc: not cut)
-    int ll : 8;              // the product of the l planes too (LL)  (bits: of bytes the scalar loads of the arguments know nothing)
+    int ll : 8;              // the product of the l planes too (WITH_LL)  (bits: of bytes the scalar loads of the arguments know nothing)
     int opl : 8, cpl : 8;    // planes of out / outT, of C
 };
 // A launch's work items, one a workgroup: the first `whole` tiles uncut, then the rest in segments of K.  Items are ordered by segment, then by
@@ -382,7 +382,11 @@ template <int PL> __device__ __forceinline__ int swz(int row) { return PL == 2 ?
 // KW: the four waves share a (32 WM) x (32 WN) tile by K instead, wave v taking chunks v, v + 4, ..: each with a ring of its own and no
 // meeting at all; their sums meet in LDS at the end, added in the order of the waves.  For 64 x 64 tiles, where a wave of the shared form has
 // three products between two meetings (136 tiles of K = 1024: 15.2 us shared, 12.7 this way).
-template <int WM, int WN, int PL, int PR, int NS, bool KW, bool LL>
+// MODE: PLAIN; WITH_LL: products of the l planes too, for the problems that ask for them; PAIRS: images of one plane with an even number of chunks,
+// two of them where the others have h and l -- the same loads, reads and meetings, products h h and l l.  (A chunk of one plane has too few
+// matrix instructions between two meetings: 8 of 2048 x 2048, X <- Q X: 250 us chunk by chunk, 222 in pairs.)
+enum Mode { PLAIN, WITH_LL, PAIRS };
+template <int WM, int WN, int PL, int PR, int NS, bool KW, int MODE>
 __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 {
     constexpr int WAVES = KW ? 1 : 4;                              // waves that load a stage together
@@ -457,7 +461,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 
         const int rowL = wm + fr, rowR = wn + fr;        // (32 rows on: the same swizzle)
         half8 fl[2][WM][PL], fq[2][WN][PR];
-        constexpr int READS = WM * PL + WN * PR, PRODS = (PL + PR - 1) * WM * WN, FETCHES = NL + NR;
+        constexpr int READS = WM * PL + WN * PR, PRODS = (MODE == PAIRS ? 2 : PL + PR - 1) * WM * WN, FETCHES = NL + NR;
         auto read_one = [&](int buf, int ks, int k) {
             const char* s = ring + buf * STAGE;
             if (k < WM * PL) {
@@ -471,7 +475,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
         // The PRODS matrix instructions of 16 k, the small products first, a block's WM * WN apart; in the shadow of each (32 cycles) go its
         // share of the reads of the other half's fragments and of the loads of a chunk to come: with one wave a SIMD nothing else fills it.
         auto multiply = [&](int ks, bool reads, int rbuf, bool fetches, int fbuf) {
-            if constexpr (LL)        // (a question of its own kernel: asked in all of them it costs 1 % of a small launch)
+            if constexpr (MODE == WITH_LL)        // (a question of its own kernel: asked in all of them it costs 1 % of a small launch)
                 if (p.ll)
 #pragma unroll
                     for (int g = 0; g < WM * WN; ++g)
@@ -479,7 +483,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 #pragma unroll
             for (int g = 0; g < PRODS; ++g) {
                 const int k = g / (WM * WN), x = g / WN % WM, y = g % WN;
-                const int pl = PL == 2 && k == 0 ? 1 : 0, pr = PR == 2 && k == PL - 1 ? 1 : 0;
+                const int pl = MODE == PAIRS ? k : PL == 2 && k == 0 ? 1 : 0, pr = MODE == PAIRS ? k : PR == 2 && k == PL - 1 ? 1 : 0;
                 acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][pl], fq[ks][y][pr], acc[x][y], 0, 0, 0);
                 if (reads)
 #pragma unroll
@@ -1049,7 +1053,7 @@ int hop_cap(const Shape& s, int steps, int dtype, double g)
 
 // Steps at the end that run one by one on one plane, h alone, where that is cheaper: bf16 only, two.  The singular values are within a factor
 // of a few of 1 by then, nothing grows any more: whatever the spectrum it adds 4e-4 (one step) to 8e-4 (two; three: up to 2e-3) to the
-// result's own rounding of 1.7e-3 (8 of 2048 x 2048: 4180 us without, 3560 with two).  Other coefficients: while |Q| and |X| stay as small.
+// result's own rounding of 1.7e-3 (8 of 2048 x 2048: 4180 us without, 3460 with two).  Other coefficients: while |Q| and |X| stay as small.
 constexpr int MAX_TAIL = 2;
 int tail_cap(int steps, int dtype, const Bounds& b) { return dtype == MP_DTYPE_BF16 && steps > MAX_TAIL && b.q <= 4.0 && b.x <= 2.0 ? MAX_TAIL : 0; }
 
@@ -1188,15 +1192,15 @@ Plan plan_of(const Prob* p, int count, int products)
     return best;
 }
 
-template <int WM, int WN, int PL, int PR, int NS, bool KW, bool LL>
+template <int WM, int WN, int PL, int PR, int NS, bool KW, int MODE>
 int launch_ring(const Probs& a, double flops, hipStream_t stream)
 {
     static mp::DynLds dyn;
     constexpr int TM = KW ? 32 * WM : 64 * WM, TN = KW ? 32 * WN : 64 * WN, RINGS = KW ? 4 : 1;
     constexpr size_t ring = (size_t)RINGS * NS * 64 * (TM * PL + TN * PR), tile = (size_t)RINGS * TM * (TN + TPAD) * sizeof(float);
     constexpr size_t smem = ring > tile ? ring : tile;
-    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW, LL>), smem)) return MP_ELAUNCH;
-    MP_LAUNCH("ns_gemm_kernel", flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW, LL>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
+    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW, MODE>), smem)) return MP_ELAUNCH;
+    MP_LAUNCH("ns_gemm_kernel", flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW, MODE>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
     MP_CHECK_LAUNCH();
     if (a.whole < a.tiles) {
         MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<TM, TN>), dim3((unsigned)(a.tiles - a.whole) * (TM / 32)), dim3(256), 0, stream, a);
@@ -1207,25 +1211,29 @@ int launch_ring(const Probs& a, double flops, hipStream_t stream)
 
 // Depth of the ring: what 144 KB hold (at most 8 chunks) where the launch has one workgroup a CU at most, else half of that so that two
 // share a CU (256 x 128 and the K-sharing 64 x 64: always one).
-template <int WM, int WN, int PL, int PR, bool KW>
+template <int WM, int WN, int PL, int PR, bool KW, int MODE>
 int launch_as(const Probs& a, double flops, hipStream_t stream)
 {
     constexpr int lds = 147456, stage = KW ? 4 * 64 * 32 * (WM * PL + WN * PR) : 64 * 64 * (WM * PL + WN * PR);
     constexpr int deep = lds / stage < 8 ? lds / stage : 8, half = KW || WM * WN >= 8 ? deep : (lds / 2 / stage < 8 ? lds / 2 / stage : 8);
-    if constexpr (KW && PL == 2 && PR == 2) {
+    if constexpr (KW && PL == 2 && PR == 2 && MODE == PLAIN) {
         bool ll = false;
         for (int i = 0; i < a.count; ++i) ll = ll || a.p[i].ll;
-        if (ll) return launch_ring<WM, WN, PL, PR, deep, KW, true>(a, flops, stream);
+        if (ll) return launch_ring<WM, WN, PL, PR, deep, KW, WITH_LL>(a, flops, stream);
     }
-    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW, false>(a, flops, stream);
-    return launch_ring<WM, WN, PL, PR, half, KW, false>(a, flops, stream);
+    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW, MODE>(a, flops, stream);
+    return launch_ring<WM, WN, PL, PR, half, KW, MODE>(a, flops, stream);
 }
 
 // planes of the left and the right operands: (2, 2), (2, 1) or (1, 1)
 int launch(Probs& a, int left, int right, hipStream_t stream)
 {
     if (a.count == 0) return MP_OK;
-    const int products = left + right - 1;
+    bool pairs = left == 1 && right == 1;
+    for (int i = 0; i < a.count; ++i) pairs = pairs && a.p[i].kc % 2 == 0;
+    if (pairs)
+        for (int i = 0; i < a.count; ++i) a.p[i].kc /= 2;
+    const int products = pairs ? 2 : left + right - 1;
     const Plan pl = plan_of(a.p, a.count, products);
     const TileShape ts = SHAPES[pl.shape];
     if (pl.shape < 0) return MP_EUNSUPPORTED;
@@ -1252,14 +1260,15 @@ int launch(Probs& a, int left, int right, hipStream_t stream)
     if (a.whole == a.tiles) items = tiles;
     else if (a.equal) items = a.whole + (int64_t)a.rest * ((a.p[0].kc + a.p[0].seg - 1) / a.p[0].seg);
     a.items = (int)items;
-#define NS_SHAPES(PL, PR)                                                                  \
-    return pl.shape == 0   ? launch_as<4, 2, PL, PR, false>(a, flops, stream)         \
-           : pl.shape == 1 ? launch_as<2, 2, PL, PR, false>(a, flops, stream)         \
-           : pl.shape == 2 ? launch_as<2, 2, PL, PR, true>(a, flops, stream)          \
-                           : launch_as<1, 1, PL, PR, true>(a, flops, stream)
-    if (left == 2 && right == 2) NS_SHAPES(2, 2);
-    if (left == 2) NS_SHAPES(2, 1);
-    NS_SHAPES(1, 1);
+#define NS_SHAPES(PL, PR, MODE)                                                     \
+    return pl.shape == 0   ? launch_as<4, 2, PL, PR, false, MODE>(a, flops, stream) \
+           : pl.shape == 1 ? launch_as<2, 2, PL, PR, false, MODE>(a, flops, stream) \
+           : pl.shape == 2 ? launch_as<2, 2, PL, PR, true, MODE>(a, flops, stream)  \
+                           : launch_as<1, 1, PL, PR, true, MODE>(a, flops, stream)
+    if (left == 2 && right == 2) NS_SHAPES(2, 2, PLAIN);
+    if (left == 2) NS_SHAPES(2, 1, PLAIN);
+    if (pairs) NS_SHAPES(2, 2, PAIRS);
+    NS_SHAPES(1, 1, PLAIN);
 #undef NS_SHAPES
 }
 
