@@ -253,3 +253,17 @@ def test_every_form_backward(ops, vecs, rows, off, dtype, wdtype):
     V = 16 // dtype.itemsize
     x, w, b, dy = make((rows, vecs * V - off), dtype, wdtype, vecs + off)
     check(x, w, b, dy, 1e-5, run(ops, x, w, b, dy))
+
+
+def test_offsets_beyond_32_bits(ops):
+    """2^31 elements and more, 4.3 GB a tensor: first, middle and last rows against 64 bits, the others zeros (y = b, dx = 0, nothing in dw)"""
+    rows, D = (1 << 21) + 3, 1100
+    x = torch.zeros((rows, D), dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros_like(x)
+    at = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    xs, w, b, dys = make((len(at), D), torch.bfloat16, torch.float32, 5)
+    x[at], dy[at] = xs, dys
+    y, dx, dw, db = run(ops, x, w, b, dy)
+    check(xs, w, b, dys, 1e-5, (y[at], dx[at], dw, db))
+    for r in (2, rows // 2 + 1, rows - 3):
+        assert torch.equal(y[r], b.to(torch.bfloat16)) and not dx[r].any()

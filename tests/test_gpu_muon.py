@@ -288,3 +288,30 @@ def test_bfloat16_steps_on_one_plane(ops, rows, cols, kind):
     ops.muon_step([p], [g], [m], lr=1.0, scale=None)         # the momentum is the gradient: p = -orthogonalize(g)
     for out in outs + [-p]:
         assert float((out.double().cpu() - want).norm()) <= 1.19 * rounding
+
+
+def test_offsets_beyond_32_bits(ops):
+    """more than 2^31 elements: columns of the result from the small side in float64, R = Q_5 .. Q_1 of A = X X^T.  Tolerance as above."""
+    m, n = 1040, (1 << 21) - 5
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    g = torch.empty((m, n), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    gram = torch.zeros((m, m), dtype=torch.float64, device="cuda")
+    for c in range(0, n, 1 << 18):
+        part = g[:, c:c + (1 << 18)].double()
+        gram += part @ part.t()
+        del part
+    norm = float(gram.trace().sqrt())
+    a, r = gram / norm ** 2, torch.eye(m, dtype=torch.float64, device="cuda")
+    for _ in range(5):
+        q = COEF[0] * torch.eye(m, dtype=torch.float64, device="cuda") + COEF[1] * a + COEF[2] * a @ a
+        a, r = q @ a @ q, q @ r
+    cols = torch.tensor([0, 1, 12345, n // 2, n - 700, n - 2, n - 1], device="cuda")
+    want = r @ (g[:, cols].double() / norm)
+    tol = tolerance(want.cpu(), (g[:, cols].double() / norm).cpu(), torch.bfloat16)
+    (out,) = ops.orthogonalize([g])
+    assert float((out[:, cols].double() - want).norm()) <= tol
+    del out
+    tall = g.t().contiguous()
+    del g
+    (out,) = ops.orthogonalize([tall])
+    assert float((out[cols].t().double() - want).norm()) <= tol
