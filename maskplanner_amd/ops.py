@@ -984,66 +984,7 @@ def _rows_of(x):
     return x, x.stride(0)
 
 
-class _LayerNorm(torch.autograd.Function):
-    # Host time is all of a small call (32 x 1024: 3 us of kernels each way): outputs by empty_like (1.1 us; torch.empty with shape, dtype and
-    # device 3.2), no wrapper around the backward pass where none is needed.
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        D = x.shape[-1]
-        rows = x.numel() // D
-        if x.is_contiguous():
-            x2, xs, y = x, D, torch.empty_like(x)
-        else:
-            x2, xs = _rows_of(x)
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        like = weight if weight is not None else bias
-        wt = _DTYPE[x.dtype if like is None else like.dtype]
-        mean = None
-        if True in ctx.needs_input_grad:
-            stats = x.new_empty((2, rows), dtype=torch.float32)
-            mean = stats.data_ptr() if rows else None
-            ctx.save_for_backward(x, weight, bias, stats)
-            ctx.args = rows, D, wt
-        _run("layer_norm", x, _lib.load().mp_layer_norm_fwd, x2.data_ptr(), _DTYPE[x.dtype], rows, D, xs, _p(weight), _p(bias), wt, eps,
-             y.data_ptr(), mean, mean + 4 * rows if mean else None)
-        return y
-
-    @staticmethod
-    def backward(ctx, grad_y):
-        # (once_differentiable's wrapper costs 4-5 us: only where a second derivative can be asked for)
-        return (_LayerNorm._backward_once if torch.is_grad_enabled() else _LayerNorm._backward)(ctx, grad_y)
-
-    @staticmethod
-    def _backward(ctx, grad_y):
-        x, weight, bias, stats = ctx.saved_tensors
-        rows, D, wt = ctx.args
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        if x.is_contiguous():
-            x2, xs, gx = x, D, torch.empty_like(x) if need_x else None
-        else:
-            x2, xs = _rows_of(x)
-            gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dy, dys = _rows_of(grad_y if grad_y.dtype == x.dtype else grad_y.to(x.dtype))
-        gw = torch.empty_like(weight) if need_w else None
-        gb = torch.empty_like(bias) if need_b else None
-        lib, dt, ws, nbytes = _lib.load(), _DTYPE[x.dtype], None, 0
-        if need_w or need_b:
-            nbytes = lib.mp_layer_norm_bwd_workspace_bytes(rows, D, dt)
-            if nbytes:
-                ws = x.new_empty((nbytes,), dtype=torch.uint8)
-        mean = stats.data_ptr()
-        _run("layer_norm_bwd", x, lib.mp_layer_norm_bwd, dy.data_ptr(), dys, x2.data_ptr(), xs, dt, rows, D, _p(weight), wt, mean, mean + 4 * rows,
-             _p(gx), _p(gw), _p(gb), _p(ws), nbytes)
-        return gx, gw, gb, None
-
-    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
-
-
-def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """Layer normalisation of x [..., D] over its last axis: weight * (x - mean) / sqrt(var + eps) + bias, one launch forward; backward the
-    gradients of x, weight and bias (two launches, fixed summation order).  x float32, float16 or bfloat16; weight / bias [D] in float32 or
-    x's type, both of one type, or None.  Any leading shape, also none or an empty one; rows may be strided (a view with another element
-    stride is copied).  Arithmetic in fp32, rounded once to x's type.  Not differentiable twice."""
+def _check_layer_norm(x, weight, bias, eps):
     _need_hip(x, weight, bias)
     if x.ndim == 0 or x.shape[-1] < 1:
         raise ValueError("layer_norm expects [..., D] input with D >= 1")
@@ -1061,7 +1002,101 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
             raise ValueError(f"layer_norm: {name} is on {t.device}, the input on {x.device}")
     if not eps >= 0:
         raise ValueError("layer_norm: eps must not be negative")
-    return _LayerNorm.apply(x, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), float(eps))
+
+
+def _layer_norm_backward(ctx, grad_y):
+    x, weight = ctx.saved_tensors
+    _, mean, rstd, rows, D, dt, wt, wdtype, dev, fn, nbytes = ctx.args
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    gx = gw = gb = px = pw = pb = ws = None
+    x2, xs, dys = x, D, D
+    if x.is_contiguous():
+        if need_x:
+            gx = torch.empty_like(x)
+    else:
+        x2, xs = _rows_of(x)
+        if need_x:
+            gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if need_x:
+        px = gx.data_ptr()
+    if not grad_y.is_contiguous() or grad_y.dtype is not x.dtype:
+        grad_y, dys = _rows_of(grad_y.to(x.dtype))
+    if need_w:
+        gw = torch.empty_like(weight)
+        pw = gw.data_ptr()
+    if need_b:
+        gb = x.new_empty((D,), dtype=wdtype) if gw is None else torch.empty_like(gw)
+        pb = gb.data_ptr()
+    if nbytes:
+        ws = x.new_empty((nbytes,), dtype=torch.uint8)
+    args = (grad_y.data_ptr(), dys, x2.data_ptr(), xs, dt, rows, D, None if weight is None else weight.data_ptr(), wt, mean, rstd, px, pw, pb,
+            _p(ws), nbytes)
+    if KernelTimer.active is None and dev == _cur_device():       # (as _run)
+        rc = fn(*args, _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "layer_norm_bwd")
+    else:
+        _run("layer_norm_bwd", x, fn, *args)
+    return gx, gw, gb, None
+
+
+class _LayerNorm(torch.autograd.Function):
+    # Host time is all of a small call (32 x 1024: 3 us of kernels each way): every attribute is looked at once, outputs come by empty_like (1.1 us;
+    # torch.empty with shape, dtype and device 3.2), nothing wraps the backward pass where no second derivative can be asked for, and what it
+    # needs is put together in forward (autograd's device thread often starts with cold caches: Python costs twice as much there).
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        dtype, shape, dev = x.dtype, x.shape, x.get_device()
+        wdtype = None if weight is None else weight.dtype
+        # the usual call in one expression; what it does not cover goes through the checks one by one
+        if (dev < 0 or weight is None or bias is None or not shape or weight.shape != shape[-1:] or bias.shape != shape[-1:]
+                or bias.dtype is not wdtype or (wdtype is not dtype and wdtype is not torch.float32) or dtype not in _DTYPE
+                or weight.get_device() != dev or bias.get_device() != dev or shape[-1] < 1 or not eps >= 0):
+            _check_layer_norm(x, weight, bias, eps)
+            if weight is None:
+                wdtype = dtype if bias is None else bias.dtype
+        D = shape[-1]
+        rows = x.numel() // D
+        dt, wt = _DTYPE[dtype], _DTYPE[wdtype]
+        if x.is_contiguous():
+            x2, xs, y = x, D, torch.empty_like(x)
+        else:
+            x2, xs = _rows_of(x)
+            y = torch.empty(shape, dtype=dtype, device=x.device)
+        mean = rstd = None
+        lib = _lib.load()
+        needs = ctx.needs_input_grad
+        if True in needs:
+            stats = x.new_empty((2, rows), dtype=torch.float32)      # (neither input nor output: no need of the saved tensors' checks)
+            if rows:
+                mean = stats.data_ptr()
+                rstd = mean + 4 * rows
+            ctx.save_for_backward(x, weight)
+            ctx.args = (stats, mean, rstd, rows, D, dt, wt, wdtype, dev, lib.mp_layer_norm_bwd,
+                        lib.mp_layer_norm_bwd_workspace_bytes(rows, D, dt) if needs[1] or needs[2] else 0)
+        _run("layer_norm", x, lib.mp_layer_norm_fwd, x2.data_ptr(), dt, rows, D, xs, None if weight is None else weight.data_ptr(),
+             None if bias is None else bias.data_ptr(), wt, eps, y.data_ptr(), mean, rstd)
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        if torch.is_grad_enabled():
+            return _LayerNorm._backward_once(ctx, grad_y)         # (once_differentiable's wrapper: 4-5 us)
+        return _layer_norm_backward(ctx, grad_y)
+
+    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_layer_norm_backward))
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer normalisation of x [..., D] over its last axis: weight * (x - mean) / sqrt(var + eps) + bias, one launch forward; backward the
+    gradients of x, weight and bias (two launches, fixed summation order).  x float32, float16 or bfloat16; weight / bias [D] in float32 or
+    x's type, both of one type, or None.  Any leading shape, also none or an empty one; rows may be strided (a view with another element
+    stride is copied).  Arithmetic in fp32, rounded once to x's type.  Not differentiable twice."""
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return _LayerNorm.apply(x, weight, bias, eps)
 
 
 # ----------------------------------------------------------------------------------------------------------------
