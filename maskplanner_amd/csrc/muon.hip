@@ -736,7 +736,7 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
 
 // ---- small matrices: everything in one launch ------------------------------------------------------------------------------------
 // m <= 64 and planes that fit a CU's LDS: a workgroup of eight waves has a matrix from gradient to result.  17 launches of a few
-// microseconds would be all there is to it (64 x 64 fp32: 100 us, 26 here; from m = 96 on the launches win: 128 x 131 took 118 us this
+// microseconds would be all there is to it (64 x 64 fp32: 100 us, 27 here; from m = 96 on the launches win: 128 x 131 took 118 us this
 // way).  Wave v holds the columns of blocks v, v + 8, .. of 32 of X in registers (packed planes, in the accumulator layout of the product
 // that made them: that layout is the right operand's of the next product Q X if Q's columns are read in the same order, two runs of four).
 // LDS holds X's planes for the Gram product and one m x m matrix, A and then Q.
@@ -758,6 +758,11 @@ static_assert(sizeof(Smalls) <= 3584, "travels in the kernel arguments");
 
 constexpr int SMALL_LDS = 147456 + 256;        // (256: the padding of the fp32 tile that lies over X's planes on the way in and out)
 constexpr int small_nb(int mb) { return mb == 1 ? 4 : 2; }      // column blocks a wave
+// Waves that share a block of the Gram product by K, from 256 columns on: one wave alone is what 16 x 900 waits for (57 us, with four 45), short
+// ones lose two meetings a step (32 x 32: 16 us, 18); with 64 rows four waves have a block each (64 x 500: 65, with two 64).
+constexpr int small_ks(int mb) { return mb == 1 ? 4 : 1; }
+constexpr int SMALL_KS_CHUNKS = 8;
+constexpr int small_s(int mb) { return mb == 1 ? 12288 : 16384; }      // bytes in front of X: the m x m image, before it the sums of those waves
 
 template <int MB, int DT>
 __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
@@ -770,7 +775,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
     const bool tall = m.rows > m.cols;
     const int M = tall ? m.cols : m.rows, N = tall ? m.rows : m.cols, npc = chunks(N);
     char* S = lds;
-    char* X = lds + 32 * MB * MB * 128;
+    char* X = lds + small_s(MB);
     auto unit = [&](char* img, int row, int nch, int chunk, int u) { return img + ((size_t)row * nch + chunk) * 128 + ((u ^ (row & 7)) * 16); };
 
     // In and out by way of LDS (over X's planes): a wave reads rows of the matrix as it lies in memory.
@@ -838,7 +843,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
         int zero = 0;
         asm volatile("" : "+v"(zero));
         S = lds + zero;
-        X = lds + 32 * MB * MB * 128 + zero;
+        X = lds + small_s(MB) + zero;
         // X's planes to LDS.  A lane has a column: neighbours swap so that each writes two columns of one row.
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -858,21 +863,24 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
                 }
         }
         __syncthreads();
-        auto product = [&](char* img, int nch, int i, int j, bool full) {        // rows 32 i .. of the image times rows 32 j ..
-            float16v acc;
+        auto product = [&](char* img, int c0, int step, int nch, int i, int j, bool full) {        // rows 32 i .. of the image times rows 32 j ..
+            // (h h by itself: a third of the roundings at the size of the sum, and two chains of matrix instructions)
+            float16v acc, big;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) acc[k] = 0.0f;
+            for (int k = 0; k < 16; ++k) acc[k] = big[k] = 0.0f;
             const int ri = 32 * i + fr, rj = 32 * j + fr;
-            for (int c = 0; c < nch; ++c)
+            for (int c = c0; c < nch; c += step)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     const half8 lh = *reinterpret_cast<const half8*>(unit(img, ri, nch, c, ks * 2 + fh)), ll = *reinterpret_cast<const half8*>(unit(img, ri, nch, c, 4 + ks * 2 + fh));
                     const half8 rh = *reinterpret_cast<const half8*>(unit(img, rj, nch, c, ks * 2 + fh)), rl = *reinterpret_cast<const half8*>(unit(img, rj, nch, c, 4 + ks * 2 + fh));
                     if (full) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rl, acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh, acc, 0, 0, 0);
+                    big = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, big, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl, acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, acc, 0, 0, 0);
                 }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[k] += big[k];
             return acc;
         };
         auto keep = [&](float16v& v, float scale, int i, int j) {      // block (i, j) of a symmetric matrix as block (j, i), runs of four; v: what the planes hold
@@ -890,19 +898,34 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
                 *reinterpret_cast<half4*>(unit(S, 32 * j + fr, MB, i, 4 + rg) + fh * 8) = l;
             }
         };
-        // A, then Q, block (i, j) by wave i MB + j
+        // A, then Q, block (i, j) by wave i MB + j; the Gram product by KS waves
         float16v A;
-        const int i0 = wave / MB, j0 = wave % MB;
-        const bool mine = wave < MB * MB;
+        constexpr int KS = small_ks(MB), BLOCKS = MB * MB;
+        const int block = wave % BLOCKS, part = wave / BLOCKS, i0 = block / MB, j0 = block % MB;
+        const bool mine = part == 0;
+        const int share = KS > 1 && npc >= SMALL_KS_CHUNKS ? KS : 1;
+        if (part < share) A = product(X, part, share, npc, i0, j0, false);
+        if (share > 1) {
+            float* const sums = reinterpret_cast<float*>(S) + lane;
+            if (!mine && part < share)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) sums[((part - 1) * BLOCKS + block) * 1024 + k * 64] = A[k];
+            __syncthreads();
+            if (mine)
+#pragma unroll
+                for (int p = 0; p < KS - 1; ++p)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) A[k] += sums[(p * BLOCKS + block) * 1024 + k * 64];
+            __syncthreads();
+        }
         if (mine) {
-            A = product(X, npc, i0, j0, false);
 #pragma unroll
             for (int k = 0; k < 16; ++k) A[k] *= sx * sx;
             keep(A, a.sA, i0, j0);
         }
         __syncthreads();
         if (mine) {
-            const float16v sq = product(S, MB, i0, j0, DT == MP_DTYPE_F32);
+            const float16v sq = product(S, 0, 1, MB, i0, j0, DT == MP_DTYPE_F32);
             const float cc = a.c / (a.sA * a.sA), bb = a.b / a.sA;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
@@ -994,8 +1017,8 @@ constexpr int MAX_STEPS = 16;
 struct Bounds { double x, q, r[MAX_STEPS + 1]; bool ok; };    // of |X|, |Q| and |Q^h| (products of up to h successive Q) in spectral norm
 
 // The scalar recursion of a singular value, on a grid of starting values in [0, 1]: what the matrices can grow to.  30 us of host time, the
-// same for all steps of a training run: a thread keeps the last one (a property of the coefficients alone; 64 x 64 fp32: 31 us a call with
-// it formed every time, 26 this way).
+// same for all steps of a training run: a thread keeps the last one, a property of the coefficients alone (64 x 64 fp32 takes 5 us longer with
+// it formed every time).
 Bounds bounds_of(int steps, const double* c)
 {
     thread_local Bounds b;
@@ -1286,7 +1309,7 @@ size_t small_lds(int64_t rows, int64_t cols)
     const Shape s = shape_of(rows, cols);
     if (s.m > 64 || s.n > 1024) return 0;
     const int mb = chunks(s.m), npc = chunks(s.n);
-    const size_t lds = (size_t)32 * mb * 128 * (npc + mb) + 256;
+    const size_t lds = (size_t)32 * mb * 128 * npc + small_s(mb) + 256;
     return npc <= 8 * small_nb(mb) && lds <= SMALL_LDS ? lds : 0;
 }
 
