@@ -1003,6 +1003,134 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
         }
 }
 
+// ---- up to eight rows (or columns) ---------------------------------------------------------------------------------------------------
+// A thread has NC columns of X in fp32 registers: 36 dot products, an 8 x 8 polynomial and 64 multiply-adds a column are little for the vector
+// units (blocks of 32 rows of the matrix cores would be three quarters zeros), and fp32 throughout: sums of so few terms leave the planes' 22
+// bits bare (165 matrices up to 64 x 512: at most 3.7 times as far from the exact result as fp32 products, 2.3 with this kernel).  fp32, 5 x 100:
+// 19 us by ns_small_kernel, 11 this way; 8 x 1000: 45, 12; 8 x 4000: 97 by products' launches, 28.  (Summed value by value over a wave, six
+// dependent steps each, it took 43 us whatever the size.)
+constexpr int TINY_M = 8, TINY_THREADS = 512;
+
+template <int NC, int DT>
+__global__ __launch_bounds__(TINY_THREADS) void ns_tiny_kernel(Smalls a)
+{
+    __shared__ double s_sum[8];
+    __shared__ float part[8][36];
+    __shared__ __align__(16) float A[8][8], Q[8][8];
+    const Small m = a.m[blockIdx.x];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool tall = m.rows > m.cols;
+    const int M = tall ? m.cols : m.rows, N = tall ? m.rows : m.cols;
+    float x[NC][8];
+    double sum = 0.0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = c * TINY_THREADS + threadIdx.x;
+        float v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const bool in = col < N && r < M;
+            const size_t at = tall ? (size_t)col * M + r : (size_t)r * N + col;
+            x[c][r] = in ? load_any(m.g, DT, at) : 0.0f;
+            v[r] = in && m.mom ? m.mom[at] : 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if (m.mom && col < N && r < M) {
+                v[r] = v[r] + (1.0f - a.mu) * (x[c][r] - v[r]);
+                m.mom[tall ? (size_t)col * M + r : (size_t)r * N + col] = v[r];
+                x[c][r] = a.nesterov ? x[c][r] + a.mu * (v[r] - x[c][r]) : v[r];
+            }
+            sum += (double)x[c][r] * (double)x[c][r];
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += s_sum[k];
+    const double norm = sqrt(sum), scale = 1.0 / (norm > a.eps || norm != norm ? norm : a.eps);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) x[c][r] = (float)((double)x[c][r] * scale);
+    for (int step = 0; step < a.steps; ++step) {
+        // A: entry (i, j), j <= i, is number i (i + 1) / 2 + j.  A wave's sums of 36 numbers: halves of the wave keep 18 each, rows of 16 lanes 9 each
+        float g[36];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j <= i; ++j) {
+                float v = 0.0f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) v = fmaf(x[c][i], x[c][j], v);
+                g[i * (i + 1) / 2 + j] = v;
+            }
+#pragma unroll
+        for (int k = 0; k < 18; ++k) {
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(g[k]), __float_as_uint(g[k + 18]), false, false);
+            g[k] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 9; ++k) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(g[k]), __float_as_uint(g[k + 9]), false, false);
+            float v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+            v += __uint_as_float(mp::dpp_u32<mp::DPP_QUAD_XOR1>(__float_as_uint(v)));
+            v += __uint_as_float(mp::dpp_u32<mp::DPP_QUAD_XOR2>(__float_as_uint(v)));
+            v += __uint_as_float(mp::dpp_u32<mp::DPP_ROW_HALF_MIRROR>(__float_as_uint(v)));
+            v += __uint_as_float(mp::dpp_u32<mp::DPP_ROW_MIRROR>(__float_as_uint(v)));
+            if ((lane & 15) == 0) part[wave][k + 9 * (lane >> 4 & 1) + 18 * (lane >> 5)] = v;
+        }
+        __syncthreads();
+        const int i = lane >> 3, j = lane & 7, hi = i > j ? i : j, lo = i > j ? j : i;
+        if (wave == 0) {
+            float g = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) g += part[w][hi * (hi + 1) / 2 + lo];
+            A[i][j] = g;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            float q = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) q = fmaf(A[i][k], A[k][j], q);
+            Q[i][j] = fmaf(a.c, q, a.b * A[i][j]) + (i == j ? a.a : 0.0f);
+        }
+        __syncthreads();
+        float y[NC][8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            float q[8];
+            *reinterpret_cast<float4*>(q) = *reinterpret_cast<const float4*>(Q[r]);
+            *reinterpret_cast<float4*>(q + 4) = *reinterpret_cast<const float4*>(Q[r] + 4);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float acc = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc = fmaf(q[k], x[c][k], acc);
+                y[c][r] = acc;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[c][r] = y[c][r];
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = c * TINY_THREADS + threadIdx.x;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            if (col >= N || r >= M) continue;
+            const size_t at = tall ? (size_t)col * M + r : (size_t)r * N + col;
+            const float v = x[c][r];
+            store_fin(m.out, DT, at, a.update ? m.fdecay * load_any(m.out, DT, at) - m.fmul * v : v);
+        }
+    }
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 struct Shape { int64_t rows, cols, m, n; };
 
@@ -1303,21 +1431,38 @@ double update_scale(const Update& u, int64_t rows, int64_t cols)
     return u.scale == MP_MUON_SCALE_MATCH_RMS ? 0.2 * sqrt(r > c ? r : c) : u.scale == MP_MUON_SCALE_ORIGINAL ? sqrt(r > c ? r / c : 1.0) : 1.0;
 }
 
-// LDS that ns_small_kernel needs for a matrix; 0: it is not for it
-size_t small_lds(int64_t rows, int64_t cols)
+// Which of the one-launch kernels a matrix is for: TINY_2 / TINY_8 (ns_tiny_kernel with that many columns a thread), SMALL_1 / SMALL_2 (blocks of
+// 32 rows in ns_small_kernel; lds: what it needs), or none
+enum Kind { NOT_SMALL, TINY_2, TINY_8, SMALL_1, SMALL_2 };
+Kind kind_of(int64_t rows, int64_t cols, size_t* lds = nullptr)
 {
     const Shape s = shape_of(rows, cols);
-    if (s.m > 64 || s.n > 1024) return 0;
+    if (s.m <= TINY_M && s.n <= 8 * TINY_THREADS) return s.n <= 2 * TINY_THREADS ? TINY_2 : TINY_8;
+    if (s.m > 64 || s.n > 1024) return NOT_SMALL;
     const int mb = chunks(s.m), npc = chunks(s.n);
-    const size_t lds = (size_t)32 * mb * 128 * npc + small_s(mb) + 256;
-    return npc <= 8 * small_nb(mb) && lds <= SMALL_LDS ? lds : 0;
+    const size_t need = (size_t)32 * mb * 128 * npc + small_s(mb) + 256;
+    if (npc > 8 * small_nb(mb) || need > SMALL_LDS) return NOT_SMALL;
+    if (lds) *lds = need;
+    return mb == 1 ? SMALL_1 : SMALL_2;
 }
 
 bool all_small(int64_t count, const int64_t* rows, const int64_t* cols)
 {
     for (int64_t i = 0; i < count; ++i)
-        if (rows[i] > 0 && cols[i] > 0 && !small_lds(rows[i], cols[i])) return false;
+        if (rows[i] > 0 && cols[i] > 0 && kind_of(rows[i], cols[i]) == NOT_SMALL) return false;
     return true;
+}
+
+template <int NC>
+int launch_tiny(const Smalls& a, int dtype, double flops, double bytes, hipStream_t stream)
+{
+#define NS_TINY(DT) MP_LAUNCH("ns_tiny_kernel", flops, bytes, (ns_tiny_kernel<NC, DT>), dim3((unsigned)a.count), dim3(TINY_THREADS), 0, stream, a)
+    if (dtype == MP_DTYPE_F32) NS_TINY(MP_DTYPE_F32);
+    else if (dtype == MP_DTYPE_F16) NS_TINY(MP_DTYPE_F16);
+    else NS_TINY(MP_DTYPE_BF16);
+#undef NS_TINY
+    MP_CHECK_LAUNCH();
+    return MP_OK;
 }
 
 template <int MB, int DT>
@@ -1337,7 +1482,7 @@ int launch_small_of(const Smalls& a, int dtype, double flops, double bytes, size
     return launch_small<MB, MP_DTYPE_BF16>(a, flops, bytes, lds, stream);
 }
 
-// one launch for the matrices of each number of 32-row blocks
+// one launch for the matrices of each kind
 int run_small(int64_t count, const void* const* in, void* const* out, float* const* mom, const int64_t* rows, const int64_t* cols, int dtype, int steps,
               const double* coef, double eps, const Bounds& bd, const Update& u, hipStream_t stream)
 {
@@ -1345,14 +1490,14 @@ int run_small(int64_t count, const void* const* in, void* const* out, float* con
     a.nesterov = u.nesterov; a.update = u.on; a.steps = steps;
     a.mu = (float)u.mu; a.a = (float)coef[0]; a.b = (float)coef[1]; a.c = (float)coef[2]; a.eps = eps;
     a.sX = pow2_scale(bd.x); a.sA = pow2_scale(bd.x * bd.x); a.sQ = pow2_scale(bd.q);
-    for (int mb = 1; mb <= 2; ++mb)
+    for (int kind = TINY_2; kind <= SMALL_2; ++kind)
         for (int64_t i = 0; i < count;) {
             size_t lds = 0;
             double elems = 0.0, flops = 0.0;
             for (a.count = 0; i < count && a.count < MAX_SMALL; ++i) {
                 const Shape s = shape_of(rows[i], cols[i]);
-                if (s.m <= 0 || chunks(s.m) != mb) continue;
-                const size_t need = small_lds(rows[i], cols[i]);
+                size_t need = 0;
+                if (s.m <= 0 || kind_of(rows[i], cols[i], &need) != kind) continue;
                 lds = need > lds ? need : lds;
                 a.m[a.count++] = Small{in[i], mom ? mom[i] : nullptr, out[i], (int)rows[i], (int)cols[i], (float)(u.lr * update_scale(u, rows[i], cols[i])),
                                        (float)(1.0 - u.lr * u.decay)};
@@ -1360,7 +1505,10 @@ int run_small(int64_t count, const void* const* in, void* const* out, float* con
                 flops += 6.0 * steps * s.m * s.m * (2.0 * s.n + s.m);
             }
             if (a.count == 0) break;
-            const int rc = mb == 1 ? launch_small_of<1>(a, dtype, flops, elems * 8.0, lds, stream) : launch_small_of<2>(a, dtype, flops, elems * 8.0, lds, stream);
+            const int rc = kind == TINY_2    ? launch_tiny<2>(a, dtype, flops, elems * 8.0, stream)
+                           : kind == TINY_8  ? launch_tiny<8>(a, dtype, flops, elems * 8.0, stream)
+                           : kind == SMALL_1 ? launch_small_of<1>(a, dtype, flops, elems * 8.0, lds, stream)
+                                             : launch_small_of<2>(a, dtype, flops, elems * 8.0, lds, stream);
             if (rc) return rc;
         }
     return MP_OK;

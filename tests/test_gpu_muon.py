@@ -315,3 +315,35 @@ def test_offsets_beyond_32_bits(ops):
     del g
     (out,) = ops.orthogonalize([tall])
     assert float((out[cols].t().double() - want).norm()) <= tol
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(1, 2), (8, 8), (3, 5), (8, 1024), (1024, 8), (7, 1025), (1025, 7), (5, 2000), (1, 4096), (4096, 8), (8, 4096),
+                                       (8, 4097), (4097, 3), (9, 500), (500, 9), (32, 1000), (1000, 20)])
+def test_thin_matrices(ops, rows, cols, dtype):
+    """both sides of the limits of the one-launch forms for up to 8, 32 and 64 rows, alone and in one list"""
+    dirty()
+    g = make(rows, cols, dtype, 4)
+    other = make(cols, rows, dtype, 5)
+    for got, want in zip(ops.orthogonalize([g]) + ops.orthogonalize([other, g, make(40, 60, dtype, 6)]), (g, other, g, make(40, 60, dtype, 6))):
+        check(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_step_of_small_matrices(ops, dtype, nesterov):
+    """lists that take the one-launch forms only: update and momentum as in test_muon_step, same tolerances"""
+    u = 2.0 ** -24
+    shapes = [(64, 3, 1, 1), (64, 64, 1, 1), (5, 100), (100, 5), (8, 4096), (3000, 7), (33, 200), (1, 1), (200, 40), (20, 900)]
+    ps = [torch.randn(s, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)).to(dtype) for i, s in enumerate(shapes)]
+    gs = [make(s[0], p.numel() // s[0], dtype, 6).view(s) for s, p in zip(shapes, ps)]
+    ms = [make(s[0], p.numel() // s[0], torch.float32, 7).view(s) for s, p in zip(shapes, ps)]
+    for _ in range(2):
+        want = [muon_reference(p, g, m, 0.05, 0.9, nesterov, 0.1, "original") for p, g, m in zip(ps, gs, ms)]
+        old = [m.clone() for m in ms]
+        ops.muon_step(ps, gs, ms, lr=0.05, momentum=0.9, nesterov=nesterov, weight_decay=0.1)
+        for p, g, m, o, w in zip(ps, gs, ms, old, want):
+            assert ((m.double().cpu() - w[1]).abs() <= 4 * u * (g.double().abs().cpu() + o.double().abs().cpu())).all()
+            tol_o, h = tolerance(w[3], w[4], torch.float32), torch.finfo(dtype).eps / 2
+            err = (p.double().cpu() - w[0]).norm()
+            assert float(err) <= w[2] * (tol_o + 4 * u * float(w[3].norm())) + (4 * u + h) * float(w[0].norm() + w[2] * w[3].norm()) + torch.finfo(dtype).tiny
