@@ -615,7 +615,8 @@ int mp_layer_norm_bwd(const void* dy, int64_t dy_row_stride, const void* x, int6
  * (a matrix with more rows than columns: of its transpose, transposed back).  in / out are HOST arrays of `count` device pointers of
  * `dtype` (they travel in the kernel arguments), rows / cols / coefficients [3] HOST arrays; out[i] may be in[i] (no other overlap).
  * Products and sums in fp32 accuracy, one rounding at the end (16-bit types: the singular values' polynomial may be evaluated on the Gram
- * matrix; bf16: the last two steps' operands may be fp16; both add less than the result's own rounding).  The scalar recursion
+ * matrix, which adds less than the result's own rounding whatever the spectrum, for up to five steps of the usual coefficients; a further
+ * step multiplies by c0 what fp32 arithmetic leaves in directions that U does not have, in every type).  The scalar recursion
  * s <- |s (c0 + c1 s^2 + c2 s^4)| of the coefficients must keep s <= 16 from every start in [0, 1], steps <= 16,
  * min(rows, cols) <= 65536, max <= 2^21: else MP_EUNSUPPORTED.  Matrices without elements are skipped.  workspace: 256-byte aligned,
  * mp_orthogonalize_workspace_bytes bytes (of the same rows, cols, dtype and steps; 0 where all matrices are small: NULL will do), used by

@@ -45,8 +45,7 @@ struct Prob {                // out = (alpha acc + cb C + ca I), acc = L R^T ove
     int M, N, kc, oc, otc, rpow, sym, tiles_n, fin_t;
     float alpha, cb, ca, so, fmul, fdecay;
     int tiles, seg;          // tiles of the result; chunks of a segment of K (kc: not cut)
-    int ll : 8;              // the product of the l planes too (WITH_LL)  (bits: of bytes the scalar loads of the arguments know nothing)
-    int opl : 8, cpl : 8;    // planes of out / outT, of C
+    int ll;                  // the product of the l planes too
 };
 // A launch's work items, one a workgroup: the first `whole` tiles uncut, then the rest in segments of K.  Items are ordered by segment, then by
 // tile: neighbours share operand rows, not just the tile.  equal: all problems have one K, the rest is `rest` tiles x segments; else every
@@ -208,10 +207,10 @@ __device__ __forceinline__ unsigned planes_of(float x)
     __builtin_memcpy(&lb, &l, 2);
     return (unsigned)hb | ((unsigned)lb << 16);
 }
-// eight packed elements to the h and l runs of an image (16 bytes each), or to the h run alone
-__device__ __forceinline__ void put_packed(_Float16* img, int row, int nchunk, int col, int planes, const unsigned (&w)[8])
+// eight packed elements to the h and l runs of an image (16 bytes each)
+__device__ __forceinline__ void put_packed(_Float16* img, int row, int nchunk, int col, const unsigned (&w)[8])
 {
-    _Float16* o = img + ((size_t)row * nchunk + (col >> 5)) * (32 * planes) + (col & 31);
+    _Float16* o = img + ((size_t)row * nchunk + (col >> 5)) * 64 + (col & 31);
     uint4v h, l;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -219,7 +218,7 @@ __device__ __forceinline__ void put_packed(_Float16* img, int row, int nchunk, i
         l[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302);
     }
     *reinterpret_cast<uint4v*>(o) = h;
-    if (planes == 2) *reinterpret_cast<uint4v*>(o + 32) = l;
+    *reinterpret_cast<uint4v*>(o + 32) = l;
 }
 constexpr int TPAD = 4;      // a tile's rows in LDS are TN + 4 floats apart: 16-byte pieces, columns spread over the banks
 
@@ -249,8 +248,8 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= alpha;
         if (p.C && row < p.M && col < padN) {
-            const half8* c = reinterpret_cast<const half8*>(p.C + ((size_t)row * p.oc + (col >> 5)) * (32 * p.cpl) + (col & 31));
-            const half8 h = c[0], l = p.cpl == 2 ? c[4] : half8{0, 0, 0, 0, 0, 0, 0, 0};
+            const half8* c = reinterpret_cast<const half8*>(p.C + ((size_t)row * p.oc + (col >> 5)) * 64 + (col & 31));
+            const half8 h = c[0], l = c[4];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += cb * ((float)h[e] + (float)l[e]);
         }
@@ -277,7 +276,7 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
         wt[0] = uint4v{w[0], w[1], w[2], w[3]};
         wt[1] = uint4v{w[4], w[5], w[6], w[7]};
         // a symmetric result takes its lower half in pieces of 8 x 8: those below the diagonal here and, mirrored, in the second pass
-        if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) put_packed(p.out, row, p.oc, col, p.opl, w);
+        if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) put_packed(p.out, row, p.oc, col, w);
     }
     if (p.fin && !p.fin_t) return;
     lds_barrier();          // (not __syncthreads: it would wait for the stores above)
@@ -302,7 +301,7 @@ __device__ __forceinline__ void epilogue(const Probs& a, const Prob& p, float* t
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = row + e < col ? d[e] : w[e];
         }
-        put_packed(p.outT, col, p.otc, row, p.opl, w);
+        put_packed(p.outT, col, p.otc, row, w);
     }
 }
 
@@ -329,9 +328,9 @@ __device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, cons
                     const int row = m0 + wm + 32 * x + 8 * g + 4 * fh;
                     ch[g] = cl4[g] = half4{0, 0, 0, 0};
                     if (col < p.N && row < padM) {
-                        const _Float16* c = p.C + ((size_t)col * p.oc + (row >> 5)) * (32 * p.cpl) + (row & 31);
+                        const _Float16* c = p.C + ((size_t)col * p.oc + (row >> 5)) * 64 + (row & 31);
                         ch[g] = *reinterpret_cast<const half4*>(c);
-                        if (p.cpl == 2) cl4[g] = *reinterpret_cast<const half4*>(c + 32);
+                        cl4[g] = *reinterpret_cast<const half4*>(c + 32);
                     }
                 }
 #pragma unroll
@@ -352,7 +351,7 @@ __device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, cons
         if (row < p.M && col < padN && (!p.sym || row >> 3 > col >> 3)) {
             const uint4v lo = *reinterpret_cast<const uint4v*>(t + rl * S + cl), hi = *reinterpret_cast<const uint4v*>(t + rl * S + cl + 4);
             const unsigned w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            put_packed(p.out, row, p.oc, col, p.opl, w);
+            put_packed(p.out, row, p.oc, col, w);
         }
     }
 #pragma unroll 4
@@ -367,7 +366,7 @@ __device__ __forceinline__ void epilogue_planes(const Prob& p, unsigned* t, cons
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = row + e < col ? d[e] : w[e];
             }
-            put_packed(p.outT, col, p.otc, row, p.opl, w);
+            put_packed(p.outT, col, p.otc, row, w);
         }
     }
 }
@@ -382,11 +381,8 @@ template <int PL> __device__ __forceinline__ int swz(int row) { return PL == 2 ?
 // KW: the four waves share a (32 WM) x (32 WN) tile by K instead, wave v taking chunks v, v + 4, ..: each with a ring of its own and no
 // meeting at all; their sums meet in LDS at the end, added in the order of the waves.  For 64 x 64 tiles, where a wave of the shared form has
 // three products between two meetings (136 tiles of K = 1024: 15.2 us shared, 12.7 this way).
-// MODE: PLAIN; WITH_LL: products of the l planes too, for the problems that ask for them; PAIRS: images of one plane with an even number of chunks,
-// two of them where the others have h and l -- the same loads, reads and meetings, products h h and l l.  (A chunk of one plane has too few
-// matrix instructions between two meetings: 8 of 2048 x 2048, X <- Q X: 250 us chunk by chunk, 222 in pairs.)
-enum Mode { PLAIN, WITH_LL, PAIRS };
-template <int WM, int WN, int PL, int PR, int NS, bool KW, int MODE>
+// LL: products of the l planes too, for the problems that ask for them.
+template <int WM, int WN, int PL, int PR, int NS, bool KW, bool LL>
 __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 {
     constexpr int WAVES = KW ? 1 : 4;                              // waves that load a stage together
@@ -461,7 +457,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 
         const int rowL = wm + fr, rowR = wn + fr;        // (32 rows on: the same swizzle)
         half8 fl[2][WM][PL], fq[2][WN][PR];
-        constexpr int READS = WM * PL + WN * PR, PRODS = (MODE == PAIRS ? 2 : PL + PR - 1) * WM * WN, FETCHES = NL + NR;
+        constexpr int READS = WM * PL + WN * PR, PRODS = (PL + PR - 1) * WM * WN, FETCHES = NL + NR;
         auto read_one = [&](int buf, int ks, int k) {
             const char* s = ring + buf * STAGE;
             if (k < WM * PL) {
@@ -475,7 +471,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
         // The PRODS matrix instructions of 16 k, the small products first, a block's WM * WN apart; in the shadow of each (32 cycles) go its
         // share of the reads of the other half's fragments and of the loads of a chunk to come: with one wave a SIMD nothing else fills it.
         auto multiply = [&](int ks, bool reads, int rbuf, bool fetches, int fbuf) {
-            if constexpr (MODE == WITH_LL)        // (a question of its own kernel: asked in all of them it costs 1 % of a small launch)
+            if constexpr (LL)        // (a question of its own kernel: asked in all of them it costs 1 % of a small launch)
                 if (p.ll)
 #pragma unroll
                     for (int g = 0; g < WM * WN; ++g)
@@ -483,7 +479,7 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 #pragma unroll
             for (int g = 0; g < PRODS; ++g) {
                 const int k = g / (WM * WN), x = g / WN % WM, y = g % WN;
-                const int pl = MODE == PAIRS ? k : PL == 2 && k == 0 ? 1 : 0, pr = MODE == PAIRS ? k : PR == 2 && k == PL - 1 ? 1 : 0;
+                const int pl = PL == 2 && k == 0 ? 1 : 0, pr = PR == 2 && k == PL - 1 ? 1 : 0;
                 acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][pl], fq[ks][y][pr], acc[x][y], 0, 0, 0);
                 if (reads)
 #pragma unroll
@@ -1202,48 +1198,37 @@ int hop_cap(const Shape& s, int steps, int dtype, double g)
     return h;
 }
 
-// Steps at the end that run one by one on one plane, h alone, where that is cheaper: bf16 only, two.  The singular values are within a factor
-// of a few of 1 by then, nothing grows any more: whatever the spectrum it adds 4e-4 (one step) to 8e-4 (two; three: up to 2e-3) to the
-// result's own rounding of 1.7e-3 (8 of 2048 x 2048: 4180 us without, 3460 with two).  Other coefficients: while |Q| and |X| stay as small.
-constexpr int MAX_TAIL = 2;
-int tail_cap(int steps, int dtype, const Bounds& b) { return dtype == MP_DTYPE_BF16 && steps > MAX_TAIL && b.q <= 4.0 && b.x <= 2.0 ? MAX_TAIL : 0; }
-
-// -> tail.  work: operations of plane products, at 0.4 PFLOP/s (1024 x 1024 x 1024 reach 0.25, large ones 1.0)
-int plan_hops(const Shape* s, int k, int steps, int dtype, int planes, const Bounds& bd, int* hop)
+// work: operations of plane products, at 0.4 PFLOP/s (1024 x 1024 x 1024 reach 0.25, large ones 1.0)
+void plan_hops(const Shape* s, int k, int steps, int dtype, int planes, const Bounds& bd, int* hop)
 {
     const double g = bd.q * bd.q;
     double best = 1e300;
-    int best_tail = 0;
-    for (int tail = 0; tail <= tail_cap(steps, dtype, bd); tail += MAX_TAIL)
-        for (int h = 1; h <= steps - tail; ++h) {
-            int use[MAX_MAT];
-            bool more = h == 1;
-            double work = 0.0;
-            int launches = 0;
-            for (int q = 0; q < k; ++q) {
-                int mine = 2 + 3 * tail;
-                const int cap = hop_cap(s[q], steps - tail, dtype, g);
-                use[q] = h < cap ? h : cap;
-                more = more || use[q] == h;
-                const double m = (double)s[q].m, n = (double)s[q].n;
-                for (int left = steps - tail; left > 0; left -= use[q]) {
-                    const int len = left < use[q] ? left : use[q];
-                    // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
-                    work += m * m * ((left == steps - tail && planes == 1 ? 1.0 + 2.0 * 2.0 : 3.0 * 3.0) * n + 3.0 * (4.0 * len - 3.0) * m);
-                    mine += len == 1 ? 3 : 3 * len + 1;       // Gram, apply; Q a step; T (and R), A between steps; R behind the last
-                }
-                work += tail * m * m * (3.0 * n + m);
-                launches = mine > launches ? mine : launches;
+    for (int h = 1; h <= steps; ++h) {
+        int use[MAX_MAT];
+        bool more = h == 1;
+        double work = 0.0;
+        int launches = 0;
+        for (int q = 0; q < k; ++q) {
+            int mine = 2;
+            const int cap = hop_cap(s[q], steps, dtype, g);
+            use[q] = h < cap ? h : cap;
+            more = more || use[q] == h;
+            const double m = (double)s[q].m, n = (double)s[q].n;
+            for (int left = steps; left > 0; left -= use[q]) {
+                const int len = left < use[q] ? left : use[q];
+                // (the first hop of a one-plane matrix: one product for the Gram matrix, two for the last one)
+                work += m * m * ((left == steps && planes == 1 ? 1.0 + 2.0 * 2.0 : 3.0 * 3.0) * n + 3.0 * (4.0 * len - 3.0) * m);
+                mine += len == 1 ? 3 : 3 * len + 1;       // Gram, apply; Q a step; T (and R), A between steps; R behind the last
             }
-            if (!more) break;        // (no matrix may take that many)
-            const double cost = work / 0.4e15 + launches * 6.5e-6;
-            if (cost < best * 0.999) {
-                best = cost;
-                best_tail = tail;
-                for (int q = 0; q < k; ++q) hop[q] = use[q];
-            }
+            launches = mine > launches ? mine : launches;
         }
-    return best_tail;
+        if (!more) break;        // (no matrix may take that many)
+        const double cost = work / 0.4e15 + launches * 6.5e-6;
+        if (cost < best * 0.999) {
+            best = cost;
+            for (int q = 0; q < k; ++q) hop[q] = use[q];
+        }
+    }
 }
 
 size_t up(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -1343,15 +1328,15 @@ Plan plan_of(const Prob* p, int count, int products)
     return best;
 }
 
-template <int WM, int WN, int PL, int PR, int NS, bool KW, int MODE>
+template <int WM, int WN, int PL, int PR, int NS, bool KW, bool LL>
 int launch_ring(const Probs& a, double flops, hipStream_t stream)
 {
     static mp::DynLds dyn;
     constexpr int TM = KW ? 32 * WM : 64 * WM, TN = KW ? 32 * WN : 64 * WN, RINGS = KW ? 4 : 1;
     constexpr size_t ring = (size_t)RINGS * NS * 64 * (TM * PL + TN * PR), tile = (size_t)RINGS * TM * (TN + TPAD) * sizeof(float);
     constexpr size_t smem = ring > tile ? ring : tile;
-    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW, MODE>), smem)) return MP_ELAUNCH;
-    MP_LAUNCH("ns_gemm_kernel", flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW, MODE>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
+    if (!dyn.ensure(reinterpret_cast<const void*>(&ns_gemm_kernel<WM, WN, PL, PR, NS, KW, LL>), smem)) return MP_ELAUNCH;
+    MP_LAUNCH("ns_gemm_kernel", flops, 0.0, (ns_gemm_kernel<WM, WN, PL, PR, NS, KW, LL>), dim3((unsigned)a.items), dim3(256), smem, stream, a);
     MP_CHECK_LAUNCH();
     if (a.whole < a.tiles) {
         MP_LAUNCH("ns_join_kernel", 0.0, 0.0, (ns_join_kernel<TM, TN>), dim3((unsigned)(a.tiles - a.whole) * (TM / 32)), dim3(256), 0, stream, a);
@@ -1362,29 +1347,25 @@ int launch_ring(const Probs& a, double flops, hipStream_t stream)
 
 // Depth of the ring: what 144 KB hold (at most 8 chunks) where the launch has one workgroup a CU at most, else half of that so that two
 // share a CU (256 x 128 and the K-sharing 64 x 64: always one).
-template <int WM, int WN, int PL, int PR, bool KW, int MODE>
+template <int WM, int WN, int PL, int PR, bool KW>
 int launch_as(const Probs& a, double flops, hipStream_t stream)
 {
     constexpr int lds = 147456, stage = KW ? 4 * 64 * 32 * (WM * PL + WN * PR) : 64 * 64 * (WM * PL + WN * PR);
     constexpr int deep = lds / stage < 8 ? lds / stage : 8, half = KW || WM * WN >= 8 ? deep : (lds / 2 / stage < 8 ? lds / 2 / stage : 8);
-    if constexpr (KW && PL == 2 && PR == 2 && MODE == PLAIN) {
+    if constexpr (KW && PL == 2 && PR == 2) {
         bool ll = false;
         for (int i = 0; i < a.count; ++i) ll = ll || a.p[i].ll;
-        if (ll) return launch_ring<WM, WN, PL, PR, deep, KW, WITH_LL>(a, flops, stream);
+        if (ll) return launch_ring<WM, WN, PL, PR, deep, KW, true>(a, flops, stream);
     }
-    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW, MODE>(a, flops, stream);
-    return launch_ring<WM, WN, PL, PR, half, KW, MODE>(a, flops, stream);
+    if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW, false>(a, flops, stream);
+    return launch_ring<WM, WN, PL, PR, half, KW, false>(a, flops, stream);
 }
 
 // planes of the left and the right operands: (2, 2), (2, 1) or (1, 1)
 int launch(Probs& a, int left, int right, hipStream_t stream)
 {
     if (a.count == 0) return MP_OK;
-    bool pairs = left == 1 && right == 1;
-    for (int i = 0; i < a.count; ++i) pairs = pairs && a.p[i].kc % 2 == 0;
-    if (pairs)
-        for (int i = 0; i < a.count; ++i) a.p[i].kc /= 2;
-    const int products = pairs ? 2 : left + right - 1;
+    const int products = left + right - 1;
     const Plan pl = plan_of(a.p, a.count, products);
     const TileShape ts = SHAPES[pl.shape];
     if (pl.shape < 0) return MP_EUNSUPPORTED;
@@ -1411,15 +1392,14 @@ int launch(Probs& a, int left, int right, hipStream_t stream)
     if (a.whole == a.tiles) items = tiles;
     else if (a.equal) items = a.whole + (int64_t)a.rest * ((a.p[0].kc + a.p[0].seg - 1) / a.p[0].seg);
     a.items = (int)items;
-#define NS_SHAPES(PL, PR, MODE)                                                     \
-    return pl.shape == 0   ? launch_as<4, 2, PL, PR, false, MODE>(a, flops, stream) \
-           : pl.shape == 1 ? launch_as<2, 2, PL, PR, false, MODE>(a, flops, stream) \
-           : pl.shape == 2 ? launch_as<2, 2, PL, PR, true, MODE>(a, flops, stream)  \
-                           : launch_as<1, 1, PL, PR, true, MODE>(a, flops, stream)
-    if (left == 2 && right == 2) NS_SHAPES(2, 2, PLAIN);
-    if (left == 2) NS_SHAPES(2, 1, PLAIN);
-    if (pairs) NS_SHAPES(2, 2, PAIRS);
-    NS_SHAPES(1, 1, PLAIN);
+#define NS_SHAPES(PL, PR)                                                     \
+    return pl.shape == 0   ? launch_as<4, 2, PL, PR, false>(a, flops, stream) \
+           : pl.shape == 1 ? launch_as<2, 2, PL, PR, false>(a, flops, stream) \
+           : pl.shape == 2 ? launch_as<2, 2, PL, PR, true>(a, flops, stream)  \
+                           : launch_as<1, 1, PL, PR, true>(a, flops, stream)
+    if (left == 2 && right == 2) NS_SHAPES(2, 2);
+    if (left == 2) NS_SHAPES(2, 1);
+    NS_SHAPES(1, 1);
 #undef NS_SHAPES
 }
 
@@ -1561,7 +1541,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     int64_t blocks = 0, tiles = 0;
     double elems = 0.0;
     for (int q = 0; q < k; ++q) sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
-    const int body = steps - plan_hops(sh, k, steps, dtype, a.planes, bd, hop);
+    plan_hops(sh, k, steps, dtype, a.planes, bd, hop);
     for (int q = 0; q < k; ++q) {
         ws += layout(sh[q], steps, dtype, ws, &bf[q]);
         Mat& m = a.m[q];
@@ -1608,7 +1588,6 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
         int done, len, s, r, q;      // steps behind it, steps of this hop, step inside it, which P holds R / Q
         float sR;
         bool first;                  // X is still the input's planes (to be multiplied by r)
-        int xpl;                     // planes of X
     } w[MAX_MAT];
     Probs g;
     g.fin_dtype = dtype;
@@ -1624,17 +1603,13 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
         p.sym = 1;
         p.alpha = 1.0f / (sl * sr);
         p.so = so;
-        p.opl = p.cpl = w[q].done < body ? 2 : 1;
         return p;
     };
-    for (int q = 0; q < k; ++q) w[q] = Walk{GRAM, 0, body < hop[q] ? body : hop[q], 0, 0, 0, sQ, true, a.planes};
+    for (int q = 0; q < k; ++q) w[q] = Walk{GRAM, 0, steps < hop[q] ? steps : hop[q], 0, 0, 0, sQ, true};
     for (;;) {
         bool more = false;
-        int planes[MAX_MAT];        // of the operands: 0 (2, 2), 1 (1, 1), 2 (2, 1)
-        for (int q = 0; q < k; ++q) {
-            const int apl = w[q].done < body ? 2 : 1, left = w[q].at == GRAM ? w[q].xpl : apl, right = w[q].at == GRAM || w[q].at == APPLY ? w[q].xpl : apl;
-            planes[q] = left + right == 4 ? 0 : left == 1 ? 1 : 2;
-        }
+        int planes[MAX_MAT];        // of the operands: 0 (2, 2), 1 (1, 1), 2 (2, 1); one plane: the input's
+        for (int q = 0; q < k; ++q) planes[q] = w[q].first && a.planes == 1 ? (w[q].at == GRAM ? 1 : w[q].at == APPLY ? 2 : 0) : 0;
         for (int kind = 0; kind < 3; ++kind) {
             g.count = 0;
             for (int q = 0; q < k; ++q) {
@@ -1689,7 +1664,6 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                         p.oc = chunks(sh[q].n);
                         p.otc = chunks(sh[q].m);
                         p.so = sX;
-                        p.opl = v.xpl = v.done + v.len < body ? 2 : 1;
                         char* t = bf[q].XT;
                         bf[q].XT = bf[q].XT2;
                         bf[q].XT2 = t;
@@ -1708,7 +1682,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
             else if (v.at == NEXT) { ++v.s; v.at = SQUARE; }
             else if (v.at == APPLY) {
                 v.done += v.len;
-                v.len = v.done >= body ? (v.done < steps ? 1 : 0) : body - v.done < hop[q] ? body - v.done : hop[q];
+                v.len = steps - v.done < hop[q] ? steps - v.done : hop[q];
                 v.s = 0;
                 v.first = false;
                 v.at = v.len ? GRAM : END;

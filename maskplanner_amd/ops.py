@@ -1139,9 +1139,10 @@ def orthogonalize(matrices, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7):
     """Newton-Schulz orthogonalisation of every matrix G: X = G / max(|G|_F, eps), `steps` times X <- (a I + b A + c A^2) X with A = X X^T
     (of the transpose where G has more rows than columns): singular values go to about 1, singular vectors stay.  `matrices`: a list of 2-D
     tensors of one type (float32, float16, bfloat16; any sizes up to 65536 by 2^21; strided ones are copied) -> a list of new tensors, or one
-    tensor [..., m, n] -> one tensor.  All matrices go through each stage in one launch.  Products in fp32 accuracy, rounded once (bfloat16:
-    the last two steps in fp16's 11 bits where that is faster; they add less than the result's own rounding).  Not differentiable.  The
-    coefficients must keep s <- |s (a + b s^2 + c s^4)| <= 16 for starts in [0, 1]."""
+    tensor [..., m, n] -> one tensor.  All matrices go through each stage in one launch.  Products in fp32 accuracy, rounded once (16-bit
+    types: what the evaluation on the Gram matrix adds is less than the result's own rounding for up to five steps; a further step multiplies by
+    `a` what fp32 arithmetic leaves in directions that G does not have).  Not differentiable.  The coefficients must keep
+    s <- |s (a + b s^2 + c s^4)| <= 16 for starts in [0, 1]."""
     if torch.is_tensor(matrices):
         _need_hip(matrices)
         if matrices.ndim < 2:

@@ -1,0 +1,82 @@
+"""How exact 16-bit Newton-Schulz results are, over the spectra that weight gradients have: full rank, rank of a batch, one dominating direction.
+
+Tolerance.  A 16-bit result is off by its own rounding, r = |round(exact) - exact|_F, and by what the evaluation adds in front of it; the
+library states that this is less than r.  The two are independent (the rounding takes whatever value it is given), so they add in squares:
+    |out - exact|_F <= sqrt(2) r.
+r is formed from the exact result itself, 1e-3 (bfloat16) or 2e-4 (float16) of its norm: a wrong tile, a missing step or a zero is hundreds of
+times as far off, which every check asserts.  At most five steps: further ones multiply by 3.4 each what any fp32 arithmetic leaves in
+directions that the matrix does not have (2^-24 to begin with).  Below 256 elements r is a matter of luck: there half a step of every element is taken for it."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+COEF = (3.4445, -4.7750, 2.0315)
+HALF = [torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs an MI355X")
+    from maskplanner_amd import ops as O
+    return O
+
+
+def normal(*shape, seed):
+    return torch.randn(shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+def make(rows, cols, kind, dtype, seed=7):
+    """kind: "full", "dominated" (one direction 100 times the rest), "decay" (singular values like 1 / k), or the rank"""
+    k = min(rows, cols)
+    if kind == "full":
+        g = normal(rows, cols, seed=seed)
+    elif kind == "dominated":
+        g = normal(rows, 1, seed=seed) * normal(1, cols, seed=seed + 1) + 1e-2 * normal(rows, cols, seed=seed + 2)
+    elif kind == "decay":
+        g = (normal(rows, k, seed=seed) / torch.arange(1, k + 1, device="cuda")) @ normal(k, cols, seed=seed + 1)
+    else:
+        k = min(k, kind)
+        g = normal(rows, k, seed=seed) @ normal(k, cols, seed=seed + 1)
+    return (1e-3 * g).to(dtype)
+
+
+def exact(u, steps=5):
+    """float64, from the definition"""
+    u = u.double()
+    x = u.t().contiguous() if u.shape[0] > u.shape[1] else u
+    x = x / max(float(x.norm()), 1e-7)
+    for _ in range(steps):
+        a = x @ x.t().contiguous()
+        x = COEF[0] * x + (COEF[1] * a + COEF[2] * (a @ a)) @ x
+    return x.t().contiguous() if u.shape[0] > u.shape[1] else x
+
+
+def check(out, want, what):
+    dtype, norm = out.dtype, float(want.norm())
+    r = float((want.to(dtype).double() - want).norm()) if want.numel() >= 256 else torch.finfo(dtype).eps / 2 * norm
+    assert r <= 0.01 * norm, what
+    assert float((out.double() - want).norm()) <= 2 ** 0.5 * r, (what, float((out.double() - want).norm()) / r)
+
+
+def both_forms(ops, g, steps, what):
+    want = exact(g, steps)
+    check(ops.orthogonalize([g], steps=steps)[0], want, what)
+    p, m = torch.zeros_like(g), g.float()                     # the momentum is the gradient and stays so: p = -orthogonalize(g), rounded once
+    ops.muon_step([p], [g], [m], lr=1.0, scale=None, steps=steps)
+    check(-p, want, (what, "muon"))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("kind", ["full", "dominated", "decay", 1, 8, 32, 128])
+@pytest.mark.parametrize("rows,cols", [(16, 1100), (100, 300), (256, 512), (512, 512), (1024, 1024), (1500, 700), (300, 3000)])
+def test_spectra_of_gradients(ops, rows, cols, kind, dtype):
+    both_forms(ops, make(rows, cols, kind, dtype), 5, (rows, cols, kind, dtype))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("kind", ["full", "dominated", 1, 32])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4])
+def test_step_counts(ops, steps, kind, dtype):
+    for rows, cols in ((512, 512), (128, 131), (60, 60)):
+        both_forms(ops, make(rows, cols, kind, dtype), steps, (rows, cols, kind, dtype, steps))
