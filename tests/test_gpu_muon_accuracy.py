@@ -80,3 +80,39 @@ def test_spectra_of_gradients(ops, rows, cols, kind, dtype):
 def test_step_counts(ops, steps, kind, dtype):
     for rows, cols in ((512, 512), (128, 131), (60, 60)):
         both_forms(ops, make(rows, cols, kind, dtype), steps, (rows, cols, kind, dtype, steps))
+
+
+SIZES = [(1, 7), (9, 1), (3, 64), (31, 33), (32, 32), (63, 65), (64, 64), (65, 64), (100, 300), (300, 100), (128, 131), (128, 128), (129, 1000), (257, 255),
+         (2100, 65), (40, 9000), (640, 500), (8, 4096), (4097, 3), (9, 500), (1000, 20), (1500, 1700)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_sizes_alone_and_in_one_list(ops, dtype):
+    gs = [make(r, c, "full", dtype, 3 * i) for i, (r, c) in enumerate(SIZES)]
+    for size, g, out in zip(SIZES, gs, ops.orthogonalize(gs)):
+        want = exact(g)
+        check(out, want, (size, "list"))
+        check(ops.orthogonalize([g])[0], want, (size, "alone"))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("scale", ["original", "match_rms", None])
+def test_muon_step_with_everything(ops, dtype, nesterov, scale):
+    """Momentum of its own, decay and step factors: the weight is rounded once, r its rounding; what is added in front of it (momentum and
+    direction in fp32, the factors) is again less than the rounding, as the step is as large as the decayed weight here (lr s = 0.5, weights of
+    an orthogonal matrix's size).  The lists take the one-launch kernels (first) and the chain."""
+    for sizes in ([(64, 3), (64, 64), (5, 100), (8, 4096), (200, 40)], [(64, 64), (128, 131), (256, 128), (70, 500), (6, 1024), (512, 512)]):
+        gs = [make(r, c, "full", dtype, 3 * i) for i, (r, c) in enumerate(sizes)]
+        ms = [1e-3 * normal(r, c, seed=100 + i) for i, (r, c) in enumerate(sizes)]
+        ps = [(normal(r, c, seed=200 + i) / max(r, c) ** 0.5).to(dtype) for i, (r, c) in enumerate(sizes)]
+        old, before = [p.double() for p in ps], [m.double() for m in ms]
+        ops.muon_step(ps, gs, ms, lr=0.5, momentum=0.9, nesterov=nesterov, weight_decay=0.2, scale=scale)
+        for (r, c), p, g, m, p0, m0 in zip(sizes, ps, gs, ms, old, before):
+            gd = g.double()
+            mean = m0 + 0.1 * (gd - m0)
+            s = {"original": max(1.0, r / c) ** 0.5, "match_rms": 0.2 * max(r, c) ** 0.5, None: 1.0}[scale]
+            want = 0.9 * p0 - 0.5 * s * exact(gd + 0.9 * (mean - gd) if nesterov else mean)
+            check(p, want, (r, c, dtype, nesterov, scale))
+            # a difference, a product with a rounded factor, a sum: four roundings of the operands' size
+            assert ((m.double() - mean).abs() <= 4 * 2.0 ** -24 * (gd.abs() + m0.abs())).all()
