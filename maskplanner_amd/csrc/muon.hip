@@ -13,8 +13,9 @@
 // 22 to 24 bits), a product is h h + h l + l h accumulated in fp32 -- three products at the fp16 rate (2.5 PFLOP/s) against one at the
 // fp32 rate (0.16).  The power of two puts the largest entry below 2^15, so l keeps its bits down to entries of 2^-24 of that.
 // What the small singular values suffer from is an error of Q that is not one of A (they grow by up to a^5 = 485 meanwhile): b A and c A^2 are
-// formed of the same planes, and in fp32 up to m = 128, where sums of so few terms hide nothing, A^2 takes l l too (400 shapes up to 300 x 1000
-// in emulation, largest error: 2.8e-6 of the exact result with b A from the accumulators, 2.1e-6 from the planes, 1.3e-6 with l l).
+// formed of the same planes, and in fp32 below m = 128, where sums of so few terms hide nothing, A^2 takes l l too (400 shapes up to 300 x 1000
+// in emulation, largest error: 2.8e-6 of the exact result with b A from the accumulators, 2.1e-6 from the planes, 1.3e-6 with l l).  150 shapes
+// of m < 128 measured: rms 0.76e-6, listed with a 2048 x 2048 one 1.07e-6 (larger tiles: a sum is one chain, not four), fp32 products 1.49e-6.
 //
 // All matrices of a call (up to 12 at a time) go through each stage in ONE launch (problem list in the kernel arguments): five steps are 17 to
 // 19 launches whatever their number.  Operand image: row r = chunks of 32 k, each [h: 32 fp16][l: 32 fp16] (128 bytes); columns up to the
@@ -381,7 +382,8 @@ template <int PL> __device__ __forceinline__ int swz(int row) { return PL == 2 ?
 // KW: the four waves share a (32 WM) x (32 WN) tile by K instead, wave v taking chunks v, v + 4, ..: each with a ring of its own and no
 // meeting at all; their sums meet in LDS at the end, added in the order of the waves.  For 64 x 64 tiles, where a wave of the shared form has
 // three products between two meetings (136 tiles of K = 1024: 15.2 us shared, 12.7 this way).
-// LL: products of the l planes too, for the problems that ask for them.
+// LL: products of the l planes too, for the problems that ask for them, and the small products in sums of their own: beside h h they would lose
+// their last bits.
 template <int WM, int WN, int PL, int PR, int NS, bool KW, bool LL>
 __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
 {
@@ -447,13 +449,16 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
                 srcR += step * 64 * PR;
             }
         };
-        float16v acc[WM][WN];
+        float16v acc[WM][WN], low[LL ? WM : 1][LL ? WN : 1];
 #pragma unroll
         for (int x = 0; x < WM; ++x)
 #pragma unroll
             for (int y = 0; y < WN; ++y)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+                for (int r = 0; r < 16; ++r) {
+                    acc[x][y][r] = 0.0f;
+                    if constexpr (LL) low[x][y][r] = 0.0f;
+                }
 
         const int rowL = wm + fr, rowR = wn + fr;        // (32 rows on: the same swizzle)
         half8 fl[2][WM][PL], fq[2][WN][PR];
@@ -475,12 +480,15 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
                 if (p.ll)
 #pragma unroll
                     for (int g = 0; g < WM * WN; ++g)
-                        acc[g / WN][g % WN] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][g / WN][1], fq[ks][g % WN][1], acc[g / WN][g % WN], 0, 0, 0);
+                        low[g / WN][g % WN] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][g / WN][1], fq[ks][g % WN][1], low[g / WN][g % WN], 0, 0, 0);
 #pragma unroll
             for (int g = 0; g < PRODS; ++g) {
                 const int k = g / (WM * WN), x = g / WN % WM, y = g % WN;
                 const int pl = PL == 2 && k == 0 ? 1 : 0, pr = PR == 2 && k == PL - 1 ? 1 : 0;
-                acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][pl], fq[ks][y][pr], acc[x][y], 0, 0, 0);
+                float16v* to = &acc[x][y];
+                if constexpr (LL)
+                    if (pl + pr) to = &low[x][y];
+                *to = __builtin_amdgcn_mfma_f32_32x32x16_f16(fl[ks][x][pl], fq[ks][y][pr], *to, 0, 0, 0);
                 if (reads)
 #pragma unroll
                     for (int r = g * READS * 2 / PRODS; r < (g + 1) * READS * 2 / PRODS; ++r)        // (in the first half: in time for the next)
@@ -519,6 +527,11 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_kernel(Probs a)
             buf = next;
         }
         // (nobody reads the buffers any more: the last meeting was behind the last fragment reads)
+        if constexpr (LL)
+#pragma unroll
+            for (int x = 0; x < WM; ++x)
+#pragma unroll
+                for (int y = 0; y < WN; ++y) acc[x][y] += low[x][y];
         if constexpr (KW) lds_barrier();
         if constexpr (!KW)
             if (n == p.kc && !p.fin) {
@@ -1352,10 +1365,12 @@ int launch_as(const Probs& a, double flops, hipStream_t stream)
 {
     constexpr int lds = 147456, stage = KW ? 4 * 64 * 32 * (WM * PL + WN * PR) : 64 * 64 * (WM * PL + WN * PR);
     constexpr int deep = lds / stage < 8 ? lds / stage : 8, half = KW || WM * WN >= 8 ? deep : (lds / 2 / stage < 8 ? lds / 2 / stage : 8);
-    if constexpr (KW && PL == 2 && PR == 2) {
+    if constexpr (PL == 2 && PR == 2) {
         bool ll = false;
         for (int i = 0; i < a.count; ++i) ll = ll || a.p[i].ll;
-        if (ll) return launch_ring<WM, WN, PL, PR, deep, KW, true>(a, flops, stream);
+        // (in every tile shape: a small matrix keeps its product whatever else is in the list)
+        if (ll && a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW, true>(a, flops, stream);
+        if (ll) return launch_ring<WM, WN, PL, PR, half, KW, true>(a, flops, stream);
     }
     if (a.items <= CUS) return launch_ring<WM, WN, PL, PR, deep, KW, false>(a, flops, stream);
     return launch_ring<WM, WN, PL, PR, half, KW, false>(a, flops, stream);

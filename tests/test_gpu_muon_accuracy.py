@@ -116,3 +116,27 @@ def test_muon_step_with_everything(ops, dtype, nesterov, scale):
             check(p, want, (r, c, dtype, nesterov, scale))
             # a difference, a product with a rounded factor, a sum: four roundings of the operands' size
             assert ((m.double() - mean).abs() <= 4 * 2.0 ** -24 * (gd.abs() + m0.abs())).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 600), (600, 64), (32, 1100), (16, 2000)])
+def test_small_float32_squares_keep_the_low_planes_in_any_company(ops, rows, cols):
+    """A^2 of fewer than 128 rows takes the product of the low planes too, whatever tiles the launch has because of other matrices in it.  A case
+    that is exact in binary: rows of 2^-4 (1, 2^-6, 2^-6, 0, ..), eps = 1 above the norm, so X is the matrix itself; the entries of A are
+    2^-8 (1 + 2^-11), high plane 1, low plane 2^-11; those of A^2 are m 2^-16 (1 + 2^-10 + 2^-22) with the low planes' product, without it the
+    2^-22 is missing from the result X <- A^2 X (coefficients 0, 0, 1).
+    Tolerance, half of that: the last product sums m entries 1 + 2^-10 (high) and 2^-22 (low), 16 at a time.  fp32 steps are 2^-19 from 16 on,
+    2^-18 from 32 on; 16 low products are 2^-18, but where the matrix instruction adds them in two parts each part is half a step from 32 on
+    and may round away: for m = 64 the last two groups of four, 2 x 2^-18 of 64, or 2^-23 of the result; none for m <= 32."""
+    m = min(rows, cols)
+    g = torch.zeros(m, max(rows, cols), device="cuda")
+    g[:, 5] = 2.0 ** -4
+    g[:, 100] = g[:, 101] = 2.0 ** -10
+    gd = g.double()
+    a = gd @ gd.t().contiguous()
+    want = (a @ a) @ gd
+    assert torch.equal(want.float().double(), want)
+    if rows > cols:
+        g, want = g.t().contiguous(), want.t().contiguous()
+    for others in ([], [normal(2048, 2048, seed=99)], [normal(300, 3000, seed=98)], [normal(1024, 1024, seed=90), normal(150, 130, seed=91)]):
+        out = ops.orthogonalize([g] + others, steps=1, coefficients=(0.0, 0.0, 1.0), eps=1.0)[0]
+        assert ((out.double() - want).abs() <= 2.0 ** -23 * want).all(), [o.shape for o in others]
