@@ -613,7 +613,7 @@ struct Mat {
     const void* g;       // gradient / input [rows, cols]
     float* mom;          // momentum or NULL
     double* sums;        // partial sums of squares
-    float* r;            // X = (U 2^e) * r
+    float* r;            // X = (U 2^e) * r[0];  r[1] = r[0] t, r[2] = 1 / t (x_shift)
     _Float16* P;         // planes of U 2^e, [rows][chunks(cols)]
     _Float16* PT;        // of its transpose, [cols][chunks(rows)]
     int rows, cols, blocks;
@@ -622,7 +622,7 @@ struct Mats {
     int blk0[MAX_MAT], tile0[MAX_MAT];       // first workgroup of every matrix in ns_norm_kernel / ns_planes_kernel; behind the last: INT_MAX
     Mat m[MAX_MAT];
     int count, dtype, nesterov, planes;
-    float mu;
+    float mu, x_room;
     double eps;
 };
 static_assert(sizeof(Mats) <= 3584, "travels in the kernel arguments");
@@ -681,6 +681,20 @@ __device__ __forceinline__ void put_plane(_Float16* img, int row, int nchunk, in
     *reinterpret_cast<half4*>(img + ((size_t)row * nchunk + (col >> 5)) * 32 + (col & 31)) = h;
 }
 
+// A norm far below eps: X stays small through all steps, and planes scaled for |X| ~ 1 would lose it in fp16's subnormals (a norm of 1e-7 eps:
+// 3e-4 of the result, 1e-11 eps: all of it).  Behind the first hop the planes hold X t, t the largest power of two (one at least) that keeps
+// |X| t within the planes' bound in every step: x_room = that bound / the largest product of |Q|, which is what |X| grows by.
+__device__ __forceinline__ double x_shift(double norm, double denom, float x_room)
+{
+    const double v = (double)x_room * denom / norm;
+    int e = 0;
+    if (norm > 0.0 && v >= 2.0) {
+        (void)frexp(v < 1e36 ? v : 1e36, &e);         // v in [2^(e-1), 2^e)
+        --e;
+    }
+    return ldexp(1.0, e);
+}
+
 // 64 x 64 elements of a matrix into both plane images.  The power of two 2^e takes the norm into [2^13, 2^14): exact, and every entry
 // below 2^14; the division by the norm itself waits for the products' epilogues (r).  A 16-bit matrix without momentum is one plane: fp16
 // holds the 8 or 11 bits of an entry exactly (down to 2^-38 of the norm, where the polynomial's slope of 485 is still far below half a step).
@@ -704,7 +718,12 @@ __global__ __launch_bounds__(256) void ns_planes_kernel(Mats a)
     }
     const int local = blockIdx.x - a.tile0[i], tn = (m.cols + 63) / 64;
     const int r0 = (local / tn) * 64, c0 = (local % tn) * 64;
-    if (local == 0 && threadIdx.x == 0) *m.r = (float)(1.0 / ldexp(norm > a.eps || norm != norm ? norm : a.eps, e));
+    if (local == 0 && threadIdx.x == 0) {
+        const double denom = norm > a.eps || norm != norm ? norm : a.eps, r = 1.0 / ldexp(denom, e), t = x_shift(norm, denom, a.x_room);
+        m.r[0] = (float)r;
+        m.r[1] = (float)(r * t);
+        m.r[2] = (float)(1.0 / t);
+    }
     const int tc = (threadIdx.x & 15) * 4, tr = threadIdx.x >> 4;
 #pragma unroll
     for (int k = 0; k < 64; k += 16) {
@@ -759,7 +778,7 @@ struct Small {
 constexpr int MAX_SMALL = 64;
 struct Smalls {
     int count, nesterov, update, steps;
-    float mu, a, b, c, sX, sA, sQ;
+    float mu, a, b, c, sX, sA, sQ, x_room;
     double eps;
     Small m[MAX_SMALL];
 };
@@ -832,7 +851,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
         (void)frexp(norm, &e2);
         e2 = 14 - e2;
     }
-    const float r = (float)(1.0 / ldexp(norm > a.eps || norm != norm ? norm : a.eps, e2));
+    const double denom = norm > a.eps || norm != norm ? norm : a.eps, r = 1.0 / ldexp(denom, e2), shift = x_shift(norm, denom, a.x_room);
     unsigned xp[NB][MB][16];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -846,7 +865,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
             }
     __syncthreads();
 
-    float sx = r;           // X = planes * sx
+    float sx = (float)r, so = (float)(r * shift) * a.sX / a.sQ;           // X = planes * sx; so: from a product Q X to the next planes
     for (int step = 0; step < a.steps; ++step) {
         // (a zero the compiler does not know: it would keep the addresses of every access below in registers across the steps, and spill)
         int zero = 0;
@@ -986,7 +1005,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) xp[b][i][k] = planes_of(acc[i][k] * alpha * a.sX);
+                    for (int k = 0; k < 16; ++k) xp[b][i][k] = planes_of(acc[i][k] * so);
             } else {        // (the planes are not read any more)
 #pragma unroll
                 for (int i = 0; i < MB; ++i)
@@ -999,7 +1018,8 @@ __global__ __launch_bounds__(512) void ns_small_kernel(Smalls a)
             }
             }
         }
-        sx = 1.0f / a.sX;
+        sx = (float)(1.0 / shift) / a.sX;
+        so = 1.0f / a.sQ;
     }
     __syncthreads();
     for (int rr = wave; rr < m.rows; rr += 8)
@@ -1192,6 +1212,13 @@ float pow2_scale(double bound)      // largest power of two that keeps bound bel
     int e;
     (void)frexp(bound > 0.0 ? bound : 1.0, &e);
     return ldexpf(1.0f, 15 - e);
+}
+
+float x_room(const Bounds& b, int steps)        // (x_shift)
+{
+    double grow = 1.0;
+    for (int h = 1; h <= steps; ++h) grow = b.r[h] > grow ? b.r[h] : grow;
+    return (float)(b.x / grow);
 }
 
 // Steps a hop of every matrix of a chunk.  Allowed, with g = max |Q|^2 (a^2 = 11.9 for the usual coefficients) the growth of the smallest
@@ -1484,7 +1511,7 @@ int run_small(int64_t count, const void* const* in, void* const* out, float* con
     Smalls a;
     a.nesterov = u.nesterov; a.update = u.on; a.steps = steps;
     a.mu = (float)u.mu; a.a = (float)coef[0]; a.b = (float)coef[1]; a.c = (float)coef[2]; a.eps = eps;
-    a.sX = pow2_scale(bd.x); a.sA = pow2_scale(bd.x * bd.x); a.sQ = pow2_scale(bd.q);
+    a.sX = pow2_scale(bd.x); a.sA = pow2_scale(bd.x * bd.x); a.sQ = pow2_scale(bd.q); a.x_room = x_room(bd, steps);
     for (int kind = TINY_2; kind <= SMALL_2; ++kind)
         for (int64_t i = 0; i < count;) {
             size_t lds = 0;
@@ -1553,6 +1580,7 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
     Mats a;
     a.count = k; a.dtype = dtype; a.nesterov = up_.nesterov; a.mu = (float)up_.mu; a.eps = eps;
     a.planes = dtype != MP_DTYPE_F32 && !mom ? 1 : 2;
+    a.x_room = x_room(bd, steps);
     int64_t blocks = 0, tiles = 0;
     double elems = 0.0;
     for (int q = 0; q < k; ++q) sh[q] = shape_of(rows[idx[q]], cols[idx[q]]);
@@ -1634,7 +1662,8 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                 if (v.at == GRAM) {                   // A = X X^T
                     Prob p = sym_prob(q, bf[q].X, bf[q].X, v.first ? 1.0f : sX, v.first ? 1.0f : sX, bf[q].A, sA);
                     p.kc = chunks(sh[q].n);
-                    if (v.first) { p.rdev = bf[q].r; p.rpow = 2; }
+                    p.rdev = bf[q].r + (v.first ? 0 : 2);
+                    p.rpow = 2;
                     g.p[g.count++] = p;
                 } else if (v.at == SQUARE) {          // Q = a I + b A + c A^2
                     v.q = v.s == 0 ? 0 : (v.r + 1) % 3;
@@ -1665,8 +1694,9 @@ int run_chunk(const void* const* in, void* const* out, float* const* mom, const 
                     p.N = (int)sh[q].n;
                     p.kc = chunks(sh[q].m);
                     p.alpha = 1.0f / (v.sR * (v.first ? 1.0f : sX));
-                    if (v.first) { p.rdev = bf[q].r; p.rpow = 1; }
-                    if (v.done + v.len == steps) {
+                    const bool last = v.done + v.len == steps;
+                    if (v.first || last) { p.rdev = bf[q].r + (!v.first ? 2 : last ? 0 : 1); p.rpow = 1; }       // (between hops: planes to planes)
+                    if (last) {
                         p.fin = out[idx[q]];
                         p.fin_t = sh[q].rows > sh[q].cols;
                         if (up_.on) {

@@ -41,11 +41,11 @@ def make(rows, cols, kind, dtype, seed=7):
     return (1e-3 * g).to(dtype)
 
 
-def exact(u, steps=5):
+def exact(u, steps=5, eps=1e-7):
     """float64, from the definition"""
     u = u.double()
     x = u.t().contiguous() if u.shape[0] > u.shape[1] else u
-    x = x / max(float(x.norm()), 1e-7)
+    x = x / max(float(x.norm()), eps)
     for _ in range(steps):
         a = x @ x.t().contiguous()
         x = COEF[0] * x + (COEF[1] * a + COEF[2] * (a @ a)) @ x
@@ -140,3 +140,33 @@ def test_small_float32_squares_keep_the_low_planes_in_any_company(ops, rows, col
     for others in ([], [normal(2048, 2048, seed=99)], [normal(300, 3000, seed=98)], [normal(1024, 1024, seed=90), normal(150, 130, seed=91)]):
         out = ops.orthogonalize([g] + others, steps=1, coefficients=(0.0, 0.0, 1.0), eps=1.0)[0]
         assert ((out.double() - want).abs() <= 2.0 ** -23 * want).all(), [o.shape for o in others]
+
+
+@pytest.mark.parametrize("rows,cols", [(8, 20), (40, 50), (20, 900), (70, 90), (90, 70), (300, 900), (1000, 9)])
+def test_norms_far_below_eps(ops, rows, cols):
+    """X = G / eps is tiny and stays so: the steps multiply it by a each (A is next to nothing).  Half a step of X's planes (2^-23), a product and a
+    scale a step: 4 x 2^-23 x 5 = 2.4e-6 of the result, however small it is."""
+    for scale, eps in ((1e-12, 1e-3), (1e-14, 1e-7), (1e-16, 1e-7), (1e-20, 1e-7), (1e-24, 1e-7), (1e-3, 1e9), (1e-18, 1.0)):
+        g = scale * normal(rows, cols, seed=2)
+        want = exact(g, eps=eps)
+        got = [ops.orthogonalize([g], eps=eps)[0], ops.orthogonalize([g, normal(400, 300, seed=3)], eps=eps)[0]]
+        p, m = torch.zeros_like(g), g.clone()
+        ops.muon_step([p], [g], [m], lr=1.0, scale=None, eps=eps)
+        for out in got + [-p]:
+            assert float((out.double() - want).norm()) <= 2.4e-6 * float(want.norm()), (scale, eps)
+        h = g.to(torch.bfloat16)
+        check(ops.orthogonalize([h], eps=eps)[0], exact(h, eps=eps), (scale, eps))
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 50), (70, 90), (300, 900)])
+def test_norms_around_eps(ops, rows, cols):
+    """From |X| = 1 down to where the steps are linear.  A step is off by at most 2^-22 (1.4 x 13 + 8) of |X| (two steps on the Gram matrix), and what
+    it leaves grows by 485 at most, as X itself does at 0."""
+    for ratio in (2.0, 1.0, 0.3, 3e-2, 3e-3, 1e-3, 3e-4, 1e-5):
+        g = normal(rows, cols, seed=4)
+        g = g / g.norm() * 1e-7 * ratio
+        want = exact(g)
+        bound = 5 * 2.0 ** -22 * (1.4 * 13 + 8) * 485 * min(ratio, 1.0)
+        assert float((ops.orthogonalize([g])[0].double() - want).norm()) <= bound, ratio
+        h = g.to(torch.bfloat16)
+        check(ops.orthogonalize([h])[0], exact(h), ratio)
