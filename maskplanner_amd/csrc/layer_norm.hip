@@ -470,30 +470,36 @@ __global__ __launch_bounds__(256) void ln_param_grad_wide_kernel(const T* __rest
     part[(size_t)blockIdx.y * 2 * D + D + c] = ab;
 }
 
-// dw, db = sums of the n partial rows, fp64, in a fixed order: 16 columns x 64 row groups a workgroup, y: dw or db
+// dw, db = sums of the n partial rows, fp64, in a fixed order: 16 columns x 64 row groups a workgroup, then the next 16 that are nobody else's
+// (a grid has fewer than 2^32 threads: 2^26 columns at once were left unwritten); y: dw or db
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_param_reduce_kernel(const float* __restrict__ part, int n, int64_t D, W* __restrict__ dw, W* __restrict__ db)
 {
     __shared__ double acc[64][17];
     const int cl = threadIdx.x & 15, rg = threadIdx.x >> 4;
-    const int64_t c = (int64_t)blockIdx.x * 16 + cl;
     W* out = blockIdx.y ? db : dw;
-    double s = 0.0;
-    if (c < D && out) {
-        const float* p = part + blockIdx.y * D + c;
+    if (!out) return;
+    for (int64_t c0 = (int64_t)blockIdx.x * 16; c0 < D; c0 += (int64_t)gridDim.x * 16) {
+        const int64_t c = c0 + cl;
+        double s = 0.0;
+        if (c < D) {
+            const float* p = part + blockIdx.y * D + c;
 #pragma unroll 8
-        for (int k = rg; k < n; k += 64) s += (double)p[(size_t)k * 2 * D];
-    }
-    acc[rg][cl] = s;
-    __syncthreads();
-    for (int o = 32; o > 0; o >>= 1) {
-        if (rg < o) acc[rg][cl] += acc[rg + o][cl];
+            for (int k = rg; k < n; k += 64) s += (double)p[(size_t)k * 2 * D];
+        }
+        acc[rg][cl] = s;
+        __syncthreads();
+        for (int o = 32; o > 0; o >>= 1) {
+            if (rg < o) acc[rg][cl] += acc[rg + o][cl];
+            __syncthreads();
+        }
+        if (rg == 0 && c < D) out[c] = (W)(float)acc[0][cl];
         __syncthreads();
     }
-    if (rg == 0 && c < D && out) out[c] = (W)(float)acc[0][cl];
 }
 
 constexpr int LN_WIDE_PARTS = 64;
+constexpr int64_t LN_REDUCE_BLOCKS = 1 << 16;
 // up to here dw / db are summed row by row by one thread a column: no partial sums, no second launch (32 x 1024 fp32: 4 us against 4 + 3)
 constexpr int LN_FEW_ROWS = 64;
 
@@ -611,7 +617,9 @@ int ln_bwd(const void* dy, int64_t dys, const void* x, int64_t xs, int dtype, in
         MP_CHECK_LAUNCH();
     }
     if (pg) {      // (no rows: the sums are zero)
-        hipLaunchKernelGGL((ln_param_reduce_kernel<W>), dim3((unsigned)((D + 15) / 16), 2), dim3(1024), 0, stream, part, parts, D, (W*)dw, (W*)db);
+        const int64_t groups = (D + 15) / 16;
+        hipLaunchKernelGGL((ln_param_reduce_kernel<W>), dim3((unsigned)(groups < LN_REDUCE_BLOCKS ? groups : LN_REDUCE_BLOCKS), 2), dim3(1024), 0, stream,
+                           part, parts, D, (W*)dw, (W*)db);
         MP_CHECK_LAUNCH();
     }
     return MP_OK;
