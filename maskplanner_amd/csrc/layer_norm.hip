@@ -400,6 +400,7 @@ __global__ __launch_bounds__(256) void ln_bwd_few_kernel(const T* __restrict__ d
 }
 
 // ---- rows wider than the register form: one workgroup walks a row three times (twice from the caches) -------------------------------
+// A thread adds cols / 256 (or rows / 64) terms one after the other: in fp64, fp32 sums of 2^26 columns left y off by 1.7e-4.
 template <typename T, typename W>
 __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(const T* __restrict__ x, int64_t rows, int64_t D, int64_t xs, const W* __restrict__ w,
                                                           const W* __restrict__ b, float eps, T* __restrict__ y,
@@ -408,15 +409,17 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(const T* __restrict__ 
     __shared__ float buf[8];
     const int64_t r = blockIdx.x;
     const T* xr = x + r * xs;
-    float s[1] = {0.0f};
-    for (int64_t c = threadIdx.x; c < D; c += 256) s[0] += (float)xr[c];
+    double sum = 0.0;
+    for (int64_t c = threadIdx.x; c < D; c += 256) sum += (double)(float)xr[c];
+    float s[1] = {(float)sum};
     row_sum<256>(s, buf);
     const float mean = s[0] / (float)D;
-    s[0] = 0.0f;
+    sum = 0.0;
     for (int64_t c = threadIdx.x; c < D; c += 256) {
         const float d = (float)xr[c] - mean;
-        s[0] += d * d;
+        sum += (double)(d * d);
     }
+    s[0] = (float)sum;
     row_sum<256>(s, buf + 4);
     const float rstd = 1.0f / sqrtf(s[0] / (float)D + eps);
     if (threadIdx.x == 0 && mean_out) {
@@ -437,12 +440,13 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_kernel(const T* __restrict__ 
     const T* xr = x + r * xs;
     const T* gr = dy + r * dys;
     const float mean = mean_in[r], rstd = rstd_in[r];
-    float s[2] = {0.0f, 0.0f};
+    double sg = 0.0, sgz = 0.0;
     for (int64_t c = threadIdx.x; c < D; c += 256) {
         const float g = (float)gr[c] * (w ? (float)w[c] : 1.0f);
-        s[0] += g;
-        s[1] += g * (((float)xr[c] - mean) * rstd);
+        sg += (double)g;
+        sgz += (double)(g * (((float)xr[c] - mean) * rstd));
     }
+    float s[2] = {(float)sg, (float)sgz};
     row_sum<256>(s, buf);
     const float inv = 1.0f / (float)D, c1 = s[0] * inv, c2 = s[1] * inv;
     for (int64_t c = threadIdx.x; c < D; c += 256) {
@@ -460,14 +464,14 @@ __global__ __launch_bounds__(256) void ln_param_grad_wide_kernel(const T* __rest
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= D) return;
     const int64_t per = (rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
-    float aw = 0.0f, ab = 0.0f;
+    double aw = 0.0, ab = 0.0;
     for (int64_t r = r0; r < r1; ++r) {
         const float g = (float)dy[r * dys + c];
-        aw += g * (((float)x[r * xs + c] - mean_in[r]) * rstd_in[r]);
-        ab += g;
+        aw += (double)(g * (((float)x[r * xs + c] - mean_in[r]) * rstd_in[r]));
+        ab += (double)g;
     }
-    part[(size_t)blockIdx.y * 2 * D + c] = aw;
-    part[(size_t)blockIdx.y * 2 * D + D + c] = ab;
+    part[(size_t)blockIdx.y * 2 * D + c] = (float)aw;
+    part[(size_t)blockIdx.y * 2 * D + D + c] = (float)ab;
 }
 
 // dw, db = sums of the n partial rows, fp64, in a fixed order: 16 columns x 64 row groups a workgroup, then the next 16 that are nobody else's
