@@ -27,7 +27,8 @@ class _SegBase(nn.Module):
 
     def _build(self, in_channel, point_norm="batch"):
         """point_norm: what follows conv1..conv3.  "batch" (the reference's BatchNorm1d) or "layer": a layer norm over each point's features
-        (bn1..bn3 are layer_norm.LayerNorm): the same result for a cloud whatever else is in the batch, in training as in evaluation."""
+        (bn1..bn3 are layer_norm.LayerNorm): from the encoder's features on a cloud's result does not depend on the other clouds of the batch,
+        in training as in evaluation.  The encoder keeps its BatchNorm, whose statistics in training are the batch's."""
         if point_norm not in ("batch", "layer"):
             raise ValueError(f"point_norm is 'batch' or 'layer', not {point_norm!r}")
         self.point_norm = point_norm
