@@ -6,6 +6,7 @@ bookkeeping only -- all arithmetic on the hot path happens inside libmaskplanner
 a non-HIP tensor raises.
 """
 import ctypes
+import threading
 import weakref
 
 import torch
@@ -645,6 +646,7 @@ def knn(p1, p2, lengths1=None, lengths2=None, K=1):
 _REDUCE_COUNTERS = {}
 _RECORDED_COUNTERS = {}      # device -> [pool of zeros, next free index, earlier pools (recordings point into them)]
 _COUNTER_POOL = 4096
+_COUNTER_LOCK = threading.Lock()
 
 
 def _reduce_counter(device):
@@ -652,17 +654,19 @@ def _reduce_counter(device):
     and may share a counter; launches on two streams (evaluation metrics next to the training stream) must not, so eager launches
     get one counter per (device, stream).  Every launch recorded into a hipGraph gets a counter of its own: two graphs may replay at the same
     time on two streams.  They come from a pool of zeros that eager calls make and refill (the harness runs eager steps before it records), so
-    no allocation or fill lands inside a capture; a recording beyond the pool makes its counter inside the graph, cleared by every replay."""
+    no allocation or fill lands inside a capture; a recording beyond the pool makes its counter inside the graph, cleared by every replay.
+    A counter is never handed out twice (nobody tells when a graph is gone): 4 bytes a recorded launch are what a process pays."""
     capturing = torch.cuda.is_current_stream_capturing()
-    pool = _RECORDED_COUNTERS.get(device)
-    if not capturing and (pool is None or pool[1] > _COUNTER_POOL // 2):
-        pool = _RECORDED_COUNTERS[device] = [torch.zeros((_COUNTER_POOL,), dtype=torch.int32, device=device), 0,
-                                             [] if pool is None else pool[2] + [pool[0]]]
+    with _COUNTER_LOCK:            # two threads may record at once
+        pool = _RECORDED_COUNTERS.get(device)
+        if not capturing and (pool is None or pool[1] > _COUNTER_POOL // 2):
+            pool = _RECORDED_COUNTERS[device] = [torch.zeros((_COUNTER_POOL,), dtype=torch.int32, device=device), 0,
+                                                 [] if pool is None else pool[2] + [pool[0]]]
+        if capturing and pool is not None and pool[1] < _COUNTER_POOL:
+            pool[1] += 1
+            return pool[0][pool[1] - 1:pool[1]]
     if capturing:
-        if pool is None or pool[1] >= _COUNTER_POOL:
-            return torch.zeros((1,), dtype=torch.int32, device=device)
-        pool[1] += 1
-        return pool[0][pool[1] - 1:pool[1]]
+        return torch.zeros((1,), dtype=torch.int32, device=device)
     key = (device, torch.cuda.current_stream(device).cuda_stream)
     t = _REDUCE_COUNTERS.get(key)
     if t is None:
