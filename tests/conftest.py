@@ -32,3 +32,13 @@ def oracle():
     from oracle import oracle as O
     O.build()
     return O
+
+
+# Its bounds are fixed shares of losses that training noise reaches now and then: equal trainers, each alone in its process, have been 2.5 % apart
+# at the fourth step (both eager: 2.03 %), where it allows 2 %.  It runs last, so that a run that stops at the first failure has been through everything else by then;
+# test_gpu_two_trainers.py looks for the same couplings where there is no noise.
+NOISY = "test_two_training_steps_on_two_streams_of_one_process"
+
+
+def pytest_collection_modifyitems(items):
+    items.sort(key=lambda item: item.name == NOISY)
