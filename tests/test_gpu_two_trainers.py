@@ -58,3 +58,47 @@ def test_two_trainers_on_two_streams_each_as_alone():
         pair[s].check()
         assert pair[s]._graph is not None and [float(x) for x in losses[s]] == want[s][0], s
         close(gradients(pair[s]), want[s][1])
+
+
+MUON = dict(hidden_size=(128, 128), optimizer="muon")
+
+
+def momentum(ts):
+    return {i: ts.opt.muon.state[p]["momentum_buffer"].clone() for i, p in enumerate(ts.opt.muon.param_groups[0]["params"])}
+
+
+def test_replayed_muon_steps_see_the_gradients_of_their_own_step():
+    """momentum over nine steps of different dropout masks, eager against eager and replayed: a gradient of another step would stay in it"""
+    runs = []
+    for graph in (False, True):
+        ts = make(5, graph=graph, muon={"muon_lr": 0.0}, **MUON)
+        losses = [ts.step().clone() for _ in range(9)]
+        torch.cuda.synchronize()
+        assert (ts._graph is not None) == graph
+        runs.append(([float(x) for x in losses], momentum(ts), gradients(ts)))
+    assert runs[0][0] == runs[1][0] and len(set(runs[0][0])) == 9
+    close(runs[1][1], runs[0][1])
+    close(runs[1][2], runs[0][2])
+    last = runs[0][2]
+    first = make(5, graph=False, muon={"muon_lr": 0.0}, **MUON)
+    first.step()
+    other = gradients(first)
+    assert any(float((other[n] - g).norm()) > 0.1 * float(g.norm()) for n, g in last.items() if n.startswith("sa") and g.ndim > 1)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_muon_steps_of_the_trainer_are_muon_steps(graph):
+    """each step's update of the encoder's matrices, to the bit: ops.muon_step on what weights and momentum were before, with the step's gradients"""
+    from maskplanner_amd import ops
+    ts = make(6, graph=graph, muon={"muon_lr": 0.02, "weight_decay": 0.01}, **MUON)
+    ps = ts.opt.muon.param_groups[0]["params"]
+    ts.step()
+    for k in range(8):
+        torch.cuda.synchronize()
+        before, m = [p.detach().clone() for p in ps], [ts.opt.muon.state[p]["momentum_buffer"].clone() for p in ps]
+        ts.step()
+        torch.cuda.synchronize()
+        ops.muon_step(before, [p.grad for p in ps], m, lr=0.02, weight_decay=0.01)
+        for p, q, n in zip(ps, before, m):
+            assert torch.equal(p, q) and torch.equal(ts.opt.muon.state[p]["momentum_buffer"], n), k
+    assert (ts._graph is not None) == graph
