@@ -1409,8 +1409,8 @@ int launch(Probs& a, int left, int right, hipStream_t stream)
     if (a.count == 0) return MP_OK;
     const int products = left + right - 1;
     const Plan pl = plan_of(a.p, a.count, products);
-    const TileShape ts = SHAPES[pl.shape];
     if (pl.shape < 0) return MP_EUNSUPPORTED;
+    const TileShape ts = SHAPES[pl.shape];
     int64_t tiles = 0, items = pl.whole;
     double flops = 0.0;
     a.equal = 1;
