@@ -7,7 +7,8 @@ from . import ops
 
 
 class LayerNorm(nn.LayerNorm):
-    """nn.LayerNorm over the last axes.  float32, float16 and bfloat16 input; parameters in float32 or the input's type."""
+    """nn.LayerNorm over the last axes.  float32, float16 and bfloat16 input; parameters in float32 or the input's type.  The output has the input's
+    type, under autocast too (nn.LayerNorm returns float32 there): statistics and arithmetic are fp32 whatever the types."""
 
     def forward(self, x):
         n = len(self.normalized_shape)

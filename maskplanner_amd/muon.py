@@ -65,7 +65,8 @@ class Muon(torch.optim.Optimizer):
 
 class MuonAdam:
     """Muon for `matrices`, factor_heads.DenseAdam for `others`, as one optimizer with DenseAdam's interface (`step_dev`, `state`,
-    step(ticked))."""
+    step(ticked)).  Like DenseAdam it has no param_groups and no state_dict: rates are scheduled and momenta saved on `muon`, which is a
+    torch.optim.Optimizer; Adam's part is in `state` and `step_dev`."""
 
     def __init__(self, matrices, others, lr=1e-3, muon_lr=0.02, capturable=False, **muon):
         from .factor_heads import DenseAdam

@@ -208,3 +208,15 @@ def test_layer_norm_model_trained_by_muon_and_adam_in_one_loop():
     for (n, p), q in zip(net.named_parameters(), ref.parameters()):
         tol = 3 * 0.02 * 1.5 * 1e-3 if p.ndim > 1 else 3 * 1e-3 * 1e-2
         assert float((p.detach().double().cpu() - q.detach()).abs().max()) <= tol + 2.0 ** -22, n
+
+
+def test_layer_norm_module_keeps_the_input_type_under_autocast():
+    """the output has the input's type; its values are those of the same numbers in float32, rounded (2^-11), each of the two within 160 roundings of
+    2^-24 (1 + max|x| / std) <= 10 of the exact one"""
+    from maskplanner_amd.layer_norm import LayerNorm
+    m = LayerNorm(300).cuda()
+    x = (3 + torch.randn(50, 300, device="cuda", generator=gen(1))).half()
+    with torch.autocast("cuda", dtype=torch.float16):
+        y, z = m(x), m(x.float())
+    assert y.dtype == torch.float16 and z.dtype == torch.float32 and torch.equal(z, m(x.float()))
+    assert ((y.float() - z).abs() <= 2.0 ** -11 * z.abs() + 2 * 160 * 2.0 ** -24 * 10).all()
