@@ -1226,7 +1226,7 @@ float x_room(const Bounds& b, int steps)        // (x_shift)
 //   fp32: two from n = 2 m and m = 256 on (it saves a fifth there; nearer to square less than 15 %, in small matrices nothing, and the error
 //         grows: 128 x 131: 2.6e-6 of the exact result against 1.4e-6 step by step, 70 x 600: 2.5e-6 against 1.6e-6);
 //   bf16: 2^-22 g^(h-1) <= 5e-3, five steps (worst case measured 6e-4, a matrix dominated by one direction; the result's rounding: 1.7e-3);
-//   fp16: 2^-22 g^(h-1) <= 5e-5, three steps (the rounding: 2e-4).
+//   fp16: 2^-22 g^(h-1) <= 5e-5, three steps (worst case measured 1e-4, rank one; the rounding: 2e-4).
 // Of one limit for the whole chunk the cheapest is taken: the work, and 6.5 us for each launch of the matrix that has most of them.
 bool hops_in_f32(const Shape& s) { return s.m >= 256 && s.n >= 2 * s.m; }
 
