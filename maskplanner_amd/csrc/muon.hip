@@ -681,8 +681,8 @@ __device__ __forceinline__ void put_plane(_Float16* img, int row, int nchunk, in
     *reinterpret_cast<half4*>(img + ((size_t)row * nchunk + (col >> 5)) * 32 + (col & 31)) = h;
 }
 
-// A norm far below eps: X stays small through all steps, and planes scaled for |X| ~ 1 would lose it in fp16's subnormals (a norm of 1e-7 eps:
-// 3e-4 of the result, 1e-11 eps: all of it).  Behind the first hop the planes hold X t, t the largest power of two (one at least) that keeps
+// A norm far below eps: X stays small through all steps, and planes scaled for |X| ~ 1 would lose it in fp16's subnormals (a norm of 5e-8 eps:
+// 3e-4 of the result, 5e-12 eps: all of it).  Behind the first hop the planes hold X t, t the largest power of two (one at least) that keeps
 // |X| t within the planes' bound in every step: x_room = that bound / the largest product of |Q|, which is what |X| grows by.
 __device__ __forceinline__ double x_shift(double norm, double denom, float x_room)
 {
